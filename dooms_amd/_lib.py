@@ -1,4 +1,4 @@
-"""ctypes binding of libmx_attn.so (the C ABI in include/mx_attn.h).
+"""ctypes binding of libmx_attn.so (the C ABI in include/mx_attn.h, mx_linear.h and mx_paged.h).
 
 This is the binding a Python caller of the C ABI would add; it mirrors the reference's own ctypes layer for its C API
 (python/dooms/_lib.py:113-229 in dooms.cpp 0.6.1): load the library, declare argument types, turn a non-zero code into
@@ -19,13 +19,14 @@ INTERNAL = 7
 CODE_NAMES = {OK: "OK", INVALID_ARGUMENT: "INVALID_ARGUMENT", UNSUPPORTED: "UNSUPPORTED",
               RESOURCE_EXHAUSTED: "RESOURCE_EXHAUSTED", INTERNAL: "INTERNAL"}
 
-# Every symbol include/mx_attn.h declares.
+# Every symbol the headers in include/ declare.
 EXPORTS = ("mx_attn_abi_version", "mx_attn_last_error", "mx_attn_prefill", "mx_attn_prefill_ws",
            "mx_attn_prefill_workspace_bytes", "mx_attn_prefill_rope", "mx_attn_prefill_rope_ws", "mx_attn_decode",
            "mx_attn_decode_f32", "mx_attn_decode_noalloc", "mx_attn_decode_rope", "mx_linear", "mx_linear_workspace_bytes",
            "mx_linear_call_workspace_bytes",
            "mx_attn_decode_workspace_bytes", "mx_attn_decode_workspace_init", "mx_self_attention",
-           "mx_self_attention_workspace_bytes")
+           "mx_self_attention_workspace_bytes", "mx_paged_store", "mx_paged_decode", "mx_paged_decode_workspace_bytes",
+           "mx_paged_prefill", "mx_paged_prefill_workspace_bytes")
 
 ROPE_NORMAL = 0  # adjacent pairs (2i, 2i + 1): llama
 ROPE_NEOX = 1    # split halves (i, i + head_dim / 2): qwen2
@@ -66,6 +67,23 @@ class MxSelfAttnDesc(ctypes.Structure):
     _fields_ = [("batch", ctypes.c_int32), ("n_tok", ctypes.c_int32), ("heads", ctypes.c_int32),
                 ("embed", ctypes.c_int32), ("dtype", ctypes.c_int32), ("scale", ctypes.c_float),
                 ("tuning", ctypes.POINTER(MxAttnTuning))]
+
+
+PAGED_MAX_AXES = 4  # MX_PAGED_MAX_AXES
+
+
+class MxPagedDesc(ctypes.Structure):
+    """mx_paged_desc (include/mx_paged.h)."""
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "n_head", "n_head_kv", "head_dim", "dtype", "row_dtype", "n_seq", "n_rows", "causal", "page_size", "n_pages", "max_pages",
+        "max_q", "max_kv_len", "reserved")] + [(n, ctypes.c_int64) for n in (
+            "page_stride", "kv_stride", "head_stride", "table_stride", "row_stride", "out_stride")] + [("scale", ctypes.c_float)]
+
+
+class MxPagedRope(ctypes.Structure):
+    """mx_paged_rope (include/mx_paged.h)."""
+    _fields_ = [("mode", ctypes.c_int32), ("n_axes", ctypes.c_int32), ("axis_pairs", ctypes.c_int32 * PAGED_MAX_AXES),
+                ("axis_restart", ctypes.c_int32), ("reserved", ctypes.c_int32), ("base", ctypes.c_double)]
 
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
@@ -133,6 +151,16 @@ def lib() -> ctypes.CDLL:
         L.mx_self_attention_workspace_bytes.argtypes = [ctypes.POINTER(MxSelfAttnDesc)]
         L.mx_self_attention.restype = ctypes.c_int32
         L.mx_self_attention.argtypes = [ctypes.POINTER(MxSelfAttnDesc), P, P, P, ctypes.c_size_t, P]
+        desc, rope = ctypes.POINTER(MxPagedDesc), ctypes.POINTER(MxPagedRope)
+        L.mx_paged_store.restype = ctypes.c_int32
+        L.mx_paged_store.argtypes = [desc, rope, P, P, P, P, P, P, P, P, P]
+        L.mx_paged_decode.restype = ctypes.c_int32
+        L.mx_paged_decode.argtypes = [desc, P, P, P, P, P, P, P, P, ctypes.c_size_t, P]
+        L.mx_paged_prefill.restype = ctypes.c_int32
+        L.mx_paged_prefill.argtypes = [desc, P, P, P, P, P, P, P, P, P, ctypes.c_size_t, P]
+        for f in (L.mx_paged_decode_workspace_bytes, L.mx_paged_prefill_workspace_bytes):
+            f.restype = ctypes.c_size_t
+            f.argtypes = [desc]
         _lib = L
     return _lib
 
@@ -276,3 +304,40 @@ def self_attention_raw(desc: MxSelfAttnDesc, qkv: int, y: int, ws: int, ws_bytes
     """mx_self_attention on raw device addresses; returns the code."""
     return lib().mx_self_attention(ctypes.byref(desc), qkv, y, ws or None, ws_bytes, stream or None)
 
+
+
+def make_paged_rope(mode: int, base: float, axis_pairs, axis_restart: bool) -> MxPagedRope:
+    pairs = list(axis_pairs)
+    if len(pairs) > PAGED_MAX_AXES:
+        raise ValueError(f"at most {PAGED_MAX_AXES} position axes")
+    return MxPagedRope(mode=mode, n_axes=len(pairs), axis_pairs=(ctypes.c_int32 * PAGED_MAX_AXES)(*pairs),
+                       axis_restart=1 if axis_restart else 0, base=base)
+
+
+def paged_store_raw(desc: MxPagedDesc, rope: MxPagedRope, qkv: int, positions: int, k: int, v: int, table: int, kv_len: int,
+                    cu_q: int, q_out: int, stream: int) -> int:
+    """mx_paged_store on raw device addresses; returns the code."""
+    return lib().mx_paged_store(ctypes.byref(desc), ctypes.byref(rope), qkv or None, positions or None, k or None, v or None,
+                                table or None, kv_len or None, cu_q or None, q_out or None, stream or None)
+
+
+def paged_decode_raw(desc: MxPagedDesc, q: int, k: int, v: int, table: int, kv_len: int, out: int, lse: int, ws: int,
+                     ws_bytes: int, stream: int) -> int:
+    """mx_paged_decode on raw device addresses; returns the code."""
+    return lib().mx_paged_decode(ctypes.byref(desc), q or None, k or None, v or None, table or None, kv_len or None, out or None,
+                                 lse or None, ws or None, ws_bytes, stream or None)
+
+
+def paged_prefill_raw(desc: MxPagedDesc, q: int, k: int, v: int, table: int, kv_len: int, cu_q: int, out: int, lse: int, ws: int,
+                      ws_bytes: int, stream: int) -> int:
+    """mx_paged_prefill on raw device addresses; returns the code."""
+    return lib().mx_paged_prefill(ctypes.byref(desc), q or None, k or None, v or None, table or None, kv_len or None, cu_q or None,
+                                  out or None, lse or None, ws or None, ws_bytes, stream or None)
+
+
+def paged_decode_workspace_bytes(desc: MxPagedDesc) -> int:
+    return lib().mx_paged_decode_workspace_bytes(ctypes.byref(desc))
+
+
+def paged_prefill_workspace_bytes(desc: MxPagedDesc) -> int:
+    return lib().mx_paged_prefill_workspace_bytes(ctypes.byref(desc))

@@ -71,6 +71,9 @@ def _native():
                          "mx_attn_prefill_ws", "mx_attn_decode", "mx_attn_decode_f32", "mx_attn_decode_rope",
                          "mx_attn_prefill_rope_ws", "mx_linear_call_workspace_bytes", "mx_linear",
                          "mx_self_attention_workspace_bytes", "mx_self_attention")])
+            ext.bind_paged(L.mx_attn_abi_version(), tuple(ctypes.sizeof(t) for t in (_lib.MxPagedDesc, _lib.MxPagedRope)),
+                           *[ctypes.cast(getattr(L, f), ctypes.c_void_p).value
+                             for f in ("mx_paged_store", "mx_paged_decode", "mx_paged_prefill")])
         _ext = ext   # before _bound: another thread that finds the library bound finds the extension too
         _bound = L
     return _ext
@@ -329,3 +332,166 @@ def self_attention(qkv, *, heads, scale=None, out=None, tuning=None):
     _lib.check(_lib.self_attention_raw(d, qkv.data_ptr(), out.data_ptr(), ws.data_ptr() if ws is not None else 0,
                                        nbytes, _stream()))
     return out
+
+
+# ---- the paged cache ----
+
+_PAGE_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+
+
+def _paged_desc(rows, k_pages, v_pages, page_table, kv_len, cu_q, n_head, max_q=None, max_kv_len=None):
+    """The checked cache of a paged call as a descriptor (its rows' and outputs' types and strides are the caller's). Every
+    tensor has to be on the device of `rows`."""
+    for t, name in ((rows, "rows"), (k_pages, "k_pages"), (v_pages, "v_pages"), (page_table, "page_table"), (kv_len, "kv_len"),
+                    (cu_q, "cu_q")):
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a device tensor")
+        if t.device != rows.device:
+            raise ValueError(f"{name} is on {t.device}, the rows on {rows.device}")
+    if k_pages.dim() != 4 or k_pages.stride(3) != 1 or k_pages.dtype not in _PAGE_DTYPES:
+        raise ValueError("k_pages must be a float16 or bfloat16 [pages][page size][kv heads][head dim] tensor with unit stride along "
+                         "the head dim")
+    if v_pages.shape != k_pages.shape or v_pages.stride() != k_pages.stride() or v_pages.dtype != k_pages.dtype:
+        raise ValueError("v_pages must have the shape, strides and type of k_pages")
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
+        raise ValueError("page_table must be an int32 [sequences][pages] tensor with unit stride along the pages")
+    n_seq = page_table.shape[0]
+    if kv_len.dtype != torch.int32 or kv_len.shape != (n_seq,) or not kv_len.is_contiguous():
+        raise ValueError("kv_len must be a contiguous int32 tensor with an entry per sequence")
+    if cu_q is not None and (cu_q.dtype != torch.int32 or cu_q.shape != (n_seq + 1,) or not cu_q.is_contiguous()):
+        raise ValueError("cu_q must be a contiguous int32 tensor of one entry more than sequences")
+    n_pages, page_size, n_head_kv, head_dim = k_pages.shape
+    return _lib.MxPagedDesc(n_head=n_head, n_head_kv=n_head_kv, head_dim=head_dim, dtype=_PAGE_DTYPES[k_pages.dtype], n_seq=n_seq,
+                            n_rows=rows.shape[0], page_size=page_size, n_pages=n_pages, max_pages=page_table.shape[1],
+                            max_q=max_q or 0, max_kv_len=max_kv_len or 0, page_stride=k_pages.stride(0),
+                            kv_stride=k_pages.stride(1), head_stride=k_pages.stride(2),
+                            table_stride=max(page_table.stride(0), page_table.shape[1]), row_stride=rows.stride(0))
+
+
+def paged_store(qkv, k_pages, v_pages, page_table, kv_len, *, n_head, rope_mode, rope_base=10000.0, cu_q=None, positions=None,
+                axis_pairs=None, axis_restart=False, q=None, want_q=True):
+    """mx_paged_store, the append of a step's new tokens: qkv (f32, f16 or bf16) [rows][>= (n_head + 2 n_head_kv) hd] unrotated
+    rows, each sequence's new tokens as cu_q has them (None: equally many each); kv_len counts them already. Their rotated keys
+    and their values go into k_pages / v_pages ([pages][page size][kv heads][hd], f16 or bf16, any strides but the last). Returns
+    the rotated queries, [rows][n_head hd] of the pages' type (None without want_q). positions: int32 [axes][rows] or [rows]
+    (None: the cache positions); axis_pairs: rotary pairs of each axis (None: one axis); axis_restart: each axis has a frequency
+    ladder of its own."""
+    r = _native().paged_store(qkv, k_pages, v_pages, page_table, kv_len, n_head, rope_mode, rope_base, cu_q, positions, axis_pairs,
+                              axis_restart, q, want_q)
+    if r is not None:
+        return _result(r)
+    if qkv.dtype not in _SA_DTYPES:
+        raise ValueError("qkv must be float32, float16 or bfloat16")
+    _rows(qkv, "qkv", qkv.dtype)
+    d = _paged_desc(qkv, k_pages, v_pages, page_table, kv_len, cu_q, n_head)
+    d.row_dtype = _SA_DTYPES[qkv.dtype]
+    if qkv.shape[1] < (n_head + 2 * d.n_head_kv) * d.head_dim:
+        raise ValueError("qkv must be [rows][>= (n_head + 2 n_head_kv) head_dim]")
+    rope = _lib.make_paged_rope(rope_mode, rope_base, (d.head_dim // 2,) if axis_pairs is None else axis_pairs, axis_restart)
+    if positions is not None:
+        if positions.device != qkv.device or positions.dtype != torch.int32 or not positions.is_contiguous():
+            raise ValueError("positions must be a contiguous int32 tensor on the rows' device")
+        if tuple(positions.shape) != (rope.n_axes, d.n_rows) and not (rope.n_axes == 1 and tuple(positions.shape) == (d.n_rows,)):
+            raise ValueError("positions must be [axes][rows]")
+    if want_q and q is None:
+        q = torch.empty(d.n_rows, n_head * d.head_dim, dtype=k_pages.dtype, device=qkv.device)
+    if q is not None:
+        _out_rows(q, "q", k_pages.dtype, d, qkv)
+        d.out_stride = q.stride(0)
+    with torch.cuda.device(qkv.device):
+        _lib.check(_lib.paged_store_raw(d, rope, qkv.data_ptr(), _ptr(positions), k_pages.data_ptr(), v_pages.data_ptr(),
+                                        page_table.data_ptr(), kv_len.data_ptr(), _ptr(cu_q), _ptr(q), _stream()))
+    return q
+
+
+def _ptr(t) -> int:
+    return t.data_ptr() if t is not None else 0
+
+
+def _out_rows(out, name, dtype, d, like):
+    _rows(out, name, dtype)
+    if out.device != like.device or out.shape[0] < d.n_rows or out.shape[1] < d.n_head * d.head_dim:
+        raise ValueError(f"{name} must be [rows][>= n_head * head_dim] on the rows' device")
+
+
+def _paged_attend(q, k_pages, v_pages, page_table, kv_len, cu_q, n_head, causal, scale, out, out_dtype, lse, want_lse, max_q,
+                  max_kv_len, workspace, call, nbytes):
+    _rows(q, "q", k_pages.dtype)
+    d = _paged_desc(q, k_pages, v_pages, page_table, kv_len, cu_q, n_head, max_q, max_kv_len)
+    if q.shape[1] < n_head * d.head_dim:
+        raise ValueError("q must be [rows][>= n_head * head_dim]")
+    if out_dtype is None:
+        out_dtype = q.dtype if out is None else out.dtype
+    if out_dtype not in (q.dtype, torch.float32):
+        raise ValueError(f"the output must be {q.dtype} or float32")
+    if out is None:
+        out = torch.empty(d.n_rows, n_head * d.head_dim, dtype=out_dtype, device=q.device)
+    _out_rows(out, "out", out_dtype, d, q)
+    if want_lse and lse is None:
+        lse = torch.empty(d.n_rows, n_head, dtype=torch.float32, device=q.device)
+    if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous() or tuple(lse.shape) != (d.n_rows, n_head) or
+                            lse.device != q.device):
+        raise ValueError("lse must be a contiguous float32 [rows][n_head] tensor on the rows' device")
+    d.row_dtype = _SA_DTYPES[out_dtype]
+    d.causal = 1 if causal else 0
+    d.scale = 1.0 / math.sqrt(d.head_dim) if scale is None else scale
+    d.out_stride = out.stride(0)
+    with torch.cuda.device(q.device):
+        if workspace is None:
+            need = nbytes(d)  # 0 also for an invalid descriptor, which the call reports
+            workspace = new_workspace(need, q.device) if need else torch.empty(0, dtype=torch.uint8, device=q.device)
+        elif workspace.device != q.device or not workspace.is_contiguous():
+            raise ValueError("workspace must be a contiguous tensor on the rows' device")
+        rest = (out.data_ptr(), _ptr(lse), workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream())
+        _lib.check(call(d, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), kv_len.data_ptr(),
+                        *(() if cu_q is None else (cu_q.data_ptr(),)), *rest))
+    return out, lse
+
+
+def paged_decode(q, k_pages, v_pages, page_table, kv_len, *, n_head, n_q=1, causal=True, scale=None, out=None, out_dtype=None, lse=None,
+                 want_lse=False, max_kv_len=None, workspace=None):
+    """mx_paged_decode: q [sequences * n_q][>= n_head hd], the n_q new rows of each sequence (rotated, of the pages' type), over
+    its kv_len[b] keys in k_pages / v_pages; page_table int32 [sequences][pages] and kv_len int32 on the device. With causal, row
+    t of the n_q sees the keys up to kv_len - n_q + t. max_kv_len: a length that no sequence is expected to pass, for the plan. The
+    output has the pages' type or out_dtype=torch.float32; workspace: paged_decode_workspace_bytes from new_workspace, kept by
+    the caller (None: made for this call). Returns (out, lse or None)."""
+    if q.dim() == 2 and page_table.dim() == 2 and q.shape[0] != page_table.shape[0] * n_q:
+        raise ValueError(f"q has {q.shape[0]} rows, not {n_q} for each of {page_table.shape[0]} sequences")
+    if workspace is not None:
+        r = _native().paged_attend(q, k_pages, v_pages, page_table, kv_len, None, n_head, causal, scale, out, out_dtype, lse, want_lse,
+                                   None, max_kv_len, workspace)
+        if r is not None:
+            return _result(r)
+    return _paged_attend(q, k_pages, v_pages, page_table, kv_len, None, n_head, causal, scale, out, out_dtype, lse, want_lse, None,
+                         max_kv_len, workspace, _lib.paged_decode_raw, _lib.paged_decode_workspace_bytes)
+
+
+def paged_prefill(q, k_pages, v_pages, page_table, kv_len, cu_q, *, n_head, causal=True, scale=None, out=None, out_dtype=None,
+                  lse=None, want_lse=False, max_q=None, max_kv_len=None, workspace=None):
+    """mx_paged_prefill: packed prompts, rows cu_q[b] .. cu_q[b + 1] - 1 (cu_q int32 on the device) the last of sequence b's
+    kv_len[b] keys, which the pages hold already. max_q: the most rows of a sequence, for the plan. Everything else as
+    paged_decode (workspace: paged_prefill_workspace_bytes)."""
+    if workspace is not None:
+        r = _native().paged_attend(q, k_pages, v_pages, page_table, kv_len, cu_q, n_head, causal, scale, out, out_dtype, lse, want_lse,
+                                   max_q, max_kv_len, workspace)
+        if r is not None:
+            return _result(r)
+    if cu_q is None:
+        raise ValueError("cu_q must be given")
+    return _paged_attend(q, k_pages, v_pages, page_table, kv_len, cu_q, n_head, causal, scale, out, out_dtype, lse, want_lse, max_q,
+                         max_kv_len, workspace, _lib.paged_prefill_raw, _lib.paged_prefill_workspace_bytes)
+
+
+def paged_decode_workspace_bytes(*, n_head, n_head_kv, head_dim, n_q, n_seq, max_kv_len) -> int:
+    """Bytes of a workspace for paged_decode of n_seq sequences of n_q rows and at most max_kv_len keys."""
+    return _lib.paged_decode_workspace_bytes(_lib.MxPagedDesc(
+        n_head=n_head, n_head_kv=n_head_kv, head_dim=head_dim, dtype=_lib.DTYPE_F16, n_seq=n_seq, n_rows=n_seq * n_q, max_kv_len=max_kv_len))
+
+
+def paged_prefill_workspace_bytes(*, n_head, n_head_kv, head_dim, n_rows, n_seq, max_q, max_kv_len) -> int:
+    """Bytes of a workspace for paged_prefill of n_rows rows of n_seq sequences, at most max_q rows and max_kv_len keys each."""
+    return _lib.paged_prefill_workspace_bytes(_lib.MxPagedDesc(
+        n_head=n_head, n_head_kv=n_head_kv, head_dim=head_dim, dtype=_lib.DTYPE_F16, n_seq=n_seq, n_rows=n_rows, max_q=max_q,
+        max_kv_len=max_kv_len))

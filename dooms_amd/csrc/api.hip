@@ -19,6 +19,7 @@
 #include <string>
 
 #include "linear_plan.hpp"
+#include "mx_host.hpp"
 #include "mx_kernels.hpp"
 
 namespace {
@@ -860,6 +861,11 @@ int32_t linear_params(const mx_linear_desc * desc, int32_t count, const uint16_t
 }
 
 }  // namespace
+
+int32_t mx::set_error(int32_t code, const char * message) {
+    g_last_error = message;
+    return code;
+}
 
 extern "C" {
 

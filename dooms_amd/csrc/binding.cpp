@@ -13,7 +13,9 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <climits>
@@ -22,6 +24,7 @@
 
 #include "mx_attn.h"
 #include "mx_linear.h"
+#include "mx_paged.h"
 
 namespace {
 
@@ -35,6 +38,9 @@ struct Api {
     decltype(&mx_linear) linear = nullptr;
     decltype(&mx_self_attention_workspace_bytes) self_attention_workspace_bytes = nullptr;
     decltype(&mx_self_attention) self_attention = nullptr;
+    decltype(&mx_paged_store) paged_store = nullptr;
+    decltype(&mx_paged_decode) paged_decode = nullptr;
+    decltype(&mx_paged_prefill) paged_prefill = nullptr;
 };
 Api api;
 
@@ -373,6 +379,137 @@ PyObject * self_attention(PyObject * const * a) {
     return a[3] != Py_None ? Py_NewRef(a[3]) : THPVariable_Wrap(out);
 }
 
+int32_t element(at::ScalarType t) { return t == at::kFloat ? MX_ATTN_F32 : t == at::kHalf ? MX_ATTN_F16 : MX_ATTN_BF16; }
+
+// The paged calls' device metadata: a contiguous int32 tensor of one dimension and n entries on like's device.
+const at::Tensor & ints(PyObject * o, int64_t n, const at::Tensor & like) {
+    const at::Tensor & t = tensor(o);
+    need(t.scalar_type() == at::kInt && t.device() == like.device() && t.dim() == 1 && t.size(0) == n && t.is_contiguous());
+    return t;
+}
+
+// k_pages, v_pages, page_table, kv_len at a; the rows' and outputs' types and strides are the caller's.
+struct Paged {
+    mx_paged_desc d{};
+    const at::Tensor &k, &v, &table, &len;
+    at::ScalarType type;
+    Paged(PyObject * const * a, const at::Tensor & rows, PyObject * n_head)
+        : k(tensor(a[0])), v(tensor(a[1])), table(tensor(a[2])), len(ints(a[3], table.dim() == 2 ? table.size(0) : -1, rows)) {
+        type = k.scalar_type();
+        need(rows.is_cuda() && k.device() == rows.device() && v.device() == rows.device() && table.device() == rows.device());
+        need(k.dim() == 4 && k.stride(3) == 1 && (type == at::kHalf || type == at::kBFloat16));
+        need(v.scalar_type() == type && v.sizes() == k.sizes() && v.strides() == k.strides());
+        need(table.scalar_type() == at::kInt && (table.stride(1) == 1 || table.size(1) <= 1));
+        for (int64_t n : {k.size(0), k.size(1), k.size(2), k.size(3), table.size(0), table.size(1), rows.size(0)}) need(n <= INT32_MAX);
+        d.n_head = int32(n_head);
+        d.n_head_kv = (int32_t)k.size(2);
+        d.head_dim = (int32_t)k.size(3);
+        need(d.head_dim > 0 && d.n_head > 0);
+        d.dtype = element(type);
+        d.n_seq = (int32_t)table.size(0);
+        d.n_rows = (int32_t)rows.size(0);
+        d.page_size = (int32_t)k.size(1);
+        d.n_pages = (int32_t)k.size(0);
+        d.max_pages = (int32_t)table.size(1);
+        d.page_stride = k.stride(0);
+        d.kv_stride = k.stride(1);
+        d.head_stride = k.stride(2);
+        d.table_stride = std::max(table.stride(0), table.size(1));
+        d.row_stride = rows.stride(0);
+    }
+    // the caller's rows of the output (checked) or new ones
+    at::Tensor out(PyObject * o, at::ScalarType t, const at::Tensor & like) {
+        const int64_t width = (int64_t)d.n_head * d.head_dim;
+        const at::Tensor r = rows_or_new(o, d.n_rows, width, t, like);
+        need(r.device() == like.device() && r.size(0) >= d.n_rows && r.size(1) >= width);
+        d.out_stride = r.stride(0);
+        return r;
+    }
+};
+
+// qkv, k_pages, v_pages, page_table, kv_len, n_head, rope_mode, rope_base, cu_q, positions, axis_pairs, axis_restart, q, want_q
+PyObject * paged_store(PyObject * const * a) {
+    const at::Tensor & x0 = tensor(a[0]);
+    const at::ScalarType t = x0.scalar_type();
+    need(t == at::kFloat || t == at::kHalf || t == at::kBFloat16);
+    const at::Tensor & x = rows(a[0], t);
+    Paged c(a + 1, x, a[5]);
+    c.d.row_dtype = element(t);
+    need(x.size(1) >= ((int64_t)c.d.n_head + 2 * (int64_t)c.d.n_head_kv) * c.d.head_dim);
+    const int32_t * cu = a[8] == Py_None ? nullptr : data<int32_t>(ints(a[8], c.d.n_seq + 1, x));
+    mx_paged_rope r{};
+    r.mode = int32(a[6]);
+    r.base = real(a[7]);
+    r.axis_restart = truth(a[11]);
+    r.n_axes = 1;
+    r.axis_pairs[0] = c.d.head_dim / 2;
+    if (a[10] != Py_None) {
+        const auto pairs = items(a[10]);
+        need(!pairs.empty() && pairs.size() <= MX_PAGED_MAX_AXES);
+        r.n_axes = (int32_t)pairs.size();
+        for (size_t i = 0; i < pairs.size(); i++) r.axis_pairs[i] = int32(pairs[i]);
+    }
+    const int32_t * pos = nullptr;
+    if (a[9] != Py_None) {
+        const at::Tensor & p = tensor(a[9]);
+        need(p.scalar_type() == at::kInt && p.device() == x.device() && p.is_contiguous());
+        need((p.dim() == 2 && p.size(0) == r.n_axes && p.size(1) == c.d.n_rows) || (p.dim() == 1 && r.n_axes == 1 && p.size(0) == c.d.n_rows));
+        pos = data<int32_t>(p);
+    }
+    const c10::DeviceGuard guard(x.device());
+    need(a[12] != Py_None || truth(a[13]));  // without queries the result is None, which would ask for the general path
+    const at::Tensor q = c.out(a[12], c.type, x);
+    int32_t rc;
+    {
+        Unlocked u;
+        rc = api.paged_store(&c.d, &r, x.data_ptr(), pos, c.k.data_ptr(), c.v.data_ptr(), data<int32_t>(c.table), data<int32_t>(c.len),
+                             cu, q.data_ptr(), stream());
+    }
+    if (rc) return code(rc);
+    if (a[12] != Py_None) return Py_NewRef(a[12]);
+    return THPVariable_Wrap(q);
+}
+
+// q, k_pages, v_pages, page_table, kv_len, cu_q (None: as many rows for each sequence), n_head, causal, scale, out, out_dtype, lse,
+// want_lse, max_q, max_kv_len, workspace
+PyObject * paged_attend(PyObject * const * a) {
+    const at::Tensor & q0 = tensor(a[0]);
+    const at::Tensor & q = rows(a[0], q0.scalar_type());
+    Paged c(a + 1, q, a[6]);
+    mx_paged_desc & d = c.d;
+    need(q.scalar_type() == c.type && q.size(1) >= (int64_t)d.n_head * d.head_dim);
+    const int32_t * cu = a[5] == Py_None ? nullptr : data<int32_t>(ints(a[5], d.n_seq + 1, q));
+    at::ScalarType t = a[9] == Py_None ? c.type : tensor(a[9]).scalar_type();
+    if (a[10] != Py_None) {
+        need(THPDtype_Check(a[10]));
+        t = reinterpret_cast<THPDtype *>(a[10])->scalar_type;
+    }
+    need(t == c.type || t == at::kFloat);
+    d.row_dtype = element(t);
+    d.causal = truth(a[7]);
+    d.scale = a[8] == Py_None ? (float)(1.0 / std::sqrt((double)d.head_dim)) : (float)real(a[8]);
+    d.max_q = a[13] == Py_None ? 0 : int32(a[13]);
+    d.max_kv_len = a[14] == Py_None ? 0 : int32(a[14]);
+    const at::Tensor & ws = tensor(a[15]);
+    need(ws.device() == q.device() && ws.is_contiguous());
+    const c10::DeviceGuard guard(q.device());
+    const at::Tensor out = c.out(a[9], t, q);
+    const at::Tensor lse = lse_or_new(a[11], a[12], d.n_rows, d.n_head, q);
+    if (lse.defined())
+        need(lse.scalar_type() == at::kFloat && lse.device() == q.device() && lse.dim() == 2 && lse.size(0) == d.n_rows &&
+             lse.size(1) == d.n_head && lse.is_contiguous());
+    float * l = lse.defined() ? data<float>(lse) : nullptr;
+    int32_t rc;
+    {
+        Unlocked u;
+        rc = cu ? api.paged_prefill(&d, q.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), data<int32_t>(c.table), data<int32_t>(c.len), cu,
+                                    out.data_ptr(), l, ws.data_ptr(), (size_t)ws.nbytes(), stream())
+                : api.paged_decode(&d, q.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), data<int32_t>(c.table), data<int32_t>(c.len),
+                                   out.data_ptr(), l, ws.data_ptr(), (size_t)ws.nbytes(), stream());
+    }
+    return rc ? code(rc) : pair(out, a[9], lse, a[11]);
+}
+
 template <PyObject * (*F)(PyObject * const *), Py_ssize_t N>
 PyObject * entry(PyObject *, PyObject * const * args, Py_ssize_t n) {
     if (n != N) {
@@ -422,11 +559,31 @@ PyObject * bind(PyObject *, PyObject * args) {
     Py_RETURN_NONE;
 }
 
+// bind_paged(version, (sizes of mx_paged_desc, mx_paged_rope), addresses of mx_paged_store, _decode, _prefill): as bind.
+PyObject * bind_paged(PyObject *, PyObject * args) {
+    int version;
+    Py_ssize_t desc, rope;
+    unsigned long long p[3];
+    if (!PyArg_ParseTuple(args, "i(nn)KKK", &version, &desc, &rope, p, p + 1, p + 2)) return nullptr;
+    if (version != MX_ATTN_ABI_VERSION || (size_t)desc != sizeof(mx_paged_desc) || (size_t)rope != sizeof(mx_paged_rope)) {
+        PyErr_SetString(PyExc_ImportError, "dooms_amd._native was built for other paged descriptors: build both with `python -m dooms_amd.build`");
+        return nullptr;
+    }
+    auto set = [](auto & f, unsigned long long v) {
+        f = reinterpret_cast<std::remove_reference_t<decltype(f)>>((uintptr_t)v);
+    };
+    set(api.paged_store, p[0]);
+    set(api.paged_decode, p[1]);
+    set(api.paged_prefill, p[2]);
+    Py_RETURN_NONE;
+}
+
 #define MX_ENTRY(name, n) \
     {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(entry<name, n>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     MX_ENTRY(decode, 14), MX_ENTRY(decode_rope, 14), MX_ENTRY(prefill, 14), MX_ENTRY(prefill_rope, 16), MX_ENTRY(linear, 8),
-    MX_ENTRY(self_attention, 4), {"bind", bind, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
+    MX_ENTRY(self_attention, 4), MX_ENTRY(paged_store, 14), MX_ENTRY(paged_attend, 16),
+    {"bind_paged", bind_paged, METH_VARARGS, nullptr}, {"bind", bind, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

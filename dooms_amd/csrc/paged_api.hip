@@ -1,0 +1,352 @@
+// C ABI of the paged cache (include/mx_paged.h): argument checks, launch plans. As in api.hip, every check of host arguments
+// runs before anything is enqueued, and nothing here aborts or throws.
+#include "mx_paged.h"
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+
+#include "mx_host.hpp"
+#include "mx_paged.hpp"
+
+namespace {
+
+int32_t fail(int32_t code, const char * fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    std::vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    return mx::set_error(code, buf);
+}
+
+bool aligned(const void * p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// What every call and the workspace sizes need.
+int32_t check_shape(const mx_paged_desc * d) {
+    if (!d) return fail(MX_ATTN_INVALID_ARGUMENT, "desc is null");
+    if (d->reserved != 0) return fail(MX_ATTN_INVALID_ARGUMENT, "desc->reserved must be 0");
+    if (d->n_head < 1 || d->n_head_kv < 1)
+        return fail(MX_ATTN_INVALID_ARGUMENT, "n_head (%d) and n_head_kv (%d) must be >= 1", d->n_head, d->n_head_kv);
+    if (d->n_head % d->n_head_kv != 0)
+        return fail(MX_ATTN_INVALID_ARGUMENT, "n_head (%d) is not a multiple of n_head_kv (%d)", d->n_head, d->n_head_kv);
+    if (d->n_head > 65535) return fail(MX_ATTN_UNSUPPORTED, "n_head (%d) beyond 65535", d->n_head);
+    if (d->head_dim != 64 && d->head_dim != 128 && d->head_dim != 256)
+        return fail(MX_ATTN_UNSUPPORTED, "head_dim %d is not supported with pages (64, 128 or 256)", d->head_dim);
+    if (d->dtype != MX_ATTN_F16 && d->dtype != MX_ATTN_BF16)
+        return fail(MX_ATTN_INVALID_ARGUMENT, "dtype (%d) must be MX_ATTN_F16 or MX_ATTN_BF16", d->dtype);
+    if (d->n_seq < 0 || d->n_seq > 65535) return fail(MX_ATTN_INVALID_ARGUMENT, "n_seq (%d) must be in [0, 65535]", d->n_seq);
+    if (d->n_rows < 0) return fail(MX_ATTN_INVALID_ARGUMENT, "n_rows (%d) must be >= 0", d->n_rows);
+    if (d->max_q < 0 || d->max_kv_len < 0)
+        return fail(MX_ATTN_INVALID_ARGUMENT, "max_q (%d) and max_kv_len (%d) must be >= 0", d->max_q, d->max_kv_len);
+    return MX_ATTN_OK;
+}
+
+int32_t check_uniform(const mx_paged_desc & d) {
+    if (d.n_seq > 0 && d.n_rows % d.n_seq)
+        return fail(MX_ATTN_INVALID_ARGUMENT, "n_rows (%d) is not a multiple of n_seq (%d)", d.n_rows, d.n_seq);
+    if (d.n_seq == 0 && d.n_rows > 0) return fail(MX_ATTN_INVALID_ARGUMENT, "%d rows of no sequence", d.n_rows);
+    return MX_ATTN_OK;
+}
+
+// The pool, its strides and the table.
+int32_t check_cache(const mx_paged_desc & d) {
+    if (d.page_size < 16 || d.page_size > 65536 || (d.page_size & (d.page_size - 1)))
+        return fail(MX_ATTN_UNSUPPORTED, "page_size (%d) must be a power of two in [16, 65536]", d.page_size);
+    if (d.n_pages < 1 || d.max_pages < 1)
+        return fail(MX_ATTN_INVALID_ARGUMENT, "n_pages (%d) and max_pages (%d) must be >= 1", d.n_pages, d.max_pages);
+    if ((int64_t)d.max_pages * d.page_size > (int64_t)1 << 30)
+        return fail(MX_ATTN_UNSUPPORTED, "max_pages (%d) x page_size (%d) beyond 2^30 keys a sequence", d.max_pages, d.page_size);
+    if (d.table_stride < d.max_pages)
+        return fail(MX_ATTN_INVALID_ARGUMENT, "table_stride (%lld) < max_pages (%d)", (long long)d.table_stride, d.max_pages);
+    if (d.kv_stride > (int64_t)1 << 26)
+        return fail(MX_ATTN_UNSUPPORTED, "kv_stride (%lld) beyond 2^26 elements", (long long)d.kv_stride);
+    // (page, row, head) rows of head_dim elements apart from each other: by ascending stride, each stride covers what the
+    // smaller ones span
+    struct Dim {
+        int64_t stride, n;
+        const char * name;
+    } dim[3] = {{d.page_stride, d.n_pages, "page_stride"}, {d.kv_stride, d.page_size, "kv_stride"}, {d.head_stride, d.n_head_kv, "head_stride"}};
+    for (const Dim & x : dim)
+        if (x.stride < 0 || x.stride % 8 || x.stride > (int64_t)1 << 46)
+            return fail(MX_ATTN_INVALID_ARGUMENT, "%s (%lld) must be a multiple of 8 elements, >= 0", x.name, (long long)x.stride);
+    std::sort(dim, dim + 3, [](const Dim & a, const Dim & b) { return a.stride < b.stride; });
+    int64_t span = d.head_dim;
+    for (const Dim & x : dim) {
+        if (x.n == 1) continue;
+        if (x.stride < span)
+            return fail(MX_ATTN_INVALID_ARGUMENT, "%s (%lld) makes rows of the pool overlap (%lld elements lie below it)", x.name,
+                        (long long)x.stride, (long long)span);
+        if (x.stride > ((int64_t)1 << 62) / x.n) return fail(MX_ATTN_INVALID_ARGUMENT, "%s (%lld) is out of range", x.name, (long long)x.stride);
+        span += x.stride * (x.n - 1);
+    }
+    return MX_ATTN_OK;
+}
+
+mx::PagedCache cache_of(const mx_paged_desc & d, const void * k, const void * v, const int32_t * table, const int32_t * kv_len) {
+    mx::PagedCache c{};
+    c.k = static_cast<const uint16_t *>(k);
+    c.v = static_cast<const uint16_t *>(v);
+    c.table = table;
+    c.kv_len = kv_len;
+    c.page_stride = d.page_stride;
+    c.kv_stride = d.kv_stride;
+    c.head_stride = d.head_stride;
+    c.table_stride = d.table_stride;
+    c.n_seq = d.n_seq;
+    c.n_pages = d.n_pages;
+    c.page_shift = __builtin_ctz((unsigned)d.page_size);
+    c.capacity = d.max_pages << c.page_shift;
+    return c;
+}
+
+int32_t check_pointers(const void * k, const void * v, const int32_t * table, const int32_t * kv_len, const int32_t * cu_q) {
+    if (!k || !v || !table || !kv_len) return fail(MX_ATTN_INVALID_ARGUMENT, "k, v, table and kv_len must not be null");
+    if (!aligned(k, 16) || !aligned(v, 16)) return fail(MX_ATTN_INVALID_ARGUMENT, "k and v must be 16-byte aligned");
+    if (!aligned(table, 4) || !aligned(kv_len, 4) || !aligned(cu_q, 4))
+        return fail(MX_ATTN_INVALID_ARGUMENT, "table, kv_len and cu_q must be 4-byte aligned");
+    return MX_ATTN_OK;
+}
+
+int32_t check_rows(const char * name, int64_t stride, int64_t width, int unit) {
+    if (stride < width || stride % unit || stride > (int64_t)1 << 31)
+        return fail(MX_ATTN_INVALID_ARGUMENT, "%s (%lld) must be >= %lld, a multiple of %d and at most 2^31", name, (long long)stride,
+                    (long long)width, unit);
+    return MX_ATTN_OK;
+}
+
+// Checks of an attention call, and its parameters but for the plan.
+int32_t attn_params(const mx_paged_desc & d, const void * q, const void * k, const void * v, const int32_t * table,
+                    const int32_t * kv_len, const int32_t * cu_q, void * out, float * lse, mx::PagedAttnParams & p) {
+    if (d.row_dtype != d.dtype && d.row_dtype != MX_ATTN_F32)
+        return fail(MX_ATTN_INVALID_ARGUMENT, "row_dtype (%d) must be MX_ATTN_F32 or dtype (%d)", d.row_dtype, d.dtype);
+    if (d.causal != 0 && d.causal != 1) return fail(MX_ATTN_INVALID_ARGUMENT, "causal must be 0 or 1");
+    if (!std::isfinite(d.scale)) return fail(MX_ATTN_INVALID_ARGUMENT, "scale is not finite");
+    if (int32_t rc = check_cache(d)) return rc;
+    const int64_t wide = (int64_t)d.n_head * d.head_dim;
+    const bool out32 = d.row_dtype == MX_ATTN_F32;
+    if (int32_t rc = check_rows("row_stride", d.row_stride, wide, 8)) return rc;
+    if (int32_t rc = check_rows("out_stride", d.out_stride, wide, out32 ? 4 : 8)) return rc;
+    if (d.n_seq == 0 || d.n_rows == 0) return MX_ATTN_OK;
+    if (!q || !out) return fail(MX_ATTN_INVALID_ARGUMENT, "q and out must not be null");
+    if (!aligned(q, 16) || !aligned(out, 16)) return fail(MX_ATTN_INVALID_ARGUMENT, "q and out must be 16-byte aligned");
+    if (!aligned(lse, 4)) return fail(MX_ATTN_INVALID_ARGUMENT, "lse must be 4-byte aligned");
+    if (int32_t rc = check_pointers(k, v, table, kv_len, cu_q)) return rc;
+    p.c = cache_of(d, k, v, table, kv_len);
+    p.q = static_cast<const uint16_t *>(q);
+    p.out = out;
+    p.lse = lse;
+    p.cu_q = cu_q;
+    p.q_stride = d.row_stride;
+    p.out_stride = d.out_stride;
+    p.n_head = d.n_head;
+    p.n_head_kv = d.n_head_kv;
+    p.group = d.n_head / d.n_head_kv;
+    p.n_rows = d.n_rows;
+    p.causal = d.causal;
+    p.out32 = out32;
+    // the kernels' exponentials take a positive factor: a negative scale turns the query's sign, 0 makes the query zero
+    p.scale_log2 = d.scale == 0.f ? 1.f : std::fabs(d.scale) * 1.4426950408889634f;
+    p.q_and = d.scale == 0.f ? 0u : 0xffffffffu;
+    p.q_xor = d.scale < 0.f ? 0x80008000u : 0u;
+    return MX_ATTN_OK;
+}
+
+// ---- decode ----
+
+constexpr int kDecodeSplits = 32;      // splits of a sequence at most
+constexpr int kDecodeWorkgroups = 1536;  // a launch of that many workgroups streams best (measured on the contiguous caches)
+
+struct DecodePlan {
+    int32_t rows, rt, n_rowtiles, waves, budget, max_splits;
+    size_t bytes;  // workspace
+};
+
+// Keys per sequence that the plan reckons with.
+int64_t kv_bound(const mx_paged_desc & d) {
+    const int64_t table = (int64_t)d.max_pages * d.page_size;
+    return std::max<int64_t>(1, d.max_kv_len > 0 && (table <= 0 || d.max_kv_len < table) ? d.max_kv_len : table);
+}
+
+int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
+    const int n_q = d.n_rows / d.n_seq;
+    if ((int64_t)n_q * (d.n_head / d.n_head_kv) > 65536)
+        return fail(MX_ATTN_UNSUPPORTED, "%d rows a sequence are a prompt (mx_paged_prefill)", n_q);
+    plan.rows = n_q * (d.n_head / d.n_head_kv);
+    plan.rt = mx::decode_rows_per_tile(plan.rows);
+    plan.n_rowtiles = (plan.rows + plan.rt - 1) / plan.rt;
+    const int64_t per_seq = (int64_t)d.n_head_kv * plan.n_rowtiles, bound = kv_bound(d);
+    // 8 waves where splits of 256 keys fit one workgroup per CU, else 4
+    plan.waves = d.head_dim != 256 && bound >= 512 && d.n_seq * per_seq * std::min<int64_t>(kDecodeSplits, (bound + 255) / 256) <= 256 ? 8 : 4;
+    auto quanta = [&](int waves) { return (bound + 32 * waves - 1) / (32 * waves); };
+    // (sequence, split) pairs beyond one a sequence: up to the workgroups that stream best, and some in any case, so that a long
+    // sequence among many short ones is split
+    static_assert(kDecodeWorkgroups <= mx::kPagedMaxSplitTiles, "a counter for every tile that is split");
+    int64_t extra = std::max((kDecodeWorkgroups / per_seq) - d.n_seq, 512 / per_seq);
+    extra = std::min<int64_t>(extra, d.n_seq * (quanta(plan.waves) - 1));
+    plan.max_splits = kDecodeSplits;
+    if ((d.n_seq + extra) * per_seq > (int64_t)1 << 30)
+        return fail(MX_ATTN_UNSUPPORTED, "%d sequences of %lld (kv head, row tile) pairs are more than one launch holds", d.n_seq, (long long)per_seq);
+    plan.budget = (int32_t)(d.n_seq + extra);
+    // a split sequence has one split more than the pairs beyond it: at most 2 extra partials a tile. Sized for the most extra
+    // pairs of any batch of up to so many sequences and keys, so that a workspace sized for those serves all smaller ones.
+    const int64_t room = std::min<int64_t>(kDecodeWorkgroups / per_seq, d.n_seq * (quanta(4) - 1));
+    plan.bytes = room ? mx::kPagedCounterBytes + (size_t)(2 * room * per_seq * plan.rt * (d.head_dim + 4)) * sizeof(float) : 0;
+    return MX_ATTN_OK;
+}
+
+// ---- prefill ----
+
+// Waves and row tiles of a workgroup (launch_paged_prefill), and the row tiles there can be: every sequence may end one early.
+struct PrefillPlan {
+    int32_t plan;
+    int64_t max_tiles;
+};
+
+int64_t prefill_tiles(const mx_paged_desc & d, int rows) { return std::min<int64_t>(d.n_rows, d.n_rows / rows + d.n_seq); }
+
+// What the plan reckons with; the grid has room for more, as max_q may not hold.
+int64_t likely_tiles(const mx_paged_desc & d, int rows) {
+    const int64_t n = prefill_tiles(d, rows);
+    return d.max_q > 0 ? std::min(n, d.n_seq * (((int64_t)d.max_q + rows - 1) / rows)) : n;
+}
+
+PrefillPlan prefill_plan(const mx_paged_desc & d) {
+    constexpr int64_t kCUs = 256;
+    PrefillPlan r{4, 0};
+    if (d.head_dim != 256) {
+        const int64_t wg8 = likely_tiles(d, 256) * d.n_head, wg4 = likely_tiles(d, 128) * d.n_head;
+        const int64_t bound = kv_bound(d);
+        if ((2 * wg4 <= kCUs && bound >= 512) || (d.head_dim == 64 && 4 * wg4 <= kCUs && bound >= 128)) r.plan = 2;
+        else r.plan = (wg8 + kCUs - 1) / kCUs * 256 * 4 <= (wg4 + kCUs - 1) / kCUs * 128 * 5 ? 8 : 4;
+    }
+    return r;
+}
+
+}  // namespace
+
+extern "C" {
+
+MX_ATTN_API int32_t mx_paged_store(const mx_paged_desc * desc, const mx_paged_rope * rope, const void * qkv,
+                                   const int32_t * positions, void * k, void * v, const int32_t * table,
+                                   const int32_t * kv_len, const int32_t * cu_q, void * q_out, mx_attn_stream stream) {
+    if (int32_t rc = check_shape(desc)) return rc;
+    const mx_paged_desc & d = *desc;
+    if (d.row_dtype != MX_ATTN_F32 && d.row_dtype != MX_ATTN_F16 && d.row_dtype != MX_ATTN_BF16)
+        return fail(MX_ATTN_INVALID_ARGUMENT, "row_dtype (%d) must be MX_ATTN_F32, MX_ATTN_F16 or MX_ATTN_BF16", d.row_dtype);
+    if (!rope) return fail(MX_ATTN_INVALID_ARGUMENT, "rope is null");
+    if (rope->reserved != 0) return fail(MX_ATTN_INVALID_ARGUMENT, "rope->reserved must be 0");
+    if (rope->mode < 0 || rope->mode > 2) return fail(MX_ATTN_INVALID_ARGUMENT, "rope->mode (%d) must be 0, 1 or 2", rope->mode);
+    mx::PagedStoreParams p{};
+    p.rope_mode = rope->mode;
+    p.n_axes = 1;
+    if (rope->mode != 2) {
+        if (rope->n_axes < 1 || rope->n_axes > MX_PAGED_MAX_AXES)
+            return fail(MX_ATTN_INVALID_ARGUMENT, "rope->n_axes (%d) must be in [1, %d]", rope->n_axes, MX_PAGED_MAX_AXES);
+        if (rope->axis_restart != 0 && rope->axis_restart != 1) return fail(MX_ATTN_INVALID_ARGUMENT, "rope->axis_restart must be 0 or 1");
+        if (!(std::isfinite(rope->base) && rope->base > 0.)) return fail(MX_ATTN_INVALID_ARGUMENT, "rope->base must be finite and > 0");
+        p.n_axes = rope->n_axes;
+        int64_t at = 0;
+        for (int a = 0; a < MX_PAGED_MAX_AXES; a++) {
+            const int64_t n = a < rope->n_axes ? rope->axis_pairs[a] : 0;
+            if (a < rope->n_axes && n < 1) return fail(MX_ATTN_INVALID_ARGUMENT, "rope->axis_pairs[%d] (%lld) must be >= 1", a, (long long)n);
+            if (at + n > d.head_dim / 2) return fail(MX_ATTN_INVALID_ARGUMENT, "the axes have more than head_dim / 2 (%d) pairs", d.head_dim / 2);
+            for (int64_t j = 0; j < n; j++)
+                p.freq[at + j] = std::pow(rope->base, rope->axis_restart ? -(double)j / (double)n : -2. * (double)(at + j) / (double)d.head_dim);
+            at += n;
+            p.axis_end[a] = (int32_t)at;
+        }
+        if (at != d.head_dim / 2) return fail(MX_ATTN_INVALID_ARGUMENT, "the axes have %lld pairs, not head_dim / 2 (%d)", (long long)at, d.head_dim / 2);
+        if (!positions && rope->n_axes > 1) return fail(MX_ATTN_INVALID_ARGUMENT, "positions must be given for more than one axis");
+        if (!aligned(positions, 4)) return fail(MX_ATTN_INVALID_ARGUMENT, "positions must be 4-byte aligned");
+    }
+    if (int32_t rc = check_cache(d)) return rc;
+    const int64_t wide = (int64_t)d.n_head * d.head_dim, all = wide + 2 * (int64_t)d.n_head_kv * d.head_dim;
+    if (int32_t rc = check_rows("row_stride", d.row_stride, all, d.row_dtype == MX_ATTN_F32 ? 4 : 8)) return rc;
+    if (q_out)
+        if (int32_t rc = check_rows("out_stride", d.out_stride, wide, 8)) return rc;
+    if (!cu_q)
+        if (int32_t rc = check_uniform(d)) return rc;
+    if (d.n_seq == 0 || d.n_rows == 0) return MX_ATTN_OK;
+    if (!qkv || !aligned(qkv, 16)) return fail(MX_ATTN_INVALID_ARGUMENT, "qkv must be a 16-byte aligned pointer");
+    if (!aligned(q_out, 16)) return fail(MX_ATTN_INVALID_ARGUMENT, "q_out must be 16-byte aligned");
+    if (int32_t rc = check_pointers(k, v, table, kv_len, cu_q)) return rc;
+    p.c = cache_of(d, k, v, table, kv_len);
+    p.qkv = qkv;
+    p.positions = rope->mode == 2 ? nullptr : positions;
+    p.cu_q = cu_q;
+    p.q_out = static_cast<uint16_t *>(q_out);
+    p.row_stride = d.row_stride;
+    p.out_stride = d.out_stride;
+    p.n_head = d.n_head;
+    p.n_head_kv = d.n_head_kv;
+    p.n_rows = d.n_rows;
+    p.n_q = d.n_rows / d.n_seq;
+    const hipError_t e = mx::launch_paged_store(p, d.head_dim, d.row_dtype, d.dtype, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(MX_ATTN_INTERNAL, "paged store launch: %s", hipGetErrorString(e));
+    return MX_ATTN_OK;
+}
+
+MX_ATTN_API size_t mx_paged_decode_workspace_bytes(const mx_paged_desc * desc) {
+    if (check_shape(desc) || check_uniform(*desc) || desc->n_seq == 0 || desc->n_rows == 0) return 0;
+    DecodePlan plan;
+    return decode_plan(*desc, plan) ? 0 : plan.bytes;
+}
+
+MX_ATTN_API int32_t mx_paged_decode(const mx_paged_desc * desc, const void * q, const void * k, const void * v,
+                                    const int32_t * table, const int32_t * kv_len, void * out, float * lse, void * workspace,
+                                    size_t ws_bytes, mx_attn_stream stream) {
+    if (int32_t rc = check_shape(desc)) return rc;
+    const mx_paged_desc & d = *desc;
+    if (int32_t rc = check_uniform(d)) return rc;
+    mx::PagedAttnParams p{};
+    if (int32_t rc = attn_params(d, q, k, v, table, kv_len, nullptr, out, lse, p)) return rc;
+    if (d.n_seq == 0 || d.n_rows == 0) return MX_ATTN_OK;
+    DecodePlan plan;
+    if (int32_t rc = decode_plan(d, plan)) return rc;
+    if (plan.bytes && (!workspace || !aligned(workspace, 256)))
+        return fail(MX_ATTN_INVALID_ARGUMENT, "a 256-byte aligned workspace of %zu bytes is needed", plan.bytes);
+    if (ws_bytes < plan.bytes)
+        return fail(MX_ATTN_RESOURCE_EXHAUSTED, "workspace of %zu bytes is smaller than the %zu bytes needed", ws_bytes, plan.bytes);
+    p.n_q = d.n_rows / d.n_seq;
+    p.rows = plan.rows;
+    p.n_rowtiles = plan.n_rowtiles;
+    p.budget = plan.budget;
+    p.max_splits = plan.max_splits;
+    p.counters = static_cast<uint32_t *>(workspace);
+    p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + mx::kPagedCounterBytes);
+    const hipError_t e = mx::launch_paged_decode(p, d.head_dim, d.dtype, plan.rt, plan.waves, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(MX_ATTN_INTERNAL, "paged decode launch: %s", hipGetErrorString(e));
+    return MX_ATTN_OK;
+}
+
+MX_ATTN_API size_t mx_paged_prefill_workspace_bytes(const mx_paged_desc * desc) {
+    if (check_shape(desc)) return 0;
+    return 0;
+}
+
+MX_ATTN_API int32_t mx_paged_prefill(const mx_paged_desc * desc, const void * q, const void * k, const void * v,
+                                     const int32_t * table, const int32_t * kv_len, const int32_t * cu_q, void * out, float * lse,
+                                     void * workspace, size_t ws_bytes, mx_attn_stream stream) {
+    if (int32_t rc = check_shape(desc)) return rc;
+    const mx_paged_desc & d = *desc;
+    mx::PagedAttnParams p{};
+    if (int32_t rc = attn_params(d, q, k, v, table, kv_len, cu_q, out, lse, p)) return rc;
+    if (d.n_seq == 0 || d.n_rows == 0) return MX_ATTN_OK;
+    if (!cu_q) return fail(MX_ATTN_INVALID_ARGUMENT, "cu_q must not be null");
+    const PrefillPlan plan = prefill_plan(d);
+    const int64_t tiles = prefill_tiles(d, plan.plan * 32);
+    if (tiles * d.n_head > INT32_MAX)
+        return fail(MX_ATTN_UNSUPPORTED, "%d rows of %d heads are more than one launch holds", d.n_rows, d.n_head);
+    p.max_tiles = (int32_t)tiles;
+    (void)workspace;
+    (void)ws_bytes;
+    const hipError_t e = mx::launch_paged_prefill(p, d.head_dim, d.dtype, plan.plan, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(MX_ATTN_INTERNAL, "paged prefill launch: %s", hipGetErrorString(e));
+    return MX_ATTN_OK;
+}
+
+}  // extern "C"

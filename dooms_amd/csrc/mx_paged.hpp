@@ -131,18 +131,25 @@ struct PagedAttnParams {
     uint32_t * counters;
     int64_t q_stride, out_stride;
     int32_t n_head, n_head_kv, group, n_rows, n_q, causal, out32;
-    int32_t budget;        // decode: (sequence, split) pairs that the grid has workgroups for
-    int32_t max_splits;    // decode: splits of one sequence at most
+    int32_t by_ranges;     // decode: 1: workgroups walk ranges of the launch's keys, 0: a chunk of a sequence each
+    int32_t ranges;        // decode: ranges, or chunks, that the launch has workgroups for, for each (kv head, row tile)
+    int32_t max_parts;     // decode: parts of one sequence at most
+    int32_t whole_keys;    // decode, chunks: sequences of up to so many keys are not split
+    int32_t fixed;         // decode, chunks: of every sequence, each a quantum (the last takes what is left); 0: the chunks follow
+                           // from the lengths
+    int32_t whole;         // decode: 1: no sequence is split (there is no workspace)
+    int32_t max_pages;     // entries of a row of the page table
     int32_t max_tiles;     // prefill: tiles of query rows that the grid has workgroups for
     int32_t rows, n_rowtiles;  // decode: query rows that share a kv head, and their tiles
     float scale_log2;      // |scale| log2 e, or 1 with a scale of 0
     uint32_t q_xor, q_and; // scale < 0 turns the sign of the query rows, scale 0 makes them zero
 };
 
-// Partial slots and counters of one decode launch (paged_decode.hip): no more tiles than this are split.
+// Counters of split tiles, where every call on a workspace keeps its own (zero between calls); the partials lie behind them.
 constexpr int kPagedMaxSplitTiles = 2048;
-// Their counters lie where every call on a workspace keeps its own (zero between calls), the partials behind them.
 constexpr size_t kPagedCounterBytes = (size_t)kPagedMaxSplitTiles * kCounterStride * 4;
+
+constexpr int kPagedDecodeBlock = 32;  // keys that a wave of the decode kernel takes at a time
 
 hipError_t launch_paged_store(const PagedStoreParams & p, int head_dim, int in_dtype, int dtype, hipStream_t stream);
 hipError_t launch_paged_decode(const PagedAttnParams & p, int head_dim, int dtype, int rt, int waves, hipStream_t stream);

@@ -157,11 +157,11 @@ int32_t attn_params(const mx_paged_desc & d, const void * q, const void * k, con
 
 // ---- decode ----
 
-constexpr int kDecodeSplits = 32;      // splits of a sequence at most
-constexpr int kDecodeWorkgroups = 1536;  // a launch of that many workgroups streams best (measured on the contiguous caches)
+constexpr int kDecodeParts = 64;  // parts of a sequence at most (the merge takes one lane each)
+constexpr int kCUs = 256;
 
 struct DecodePlan {
-    int32_t rows, rt, n_rowtiles, waves, budget, max_splits;
+    int32_t rows, rt, n_rowtiles, waves, by_ranges, ranges, whole_keys, fixed, whole;
     size_t bytes;  // workspace
 };
 
@@ -176,25 +176,36 @@ int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
     if ((int64_t)n_q * (d.n_head / d.n_head_kv) > 65536)
         return fail(MX_ATTN_UNSUPPORTED, "%d rows a sequence are a prompt (mx_paged_prefill)", n_q);
     plan.rows = n_q * (d.n_head / d.n_head_kv);
-    plan.rt = mx::decode_rows_per_tile(plan.rows);
+    plan.rt = plan.rows > 16 && d.head_dim != 256 ? 32 : mx::decode_rows_per_tile(plan.rows);
     plan.n_rowtiles = (plan.rows + plan.rt - 1) / plan.rt;
     const int64_t per_seq = (int64_t)d.n_head_kv * plan.n_rowtiles, bound = kv_bound(d);
-    // 8 waves where splits of 256 keys fit one workgroup per CU, else 4
-    plan.waves = d.head_dim != 256 && bound >= 512 && d.n_seq * per_seq * std::min<int64_t>(kDecodeSplits, (bound + 255) / 256) <= 256 ? 8 : 4;
-    auto quanta = [&](int waves) { return (bound + 32 * waves - 1) / (32 * waves); };
-    // (sequence, split) pairs beyond one a sequence: up to the workgroups that stream best, and some in any case, so that a long
-    // sequence among many short ones is split
-    static_assert(kDecodeWorkgroups <= mx::kPagedMaxSplitTiles, "a counter for every tile that is split");
-    int64_t extra = std::max((kDecodeWorkgroups / per_seq) - d.n_seq, 512 / per_seq);
-    extra = std::min<int64_t>(extra, d.n_seq * (quanta(plan.waves) - 1));
-    plan.max_splits = kDecodeSplits;
-    if ((d.n_seq + extra) * per_seq > (int64_t)1 << 30)
+    auto quanta = [&](int waves) { return (bound + mx::kPagedDecodeBlock * waves - 1) / (mx::kPagedDecodeBlock * waves); };
+    if (per_seq > mx::kPagedMaxSplitTiles)
+        return fail(MX_ATTN_UNSUPPORTED, "%lld (kv head, row tile) pairs of a sequence are more than one launch holds", (long long)per_seq);
+    const int64_t pairs = d.n_seq * per_seq;
+    plan.whole = bound <= 128;
+    // Ranges where the launch may hold several quanta of 128 keys for every workgroup, chunks below.
+    plan.by_ranges = d.n_seq > 1 && pairs * quanta(4) > (plan.rt <= 8 ? 16 : plan.rt == 16 ? 32 : 64) * kCUs;
+    plan.fixed = 0;
+    plan.whole_keys = 0;
+    if (plan.by_ranges) {
+        plan.waves = 4;
+        plan.ranges = (int32_t)std::max<int64_t>(1, (plan.rt <= 8 ? 2 : 1) * kCUs / per_seq);
+    } else {
+        plan.whole_keys = d.head_dim == 64 ? 640 : 512;
+        plan.waves = d.head_dim == 256 || bound <= 128 || (d.head_dim == 128 && plan.rt <= 8 && bound > 512 && bound <= 4096) ? 4 : 8;
+        plan.ranges = (int32_t)std::max<int64_t>(d.n_seq, (plan.waves == 8 ? 1 : 2) * kCUs / per_seq);
+        const int64_t n = quanta(plan.waves);
+        if (!plan.whole && n <= 32 && pairs * n <= 2 * kCUs) {
+            plan.fixed = (int32_t)n;
+            plan.ranges = d.n_seq * (bound <= plan.whole_keys ? 1 : plan.fixed);
+        }
+    }
+    if (plan.ranges * per_seq > (int64_t)1 << 30)
         return fail(MX_ATTN_UNSUPPORTED, "%d sequences of %lld (kv head, row tile) pairs are more than one launch holds", d.n_seq, (long long)per_seq);
-    plan.budget = (int32_t)(d.n_seq + extra);
-    // a split sequence has one split more than the pairs beyond it: at most 2 extra partials a tile. Sized for the most extra
-    // pairs of any batch of up to so many sequences and keys, so that a workspace sized for those serves all smaller ones.
-    const int64_t room = std::min<int64_t>(kDecodeWorkgroups / per_seq, d.n_seq * (quanta(4) - 1));
-    plan.bytes = room ? mx::kPagedCounterBytes + (size_t)(2 * room * per_seq * plan.rt * (d.head_dim + 4)) * sizeof(float) : 0;
+    // Two partials a range and tile, or two chunks beyond one a sequence; sized for the most of any batch and length, so that one
+    // workspace serves all calls of a head shape and row count.
+    plan.bytes = plan.whole ? 0 : mx::kPagedCounterBytes + (size_t)(2 * std::max<int64_t>(1, 2 * kCUs / per_seq) * per_seq * plan.rt * (d.head_dim + 4)) * sizeof(float);
     return MX_ATTN_OK;
 }
 
@@ -215,7 +226,6 @@ int64_t likely_tiles(const mx_paged_desc & d, int rows) {
 }
 
 PrefillPlan prefill_plan(const mx_paged_desc & d) {
-    constexpr int64_t kCUs = 256;
     PrefillPlan r{4, 0};
     if (d.head_dim != 256) {
         const int64_t wg8 = likely_tiles(d, 256) * d.n_head, wg4 = likely_tiles(d, 128) * d.n_head;
@@ -314,8 +324,13 @@ MX_ATTN_API int32_t mx_paged_decode(const mx_paged_desc * desc, const void * q, 
     p.n_q = d.n_rows / d.n_seq;
     p.rows = plan.rows;
     p.n_rowtiles = plan.n_rowtiles;
-    p.budget = plan.budget;
-    p.max_splits = plan.max_splits;
+    p.by_ranges = plan.by_ranges;
+    p.whole_keys = plan.whole_keys;
+    p.ranges = plan.ranges;
+    p.max_parts = kDecodeParts;
+    p.fixed = plan.fixed;
+    p.whole = plan.whole;
+    p.max_pages = d.max_pages;
     p.counters = static_cast<uint32_t *>(workspace);
     p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + mx::kPagedCounterBytes);
     const hipError_t e = mx::launch_paged_decode(p, d.head_dim, d.dtype, plan.rt, plan.waves, static_cast<hipStream_t>(stream));

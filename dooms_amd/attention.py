@@ -336,6 +336,7 @@ def self_attention(qkv, *, heads, scale=None, out=None, tuning=None):
 
 # ---- the paged cache ----
 
+_PAGED_COUNTERS = 512 << 10  # bytes of counters at the start of a workspace
 _PAGE_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 
 
@@ -441,7 +442,9 @@ def _paged_attend(q, k_pages, v_pages, page_table, kv_len, cu_q, n_head, causal,
     with torch.cuda.device(q.device):
         if workspace is None:
             need = nbytes(d)  # 0 also for an invalid descriptor, which the call reports
-            workspace = new_workspace(need, q.device) if need else torch.empty(0, dtype=torch.uint8, device=q.device)
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+            if need:  # the counters at its start have to be zero, the partials behind them need not be
+                _lib.check(_lib.decode_workspace_init(workspace.data_ptr(), min(need, _PAGED_COUNTERS), _stream()))
         elif workspace.device != q.device or not workspace.is_contiguous():
             raise ValueError("workspace must be a contiguous tensor on the rows' device")
         rest = (out.data_ptr(), _ptr(lse), workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream())
@@ -471,8 +474,9 @@ def paged_decode(q, k_pages, v_pages, page_table, kv_len, *, n_head, n_q=1, caus
 def paged_prefill(q, k_pages, v_pages, page_table, kv_len, cu_q, *, n_head, causal=True, scale=None, out=None, out_dtype=None,
                   lse=None, want_lse=False, max_q=None, max_kv_len=None, workspace=None):
     """mx_paged_prefill: packed prompts, rows cu_q[b] .. cu_q[b + 1] - 1 (cu_q int32 on the device) the last of sequence b's
-    kv_len[b] keys, which the pages hold already. max_q: the most rows of a sequence, for the plan. Everything else as
-    paged_decode (workspace: paged_prefill_workspace_bytes)."""
+    kv_len[b] keys, which the pages hold already. max_q: the most rows of a sequence, for the plan. workspace:
+    paged_prefill_workspace_bytes from new_workspace, kept by the caller; an empty tensor: no workgroups share a tile. Everything
+    else as paged_decode."""
     if workspace is not None:
         r = _native().paged_attend(q, k_pages, v_pages, page_table, kv_len, cu_q, n_head, causal, scale, out, out_dtype, lse, want_lse,
                                    max_q, max_kv_len, workspace)

@@ -127,19 +127,20 @@ struct PagedAttnParams {
     void * out;
     float * lse;
     const int32_t * cu_q;  // prefill
-    float * part;          // decode: partial slots of (head_dim + 4) floats a row: acc, m, l
+    float * part;          // partial slots
     uint32_t * counters;
     int64_t q_stride, out_stride;
     int32_t n_head, n_head_kv, group, n_rows, n_q, causal, out32;
     int32_t by_ranges;     // decode: 1: workgroups walk ranges of the launch's keys, 0: a chunk of a sequence each
-    int32_t ranges;        // decode: ranges, or chunks, that the launch has workgroups for, for each (kv head, row tile)
+    int32_t ranges;        // decode: ranges, or chunks, that the launch has workgroups for, for each (kv head, row tile); prefill:
+                           // workgroups, a multiple of 8
     int32_t max_parts;     // decode: parts of one sequence at most
     int32_t whole_keys;    // decode, chunks: sequences of up to so many keys are not split
     int32_t fixed;         // decode, chunks: of every sequence, each a quantum (the last takes what is left); 0: the chunks follow
                            // from the lengths
-    int32_t whole;         // decode: 1: no sequence is split (there is no workspace)
+    int32_t whole;         // 1: no sequence (prefill: no tile) is split, there is no workspace
     int32_t max_pages;     // entries of a row of the page table
-    int32_t max_tiles;     // prefill: tiles of query rows that the grid has workgroups for
+    int32_t max_tiles;     // prefill: tiles of query rows that there can be
     int32_t rows, n_rowtiles;  // decode: query rows that share a kv head, and their tiles
     float scale_log2;      // |scale| log2 e, or 1 with a scale of 0
     uint32_t q_xor, q_and; // scale < 0 turns the sign of the query rows, scale 0 makes them zero
@@ -151,8 +152,17 @@ constexpr size_t kPagedCounterBytes = (size_t)kPagedMaxSplitTiles * kCounterStri
 
 constexpr int kPagedDecodeBlock = 32;  // keys that a wave of the decode kernel takes at a time
 
+// A prefill workgroup: waves of 32 query rows, `heads` of a group among them. Head dim 256 runs 4 waves of one head.
+struct PagedPrefillPlan {
+    int32_t waves, heads;
+    int rows() const { return 32 * waves / heads; }
+    int resident(int head_dim) const { return waves == 8 || head_dim == 256 ? 256 : 512; }  // workgroups that run at once
+    // floats of a range's two partials: per lane its outputs, m and l
+    int64_t part_floats(int head_dim) const { return 2 * (int64_t)waves * (head_dim / 2 + 2) * kWave; }
+};
+
 hipError_t launch_paged_store(const PagedStoreParams & p, int head_dim, int in_dtype, int dtype, hipStream_t stream);
 hipError_t launch_paged_decode(const PagedAttnParams & p, int head_dim, int dtype, int rt, int waves, hipStream_t stream);
-hipError_t launch_paged_prefill(const PagedAttnParams & p, int head_dim, int dtype, int plan, hipStream_t stream);
+hipError_t launch_paged_prefill(const PagedAttnParams & p, int head_dim, int dtype, const PagedPrefillPlan & plan, hipStream_t stream);
 
 }  // namespace mx

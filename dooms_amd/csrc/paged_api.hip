@@ -211,12 +211,6 @@ int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
 
 // ---- prefill ----
 
-// Waves and row tiles of a workgroup (launch_paged_prefill), and the row tiles there can be: every sequence may end one early.
-struct PrefillPlan {
-    int32_t plan;
-    int64_t max_tiles;
-};
-
 int64_t prefill_tiles(const mx_paged_desc & d, int rows) { return std::min<int64_t>(d.n_rows, d.n_rows / rows + d.n_seq); }
 
 // What the plan reckons with; the grid has room for more, as max_q may not hold.
@@ -225,15 +219,24 @@ int64_t likely_tiles(const mx_paged_desc & d, int rows) {
     return d.max_q > 0 ? std::min(n, d.n_seq * (((int64_t)d.max_q + rows - 1) / rows)) : n;
 }
 
-PrefillPlan prefill_plan(const mx_paged_desc & d) {
-    PrefillPlan r{4, 0};
-    if (d.head_dim != 256) {
-        const int64_t wg8 = likely_tiles(d, 256) * d.n_head, wg4 = likely_tiles(d, 128) * d.n_head;
-        const int64_t bound = kv_bound(d);
-        if ((2 * wg4 <= kCUs && bound >= 512) || (d.head_dim == 64 && 4 * wg4 <= kCUs && bound >= 128)) r.plan = 2;
-        else r.plan = (wg8 + kCUs - 1) / kCUs * 256 * 4 <= (wg4 + kCUs - 1) / kCUs * 128 * 5 ? 8 : 4;
-    }
+mx::PagedPrefillPlan prefill_plan(const mx_paged_desc & d) {
+    mx::PagedPrefillPlan r{4, 1};
+    if (d.head_dim == 256) return r;
+    const int group = d.n_head / d.n_head_kv;
+    const int64_t wg8 = likely_tiles(d, 256) * d.n_head, wg4 = likely_tiles(d, 128) * d.n_head;
+    r.waves = (wg8 + kCUs - 1) / kCUs * 256 * 4 <= (wg4 + kCUs - 1) / kCUs * 128 * 5 ? 8 : 4;
+    r.heads = r.waves == 8 && group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
     return r;
+}
+
+// The counters, and two partials of a tile for each of the workgroups that run at once, whichever plan runs.
+size_t prefill_bytes(int head_dim) {
+    size_t floats = 0;
+    for (const int waves : {4, 8}) {
+        const mx::PagedPrefillPlan r{waves, 1};
+        if (waves == 4 || head_dim != 256) floats = std::max(floats, (size_t)(r.resident(head_dim) * r.part_floats(head_dim)));
+    }
+    return mx::kPagedCounterBytes + floats * sizeof(float);
 }
 
 }  // namespace
@@ -339,8 +342,8 @@ MX_ATTN_API int32_t mx_paged_decode(const mx_paged_desc * desc, const void * q, 
 }
 
 MX_ATTN_API size_t mx_paged_prefill_workspace_bytes(const mx_paged_desc * desc) {
-    if (check_shape(desc)) return 0;
-    return 0;
+    if (check_shape(desc) || desc->n_seq == 0 || desc->n_rows == 0) return 0;
+    return prefill_bytes(desc->head_dim);
 }
 
 MX_ATTN_API int32_t mx_paged_prefill(const mx_paged_desc * desc, const void * q, const void * k, const void * v,
@@ -352,14 +355,19 @@ MX_ATTN_API int32_t mx_paged_prefill(const mx_paged_desc * desc, const void * q,
     if (int32_t rc = attn_params(d, q, k, v, table, kv_len, cu_q, out, lse, p)) return rc;
     if (d.n_seq == 0 || d.n_rows == 0) return MX_ATTN_OK;
     if (!cu_q) return fail(MX_ATTN_INVALID_ARGUMENT, "cu_q must not be null");
-    const PrefillPlan plan = prefill_plan(d);
-    const int64_t tiles = prefill_tiles(d, plan.plan * 32);
-    if (tiles * d.n_head > INT32_MAX)
+    const mx::PagedPrefillPlan plan = prefill_plan(d);
+    const int64_t tiles = prefill_tiles(d, plan.rows());
+    if (tiles * d.n_head > INT32_MAX / 8)
         return fail(MX_ATTN_UNSUPPORTED, "%d rows of %d heads are more than one launch holds", d.n_rows, d.n_head);
     p.max_tiles = (int32_t)tiles;
-    (void)workspace;
-    (void)ws_bytes;
-    const hipError_t e = mx::launch_paged_prefill(p, d.head_dim, d.dtype, plan.plan, static_cast<hipStream_t>(stream));
+    p.ranges = plan.resident(d.head_dim);
+    p.whole = !workspace;
+    if (workspace && !aligned(workspace, 256)) return fail(MX_ATTN_INVALID_ARGUMENT, "the workspace must be 256-byte aligned");
+    if (workspace && ws_bytes < prefill_bytes(d.head_dim))
+        return fail(MX_ATTN_RESOURCE_EXHAUSTED, "workspace of %zu bytes is smaller than the %zu bytes needed", ws_bytes, prefill_bytes(d.head_dim));
+    p.counters = static_cast<uint32_t *>(workspace);
+    p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + mx::kPagedCounterBytes);
+    const hipError_t e = mx::launch_paged_prefill(p, d.head_dim, d.dtype, plan, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return fail(MX_ATTN_INTERNAL, "paged prefill launch: %s", hipGetErrorString(e));
     return MX_ATTN_OK;
 }

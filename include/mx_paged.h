@@ -117,7 +117,9 @@ MX_ATTN_API size_t mx_paged_decode_workspace_bytes(const mx_paged_desc * desc);
 /*
  * Attention of packed prompts: rows cu_q[b] .. cu_q[b + 1] - 1 are the last rows of sequence b, whose pages hold its keys
  * already (mx_paged_store), those of an earlier chunk or a shared prefix among them. Rows from cu_q[n_seq] on are left as
- * they were. Arguments as mx_paged_decode; workspace as there, of mx_paged_prefill_workspace_bytes(desc) bytes.
+ * they were. Arguments as mx_paged_decode. With a workspace (mx_paged_prefill_workspace_bytes(desc) bytes, the rules of
+ * mx_paged_decode's) the work is cut into equal ranges over the chip, which split a tile of rows between workgroups; NULL: no
+ * tile is split.
  */
 MX_ATTN_API int32_t mx_paged_prefill(const mx_paged_desc * desc, const void * q, const void * k, const void * v,
                                      const int32_t * table, const int32_t * kv_len, const int32_t * cu_q, void * out, float * lse,

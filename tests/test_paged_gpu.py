@@ -330,6 +330,34 @@ def test_prefill_plans(device, hd, n_head, n_kv, max_q):
     prefill_case(device, 83, n_head, n_kv, hd, [600, 130, 20, 1], [650, 130, 900, 77], 32, F16, max_q=max_q)
 
 
+@pytest.mark.parametrize("hd,n_head,n_kv,dtype", [(128, 8, 2, F16), (64, 7, 1, BF16), (128, 4, 4, BF16), (256, 2, 1, F16)])
+def test_prefill_split_tiles(device, hd, n_head, n_kv, dtype):
+    """A few rows behind many keys: every tile is cut over many workgroups; with a workspace and without one."""
+    for ws in (None, torch.empty(0, dtype=torch.uint8, device=device)):
+        prefill_case(device, 93, n_head, n_kv, hd, [70, 3, 200], [5000, 9000, 2000], 64, dtype, ws=ws, what=f"ws {ws is not None}")
+
+
+@pytest.mark.parametrize("n_head,n_kv,hd", [(32, 8, 128), (28, 4, 128), (14, 2, 64), (16, 16, 64)])
+def test_prefill_ranges(device, n_head, n_kv, hd):
+    """More tiles than workgroups: ranges that begin and end within tiles, sequences and kv heads."""
+    prefill_case(device, 94, n_head, n_kv, hd, [700, 33, 0, 512, 1, 900], [1000, 33, 7, 512, 800, 900], 16, BF16)
+
+
+def test_prefill_same_bits(device):
+    """Split tiles are joined in order, whichever workgroup is last; the workspace serves call after call, of any shape."""
+    g = gen(95)
+    ws = A.new_workspace(A.paged_prefill_workspace_bytes(n_head=28, n_head_kv=4, head_dim=128, n_rows=1, n_seq=1, max_q=1, max_kv_len=1), device)
+    cases = []
+    for rows, lens, n_head, n_kv in (([300, 100], [6000, 3000], 28, 4), ([800, 10], [800, 4000], 32, 8)):
+        c = Cache(g, lens, n_kv, 128, 32, BF16)
+        q = torch.randn(sum(rows), n_head * 128, generator=g).to(BF16).to(device)
+        cases.append((q, *c.to(device), cu_of(rows, device), n_head))
+    first = [A.paged_prefill(*c[:-1], n_head=c[-1], workspace=ws)[0] for c in cases]
+    for _ in range(10):
+        for c, f in zip(cases, first):
+            assert torch.equal(f, A.paged_prefill(*c[:-1], n_head=c[-1], workspace=ws)[0])
+
+
 def test_prefill_many_sequences(device):
     rows = [(b * 7) % 40 for b in range(150)]
     prefill_case(device, 84, 4, 2, 64, rows, [r + (b % 5) * 11 for b, r in enumerate(rows)], 16, BF16)

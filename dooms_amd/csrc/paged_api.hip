@@ -183,6 +183,10 @@ int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
     if (per_seq > mx::kPagedMaxSplitTiles)
         return fail(MX_ATTN_UNSUPPORTED, "%lld (kv head, row tile) pairs of a sequence are more than one launch holds", (long long)per_seq);
     const int64_t pairs = d.n_seq * per_seq;
+    // the kernel counts the quanta of all sequences in 32 bits
+    if (d.n_seq * ((std::max<int64_t>(bound, (int64_t)d.max_pages * d.page_size) + 127) / 128) > (int64_t)1 << 30)
+        return fail(MX_ATTN_UNSUPPORTED, "%d sequences of up to %lld keys are more than one launch holds", d.n_seq,
+                    (long long)std::max<int64_t>(bound, (int64_t)d.max_pages * d.page_size));
     plan.whole = bound <= 128;
     // Ranges where the launch may hold several quanta of 128 keys for every workgroup, chunks below.
     plan.by_ranges = d.n_seq > 1 && pairs * quanta(4) > (plan.rt <= 8 ? 16 : plan.rt == 16 ? 32 : 64) * kCUs;
@@ -197,11 +201,11 @@ int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
         plan.ranges = (int32_t)std::max<int64_t>(d.n_seq, (plan.waves == 8 ? 1 : 2) * kCUs / per_seq);
         const int64_t n = quanta(plan.waves);
         if (!plan.whole && n <= 32 && pairs * n <= 2 * kCUs) {
-            plan.fixed = (int32_t)n;
-            plan.ranges = d.n_seq * (bound <= plan.whole_keys ? 1 : plan.fixed);
+            plan.fixed = bound <= plan.whole_keys ? 1 : (int32_t)n;
+            plan.ranges = d.n_seq * plan.fixed;
         }
     }
-    if (plan.ranges * per_seq > (int64_t)1 << 30)
+    if (plan.ranges * per_seq * plan.waves > (int64_t)1 << 25)  // threads of a grid's dimension: below 2^32
         return fail(MX_ATTN_UNSUPPORTED, "%d sequences of %lld (kv head, row tile) pairs are more than one launch holds", d.n_seq, (long long)per_seq);
     // Two partials a range and tile, or two chunks beyond one a sequence; sized for the most of any batch and length, so that one
     // workspace serves all calls of a head shape and row count.

@@ -683,8 +683,8 @@ void paged_prefill_kernel(PagedAttnParams p) {
                         if (empty && !poison) o[dt][v] = 0.f;
             }
         }
-        // the next tile's query is here, and with it every load sent for before it: waited for ahead of the stores, which count
-        // behind them
+        // the next tile's query and every step sent for, ahead of the stores, which count behind them
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) asm volatile("" : "+v"(qb[ks])::"memory");
         waited = true;

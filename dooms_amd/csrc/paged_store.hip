@@ -49,7 +49,9 @@ __global__ __launch_bounds__(512) void paged_store_kernel(PagedStoreParams p) {
     constexpr int AHEAD = 2;                  // units a thread loads at once
     __shared__ float2 s_cs[HALF];
 
-    const int row = blockIdx.x, lane = threadIdx.x % kWave;
+    const int64_t block = blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
+    if (block >= p.n_rows) return;
+    const int row = (int)block, lane = threadIdx.x % kWave;
     const int units = (p.n_head + 2 * p.n_head_kv) * UH;
     const char * src = static_cast<const char *>(p.qkv) + (int64_t)row * p.row_stride * (IN == 0 ? 4 : 2);
     auto load = [&](int u, u32x4 (&w)[2]) __attribute__((always_inline)) {
@@ -174,7 +176,8 @@ template <int HD, class T>
 void launch_in(const PagedStoreParams & p, int in_dtype, hipStream_t stream) {
     const int units = (p.n_head + 2 * p.n_head_kv) * HD / (in_dtype == 0 ? 8 : 16);
     const int threads = std::max(HD / 2, std::min(512, (units + kWave - 1) / kWave * kWave));
-    const dim3 grid((uint32_t)p.n_rows), block((uint32_t)threads);
+    constexpr int kMost = 1 << 22;  // workgroups along x: a dimension holds fewer than 2^32 threads
+    const dim3 grid((uint32_t)std::min(p.n_rows, kMost), (uint32_t)(((int64_t)p.n_rows + kMost - 1) / kMost)), block((uint32_t)threads);
     if (in_dtype == 0) hipLaunchKernelGGL((paged_store_kernel<HD, 0, T>), grid, block, 0, stream, p);
     else if (in_dtype == 1) hipLaunchKernelGGL((paged_store_kernel<HD, 1, T>), grid, block, 0, stream, p);
     else hipLaunchKernelGGL((paged_store_kernel<HD, 2, T>), grid, block, 0, stream, p);

@@ -110,6 +110,12 @@ def test_attention_refusals():
     assert decode(desc(n_rows=4)) == _lib.INVALID_ARGUMENT and "multiple of n_seq" in _lib.last_error()
     assert decode(desc(n_seq=0)) == _lib.INVALID_ARGUMENT and "no sequence" in _lib.last_error()
     assert decode(desc(n_rows=3 * 20000)) == _lib.UNSUPPORTED and "mx_paged_prefill" in _lib.last_error()
+    wide = dict(n_seq=65535, max_pages=1 << 20, table_stride=1 << 20, page_size=1024, page_stride=1024 * 256)
+    assert decode(desc(n_rows=65535, **wide)) == _lib.UNSUPPORTED and "more than one launch" in _lib.last_error()
+    assert decode(desc(n_head=4096, n_head_kv=4096, row_stride=3 * 4096 * 128, out_stride=4096 * 128, kv_stride=4096 * 128,
+                       page_stride=16 * 4096 * 128)) == _lib.UNSUPPORTED and "row tile" in _lib.last_error()
+    assert prefill(desc(), ws=P + 16, ws_bytes=1 << 30) == _lib.INVALID_ARGUMENT and "256-byte" in _lib.last_error()
+    assert prefill(desc(), ws_bytes=1 << 20) == _lib.RESOURCE_EXHAUSTED
 
 
 def test_decode_workspace():

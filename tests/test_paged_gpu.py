@@ -108,6 +108,22 @@ def test_store_one_sequence_of_many(device):
     store_case(device, 11, 4, 2, 64, rows, [1 + b % 40 for b in range(200)], 16, F16, F32, 0)
 
 
+def test_store_many_rows(device):
+    """More rows than a grid has workgroups along one dimension, and offsets past 2^32 bytes."""
+    n = (1 << 22) + 5
+    x = torch.randn(n, 1, device=device).to(F16) * torch.arange(1, 193, device=device).to(F16)[None] / 64
+    table = torch.arange(n // 4096 + 1, dtype=torch.int32, device=device)[None].contiguous()
+    k = torch.zeros(table.shape[1], 4096, 1, 64, dtype=F16, device=device)
+    wide = torch.zeros(2, table.shape[1], 4096, 10, 64, dtype=F16, device=device)[:, :, :, 9:]
+    v = torch.zeros_like(k)
+    lens = torch.tensor([n], dtype=torch.int32, device=device)
+    q = A.paged_store(x, k, v, table, lens, n_head=1, rope_mode=2)
+    assert torch.equal(q, x[:, :64]) and torch.equal(k.view(-1, 64)[:n], x[:, 64:128]) and torch.equal(v.view(-1, 64)[:n], x[:, 128:])
+    assert (k.view(-1, 64)[n:] == 0).all()
+    A.paged_store(x, wide[0], wide[1], table, lens, n_head=1, rope_mode=2, want_q=False)
+    assert torch.equal(wide[0, -1, (n - 1) % 4096, 0], x[-1, 64:128])
+
+
 def test_store_leaves_out_what_has_no_place(device):
     """Rows whose page is none, whose length passes the table or whose position is below 0 are not stored; their queries are."""
     g = gen(12)
@@ -203,6 +219,15 @@ def test_decode_many_sequences(device, n_seq, n_q):
     lens = [(b * 37) % 90 for b in range(n_seq)]
     lens[n_seq // 2] = 3000
     decode_case(device, 29, 4, 2, 64, lens, 16, F16, n_q=n_q)
+
+
+@pytest.mark.parametrize("max_kv_len", [None, 100, 600, 3000, 1 << 20])
+@pytest.mark.parametrize("hd,n_head,n_kv,n_q", [(64, 4, 2, 1), (64, 14, 2, 1), (64, 14, 2, 2), (64, 14, 2, 7), (128, 8, 2, 1), (128, 7, 1, 1),
+                                                (128, 16, 1, 1), (128, 28, 4, 4), (256, 4, 2, 1), (256, 16, 2, 3)])
+def test_decode_plans(device, hd, n_head, n_kv, n_q, max_kv_len):
+    """Every way of cutting a launch (whole sequences, chunks planned by the host or from the lengths, ranges) at every tile of rows:
+    the hint chooses it and may not change the result, however wrong."""
+    decode_case(device, 34, n_head, n_kv, hd, [1300, 40, 0, 513, 257, 1, 700], 32, F16, n_q=n_q, max_kv_len=max_kv_len)
 
 
 def test_decode_shared_pages(device):

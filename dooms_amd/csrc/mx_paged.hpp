@@ -67,14 +67,6 @@ struct PagedCache {
 __device__ __forceinline__ bool length_ok(const PagedCache & c, int32_t len) { return len >= 0 && len <= c.capacity; }
 __device__ __forceinline__ bool page_ok(const PagedCache & c, int32_t id) { return (uint32_t)id < (uint32_t)c.n_pages; }
 
-// A load through the vector memory path of an address that is the same in every lane. The compiler would make a scalar load
-// of it, whose completion order against the LDS reads that count on the same counter is not defined.
-__device__ __forceinline__ int32_t load_uniform(const int32_t * p) {
-    int zero = 0;
-    asm volatile("" : "+v"(zero));
-    return *(const __attribute__((address_space(1))) int32_t *)(p + zero);
-}
-
 // Sum and inclusive prefix sum over the 64 lanes of a wave (every lane active).
 __device__ __forceinline__ int32_t wave_isum(int32_t v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false);

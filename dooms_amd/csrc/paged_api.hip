@@ -39,7 +39,7 @@ int32_t check_shape(const mx_paged_desc * d) {
     if (d->dtype != MX_ATTN_F16 && d->dtype != MX_ATTN_BF16)
         return fail(MX_ATTN_INVALID_ARGUMENT, "dtype (%d) must be MX_ATTN_F16 or MX_ATTN_BF16", d->dtype);
     if (d->n_seq < 0 || d->n_seq > 65535) return fail(MX_ATTN_INVALID_ARGUMENT, "n_seq (%d) must be in [0, 65535]", d->n_seq);
-    if (d->n_rows < 0) return fail(MX_ATTN_INVALID_ARGUMENT, "n_rows (%d) must be >= 0", d->n_rows);
+    if (d->n_rows < 0 || d->n_rows > 1 << 30) return fail(MX_ATTN_INVALID_ARGUMENT, "n_rows (%d) must be in [0, 2^30]", d->n_rows);
     if (d->max_q < 0 || d->max_kv_len < 0)
         return fail(MX_ATTN_INVALID_ARGUMENT, "max_q (%d) and max_kv_len (%d) must be >= 0", d->max_q, d->max_kv_len);
     return MX_ATTN_OK;
@@ -276,7 +276,8 @@ MX_ATTN_API int32_t mx_paged_store(const mx_paged_desc * desc, const mx_paged_ro
         if (rope->n_axes < 1 || rope->n_axes > MX_PAGED_MAX_AXES)
             return fail(MX_ATTN_INVALID_ARGUMENT, "rope->n_axes (%d) must be in [1, %d]", rope->n_axes, MX_PAGED_MAX_AXES);
         if (rope->axis_restart != 0 && rope->axis_restart != 1) return fail(MX_ATTN_INVALID_ARGUMENT, "rope->axis_restart must be 0 or 1");
-        if (!(std::isfinite(rope->base) && rope->base > 0.)) return fail(MX_ATTN_INVALID_ARGUMENT, "rope->base must be finite and > 0");
+        // below 1 the angles would grow past what the kernel reduces
+        if (!(std::isfinite(rope->base) && rope->base >= 1.)) return fail(MX_ATTN_INVALID_ARGUMENT, "rope->base must be finite and >= 1");
         p.n_axes = rope->n_axes;
         int64_t at = 0;
         for (int a = 0; a < MX_PAGED_MAX_AXES; a++) {
@@ -378,7 +379,9 @@ MX_ATTN_API int32_t mx_paged_prefill(const mx_paged_desc * desc, const void * q,
     if (!cu_q) return fail(MX_ATTN_INVALID_ARGUMENT, "cu_q must not be null");
     const mx::PagedPrefillPlan plan = prefill_plan(d);
     const int64_t tiles = prefill_tiles(d, plan.rows());
-    if (tiles * d.n_head > INT32_MAX / 8)
+    // tiles are counted in 32 bits, their steps in 64 (and 55 for 64 sequences), whatever cu_q holds
+    const double steps = (double)(d.n_rows / plan.rows() + 1) * ((double)d.max_pages * d.page_size / 64. + 4.);
+    if (tiles * d.n_head > INT32_MAX / 8 || steps > 0x1p49 || steps * d.n_seq * d.n_head > 0x1p61)
         return fail(MX_ATTN_UNSUPPORTED, "%d rows of %d heads are more than one launch holds", d.n_rows, d.n_head);
     p.max_tiles = (int32_t)tiles;
     p.ranges = plan.resident(d.head_dim);

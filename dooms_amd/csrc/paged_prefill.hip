@@ -106,12 +106,15 @@ __device__ __forceinline__ void row_alone(const PagedAttnParams & p, const Tile 
 #pragma unroll
     for (int d = 0; d < HD / 64; d++) q[d] = one((uint16_t)((qr[lane + 64 * d] & p.q_and) ^ p.q_xor));
     const int32_t * table = p.c.table + t.b * p.c.table_stride;
+    bool bad = false;  // a page of another part of the tile may be none
     m = kNegInf;
     l = 0.f;
 #pragma unroll
     for (int d = 0; d < HD / 64; d++) o[d] = 0.f;
     for (int j = 0; j < visible; j++) {
-        const int64_t at = (int64_t)table[j >> p.c.page_shift] * p.c.page_stride +
+        const int id = table[j >> p.c.page_shift];
+        bad |= !page_ok(p.c, id);
+        const int64_t at = (int64_t)(page_ok(p.c, id) ? id : 0) * p.c.page_stride +
                            (int64_t)(j & ((1 << p.c.page_shift) - 1)) * p.c.kv_stride + (int64_t)t.kvh * p.c.head_stride + lane;
         float s = 0.f;
 #pragma unroll
@@ -124,6 +127,7 @@ __device__ __forceinline__ void row_alone(const PagedAttnParams & p, const Tile 
         for (int d = 0; d < HD / 64; d++) o[d] = (m == kNegInf ? 0.f : o[d] * corr) + w * one(p.c.v[at + 64 * d]);
         m = mn;
     }
+    if (bad) l = __builtin_nanf("");
 }
 
 // Whether a value at keys k0 .. k1 - 1 of the tile's kv head is an infinity or NaN (wave-uniform).
@@ -133,9 +137,10 @@ __device__ __forceinline__ bool odd_values(const PagedAttnParams & p, const Tile
     const int32_t * table = p.c.table + t.b * p.c.table_stride;
     bool odd = false;
     for (int j = k0 + lane / (HD / 8); j < k1; j += kWave / (HD / 8)) {
-        const int64_t at = (int64_t)table[j >> p.c.page_shift] * p.c.page_stride +
-                           (int64_t)(j & ((1 << p.c.page_shift) - 1)) * p.c.kv_stride + (int64_t)t.kvh * p.c.head_stride +
-                           8 * (lane % (HD / 8));
+        const int id = table[j >> p.c.page_shift];
+        if (!page_ok(p.c, id)) continue;
+        const int64_t at = (int64_t)id * p.c.page_stride + (int64_t)(j & ((1 << p.c.page_shift) - 1)) * p.c.kv_stride +
+                           (int64_t)t.kvh * p.c.head_stride + 8 * (lane % (HD / 8));
         odd |= any_nonfinite<T>(load16(p.c.v + at));
     }
     return __builtin_amdgcn_ballot_w64(odd) != 0;
@@ -188,11 +193,11 @@ void paged_prefill_kernel(PagedAttnParams p) {
     for (int base = 0; base < n_seq; base += kWave) {
         read(base);
         const Rows<R> s = rows_of(nq, len);
-        tiles += __builtin_amdgcn_readlane(wave_iscan(min(s.nt, 1 << 24)), 63);
+        // more than p.max_tiles only where ranges of cu_q overlap
+        tiles = min(tiles + __builtin_amdgcn_readlane(wave_iscan(min(s.nt, 1 << 24)), 63), p.max_tiles);
         units += read_lane64(wave_scan64(s.units()), 63);
         longest = max(longest, wave_imax(s.n ? s.steps(s.nt - 1) : 0));
     }
-    tiles = min(tiles, p.max_tiles);  // more only where ranges of cu_q overlap
     const int all = tiles * sets * p.n_head_kv;
     const bool direct = all <= p.ranges && longest <= kDirectSteps;
     const int64_t per_kv = units * sets, total = per_kv * p.n_head_kv;
@@ -491,7 +496,7 @@ void paged_prefill_kernel(PagedAttnParams p) {
                 });
                 static_for<0, NG>([&](auto I) __attribute__((always_inline)) {
                     constexpr int i = decltype(I)::value;
-                    asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(kf[i]) : "i"(NG - 1 - i));
+                    asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(kf[i]) : "i"(NG - 1 - i < 14 ? NG - 1 - i : 14));  // 15: no wait
                     sc[i % 2] = T::mfma32(kf[i], qb[(g0 + i) / 2], sc[i % 2]);
                     __builtin_amdgcn_sched_barrier(0);
                 });

@@ -14,8 +14,9 @@
  * that hold no key (behind a sequence's end, or in pages of no sequence) are never used, whatever they hold.
  *
  * Device metadata cannot be checked by the host, and no entry of it makes a call read or write outside the pool:
- *   - a page outside [0, n_pages) among those that a row attends, or kv_len outside [0, max_pages * page_size], makes that
- *     sequence's outputs NaN; mx_paged_store leaves out the keys and values of a row that such a page or length would take;
+ *   - kv_len outside [0, max_pages * page_size] makes that sequence's outputs NaN, a page outside [0, n_pages) the rows that
+ *     attend it (and rows of that sequence that are computed with them); mx_paged_store leaves out the keys and values of a row
+ *     that such a page or length would take;
  *   - query rows that see no key (kv_len 0, or rows of a causal call at positions below 0) give zeros and an lse of -inf;
  *   - cu_q entries are clamped to [0, n_rows]; what overlapping ranges compute is undefined.
  *
@@ -69,7 +70,7 @@ typedef struct mx_paged_rope {
     int32_t axis_restart; /* 0: f(i) = base^(-2i / head_dim), one ladder over the head; 1: f(i) = base^(-j / axis_pairs[a]) for
                              the j-th pair of axis a, a ladder for each axis */
     int32_t reserved;     /* must be 0 */
-    double base;          /* > 0; 64 bits, as are the angles: at far positions 32 lose them */
+    double base;          /* >= 1; 64 bits, as are the angles: at far positions 32 lose them */
 } mx_paged_rope;
 
 /*
@@ -87,7 +88,7 @@ typedef struct mx_paged_rope {
  *              they were; NULL: n_rows / n_seq rows each
  *   q_out      device, [n_rows][out_stride] of dtype, or NULL: queries are not wanted
  *
- * Two rows must not be given the same cache position of the same page.
+ * Two rows must not be given the same cache position of the same page. q_out must not overlap qkv.
  */
 MX_ATTN_API int32_t mx_paged_store(const mx_paged_desc * desc, const mx_paged_rope * rope, const void * qkv,
                                    const int32_t * positions, void * k, void * v, const int32_t * table,

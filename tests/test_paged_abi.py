@@ -116,6 +116,9 @@ def test_attention_refusals():
                        page_stride=16 * 4096 * 128)) == _lib.UNSUPPORTED and "row tile" in _lib.last_error()
     assert prefill(desc(), ws=P + 16, ws_bytes=1 << 30) == _lib.INVALID_ARGUMENT and "256-byte" in _lib.last_error()
     assert prefill(desc(), ws_bytes=1 << 20) == _lib.RESOURCE_EXHAUSTED
+    assert prefill(desc(n_rows=1 << 28, **wide)) == _lib.UNSUPPORTED and "more than one launch" in _lib.last_error()
+    for call in (decode, prefill):
+        assert call(desc(n_rows=(1 << 30) + 3)) == _lib.INVALID_ARGUMENT and "n_rows" in _lib.last_error()
 
 
 def test_decode_workspace():
@@ -147,6 +150,7 @@ def test_decode_workspace_sized_once(n_head, n_kv, hd):
 @pytest.mark.parametrize("word,kw", [
     ("reserved", dict(reserved=1)), ("mode", dict(mode=3)), ("mode", dict(mode=-1)), ("n_axes", dict(n_axes=0)), ("n_axes", dict(n_axes=5)),
     ("axis_restart", dict(axis_restart=2)), ("base", dict(base=0.0)), ("base", dict(base=float("nan"))), ("base", dict(base=-2.0)),
+    ("base", dict(base=0.5)),
     ("not head_dim / 2", dict(axis_pairs=(63,))), ("more than head_dim / 2", dict(axis_pairs=(65,))),
     ("axis_pairs[1]", dict(n_axes=2, axis_pairs=(64, 0))), ("axis_pairs[0]", dict(axis_pairs=(-1,))),
     ("positions", dict(n_axes=2, axis_pairs=(32, 32))),

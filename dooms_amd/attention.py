@@ -477,13 +477,13 @@ def paged_prefill(q, k_pages, v_pages, page_table, kv_len, cu_q, *, n_head, caus
     kv_len[b] keys, which the pages hold already. max_q: the most rows of a sequence, for the plan. workspace:
     paged_prefill_workspace_bytes from new_workspace, kept by the caller; an empty tensor: no workgroups share a tile. Everything
     else as paged_decode."""
+    if cu_q is None:
+        raise ValueError("cu_q must be given")
     if workspace is not None:
         r = _native().paged_attend(q, k_pages, v_pages, page_table, kv_len, cu_q, n_head, causal, scale, out, out_dtype, lse, want_lse,
                                    max_q, max_kv_len, workspace)
         if r is not None:
             return _result(r)
-    if cu_q is None:
-        raise ValueError("cu_q must be given")
     return _paged_attend(q, k_pages, v_pages, page_table, kv_len, cu_q, n_head, causal, scale, out, out_dtype, lse, want_lse, max_q,
                          max_kv_len, workspace, _lib.paged_prefill_raw, _lib.paged_prefill_workspace_bytes)
 

@@ -230,6 +230,15 @@ def test_decode_plans(device, hd, n_head, n_kv, n_q, max_kv_len):
     decode_case(device, 34, n_head, n_kv, hd, [1300, 40, 0, 513, 257, 1, 700], 32, F16, n_q=n_q, max_kv_len=max_kv_len)
 
 
+@pytest.mark.parametrize("hd,n_head,n_kv,n_q", [(64, 14, 2, 1), (64, 14, 2, 3), (64, 8, 1, 4), (128, 32, 8, 1), (128, 7, 1, 2), (128, 28, 4, 5),
+                                                (256, 8, 2, 1), (256, 16, 1, 2)])
+def test_decode_ranges(device, hd, n_head, n_kv, n_q):
+    """Batches cut into ranges of all sequences' keys, more sequences than lanes, with empty ones and a length that is none."""
+    lens = [(b * 53) % 400 for b in range(150)]
+    lens[10], lens[70], lens[149] = 2100, 0, 1500
+    decode_case(device, 35, n_head, n_kv, hd, lens, 16, BF16, n_q=n_q)
+
+
 def test_decode_shared_pages(device):
     """Sequences that share a prefix's pages."""
     def share(c):
@@ -445,6 +454,22 @@ def test_prefill_bad_metadata(device, kind):
         close(out[s], ref[s], tol[s], "others")
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("bad", [0, 40, 61])
+def test_prefill_bad_page_and_odd_values(device, hd, bad):
+    """A page that is none in one part of a split tile, and an infinity among the values that only the last rows see."""
+    g = gen(95)
+    c = Cache(g, [4000, 90], 1, hd, 64, F16)
+    c.v[c.table[0, 3995 // 64].long(), 3995 % 64, 0, 5] = float("inf")
+    k, v, table, kv_len = c.to(device)
+    table[0, bad] = -7
+    q = torch.randn(60, 2 * hd, generator=g).to(F16).to(device)
+    out, lse = A.paged_prefill(q, k, v, table, kv_len, cu_of([30, 30], device), n_head=2, want_lse=True)
+    assert torch.isnan(out[:30]).all() and torch.isnan(lse[:30]).all()
+    ref, _, tol, _ = attend(c, q.cpu(), [30, 30], 2, hd ** -0.5, True, True, F16)
+    close(out[30:], ref[30:], tol[30:], "the other sequence")
+
+
 @pytest.mark.parametrize("cu", [[0, 999, 999], [0, -5, 30], [20, 10, 30], [0, 60, 2 ** 31 - 1]])
 def test_prefill_odd_ranges_stay_inside(device, cu):
     """Ranges of rows that pass the rows or run backwards: the call reads and writes its own rows only."""
@@ -575,6 +600,92 @@ def test_prefill_graph_replays(device):
             A.paged_prefill(q, k, v, table, kv_len, cu, n_head=8, out=ref, workspace=ws2)
             torch.cuda.synchronize()
             assert torch.equal(out, ref)
+
+
+class _General:
+    """An extension that takes no call: the general path runs."""
+
+    def __getattr__(self, name):
+        return lambda *a: None
+
+
+def test_extension_and_general_path(device, monkeypatch):
+    """The torch extension takes ordinary calls itself, and gives the bits of the general path."""
+    g = gen(114)
+    ext, taken = A._native(), []
+
+    class Counted:
+        def __getattr__(self, name):
+            def call(*a):
+                r = getattr(ext, name)(*a)
+                taken.append(r is not None)
+                return r
+            return call
+
+    lens, rows, n_head, n_kv, hd = [300, 20, 77], [100, 20, 1], 8, 2, 64
+    cu = cu_of(rows, device)
+    pos = torch.randint(0, 500, (2, 121), generator=g).to(torch.int32).to(device)
+    x = torch.randn(121, (n_head + 2 * n_kv) * hd, generator=g).to(device)
+    ws = A.new_workspace(A.paged_prefill_workspace_bytes(n_head=n_head, n_head_kv=n_kv, head_dim=hd, n_rows=121, n_seq=3, max_q=100,
+                                                         max_kv_len=400), device)
+    results = []
+    for native in (Counted(), _General()):
+        monkeypatch.setattr(A, "_native", lambda n=native: n)
+        c = Cache(gen(115), lens, n_kv, hd, 16, BF16)
+        k, v, table, kv_len = c.to(device)
+        where = (k, v, table, kv_len)
+        q = A.paged_store(x, *where, n_head=n_head, rope_mode=1, cu_q=cu, positions=pos, axis_pairs=(20, 12), axis_restart=True)
+        o, lse = A.paged_prefill(q, *where, cu, n_head=n_head, want_lse=True, max_q=100, workspace=ws)
+        o32, _ = A.paged_prefill(q, *where, cu, n_head=n_head, out_dtype=F32, causal=False, scale=0.3, workspace=ws)
+        d, dl = A.paged_decode(q[:6], *where, n_head=n_head, n_q=2, want_lse=True, max_kv_len=400, workspace=ws)
+        into = torch.zeros(6, n_head * hd + 8, dtype=BF16, device=device)
+        assert A.paged_decode(q[:6], *where, n_head=n_head, n_q=2, out=into, workspace=ws)[0] is into
+        results.append([q, k, v, o, lse, o32, d, dl, into])
+    assert taken == [True] * 5
+    for a, b in zip(*results):
+        assert a.dtype == b.dtype and torch.equal(a.nan_to_num(), b.nan_to_num())
+
+
+def test_front_end_refusals(device):
+    c = Cache(gen(116), [40, 40], 2, 64, 16, F16)
+    k, v, table, kv_len = c.to(device)
+    q = torch.zeros(2, 256, dtype=F16, device=device)
+    x = torch.zeros(2, 512, device=device)
+    cu = cu_of([1, 1], device)
+    ws = A.new_workspace(64 << 20, device)
+    bad = [dict(q=q.to(BF16)), dict(q=q.float()), dict(q=q[:, :128]), dict(q=q.cpu()), dict(q=q.t()), dict(v=v.to(BF16)), dict(v=v[:1]),
+           dict(k=k.cpu()), dict(k=k.transpose(2, 3)), dict(table=table.long()), dict(table=table[0]), dict(table=table.cpu()), dict(kv_len=kv_len[:1]),
+           dict(kv_len=kv_len.long()), dict(kv_len=kv_len.cpu())]
+    for wrong in bad:
+        a = dict(dict(q=q, k=k, v=v, table=table, kv_len=kv_len), **wrong)
+        for w in (None, ws):
+            with pytest.raises(ValueError):
+                A.paged_decode(a["q"], a["k"], a["v"], a["table"], a["kv_len"], n_head=4, workspace=w)
+            with pytest.raises(ValueError):
+                A.paged_prefill(a["q"], a["k"], a["v"], a["table"], a["kv_len"], cu, n_head=4, workspace=w)
+        if "q" not in wrong:
+            with pytest.raises(ValueError):
+                A.paged_store(x, a["k"], a["v"], a["table"], a["kv_len"], n_head=4, rope_mode=0)
+    for w in (None, ws):
+        with pytest.raises(ValueError, match="cu_q"):
+            A.paged_prefill(q, k, v, table, kv_len, cu.long(), n_head=4, workspace=w)
+        with pytest.raises(ValueError, match="cu_q"):
+            A.paged_prefill(q, k, v, table, kv_len, None, n_head=4, workspace=w)
+        with pytest.raises(ValueError, match="out"):
+            A.paged_decode(q, k, v, table, kv_len, n_head=4, out=q.to(BF16), workspace=w)
+        with pytest.raises(ValueError, match="lse"):
+            A.paged_decode(q, k, v, table, kv_len, n_head=4, lse=torch.zeros(2, 3, device=device), workspace=w)
+        with pytest.raises(ValueError, match="rows"):
+            A.paged_decode(q, k, v, table, kv_len, n_head=4, n_q=2, workspace=w)
+    with pytest.raises(_lib.MxAttnError):
+        wide = torch.cat([table, table.new_zeros(2, 200)], dim=1)  # room for sequences that are split, which needs a workspace
+        A.paged_decode(q, k, v, wide, kv_len, n_head=4, workspace=ws[:1 << 19])
+    for wrong in (dict(positions=torch.zeros(2, 2, dtype=torch.int32, device=device)), dict(positions=torch.zeros(2, device=device)),
+                  dict(axis_pairs=(16, 8)), dict(axis_pairs=(16, 16)), dict(q=q.to(BF16)), dict(rope_mode=3), dict(rope_base=0.5)):
+        with pytest.raises((ValueError, _lib.MxAttnError)):
+            A.paged_store(x, k, v, table, kv_len, **dict(dict(n_head=4, rope_mode=0), **wrong))
+    with pytest.raises(ValueError, match="qkv"):
+        A.paged_store(x[:, :448], k, v, table, kv_len, n_head=4, rope_mode=0)
 
 
 def test_two_streams(device):

@@ -197,10 +197,11 @@ int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
         plan.ranges = (int32_t)std::max<int64_t>(1, (plan.rt <= 8 ? 2 : 1) * kCUs / per_seq);
     } else {
         plan.whole_keys = d.head_dim == 64 ? 640 : 512;
-        plan.waves = d.head_dim == 256 || bound <= 128 || (d.head_dim == 128 && plan.rt <= 8 && bound > 512 && bound <= 4096) ? 4 : 8;
+        plan.waves = d.head_dim == 256 || bound <= 128 || (plan.rt <= 8 && bound > plan.whole_keys && bound <= 2048) ? 4 : 8;
+        if (plan.waves == 4) plan.whole_keys = 256;
         plan.ranges = (int32_t)std::max<int64_t>(d.n_seq, (plan.waves == 8 ? 1 : 2) * kCUs / per_seq);
         const int64_t n = quanta(plan.waves);
-        if (!plan.whole && n <= 32 && pairs * n <= 2 * kCUs) {
+        if (!plan.whole && n <= 32 && pairs * n <= (plan.waves == 8 ? 1 : 2) * kCUs) {
             plan.fixed = bound <= plan.whole_keys ? 1 : (int32_t)n;
             plan.ranges = d.n_seq * plan.fixed;
         }

@@ -32,10 +32,8 @@ __device__ __forceinline__ void publish2(float * p, float a, float b) {
     const uint64_t v = (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
     __hip_atomic_store(reinterpret_cast<uint64_t *>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ float2 collect2(const float * p) {
-    const uint64_t v = __hip_atomic_load(reinterpret_cast<uint64_t *>(const_cast<float *>(p)), __ATOMIC_RELAXED,
-                                         __HIP_MEMORY_SCOPE_AGENT);
-    return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+__device__ __forceinline__ u32x2 load8_dev(__amdgpu_buffer_rsrc_t r, int byte_off) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, byte_off, 0, kCpolSc1));
 }
 
 // Quanta of QK keys of a sequence. One at least: an empty sequence's rows are written too. whole: sequences are not split.
@@ -675,32 +673,40 @@ void paged_decode_kernel(PagedAttnParams p) {
                 float4_t * s_acc = reinterpret_cast<float4_t *>(s_row + RT);        // [stripe - 1][quad]
                 const int stripe = SF > 1 ? (int)threadIdx.x / NQ : 0;
                 auto quad = [&](int c) { return SF > 1 ? (int)threadIdx.x % NQ : (int)threadIdx.x + c * kThreads; };
+                // all rows' (m, l) of the wave and the first parts' quads are one round trip
+                constexpr int WR = (RT + NW - 1) / NW;
+                u32x2 ml[WR];
 #pragma unroll
-                for (int i0 = 0; i0 < RT; i0 += NW) {
-                    const int i = i0 + wave;
-                    if (i >= RT) break;
-                    const float2 ml = collect2(part + slot(min(lane, ns - 1)) + i * PR + HD);
-                    const float m = lane < ns ? ml.x : kNegInf;
-                    const float M = row16_max(xor16_max(xor32_max(m)));
-                    const float w = exp2_fast(m - (M == kNegInf ? 0.f : M));
-                    const float tot = row16_sum(xor16_add(xor32_add(lane < ns ? ml.y * w : 0.f)));
-                    if (lane < kMaxParts) s_w[lane * RT + i] = w;
-                    if (lane == 0) s_row[i] = make_float2(M, tot);
-                }
-                float4_t acc[CPT];
-#pragma unroll
-                for (int c = 0; c < CPT; c++) acc[c] = float4_t{0.f, 0.f, 0.f, 0.f};
-                bool first = true;
-                for (int s0 = stripe; s0 < ns || first; s0 += SF * MC) {
-                    u32x4 w[CPT][MC];
+                for (int r = 0; r < WR; r++)
+                    ml[r] = load8_dev(rsrc, 4 * (slot(min(lane, ns - 1)) + min(r * NW + wave, RT - 1) * PR + HD));
+                u32x4 w[CPT][MC];
+                auto fetch = [&](int s0) __attribute__((always_inline)) {
 #pragma unroll
                     for (int c = 0; c < CPT; c++) {
                         const int i = quad(c), at = i / (HD / 4) * PR + 4 * (i % (HD / 4));
 #pragma unroll
                         for (int e = 0; e < MC; e++) w[c][e] = load16_dev(rsrc, 4 * (at + slot(min(s0 + SF * e, ns - 1))));
                     }
-                    if (first) __syncthreads();  // the weights
-                    first = false;
+                };
+                fetch(stripe);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int r = 0; r < WR; r++) {
+                    const int i = r * NW + wave;
+                    if (i >= RT) break;
+                    const float m = lane < ns ? __uint_as_float(ml[r][0]) : kNegInf;
+                    const float M = row16_max(xor16_max(xor32_max(m)));
+                    const float w = exp2_fast(m - (M == kNegInf ? 0.f : M));
+                    const float tot = row16_sum(xor16_add(xor32_add(lane < ns ? __uint_as_float(ml[r][1]) * w : 0.f)));
+                    if (lane < kMaxParts) s_w[lane * RT + i] = w;
+                    if (lane == 0) s_row[i] = make_float2(M, tot);
+                }
+                lds_barrier();  // the weights
+                float4_t acc[CPT];
+#pragma unroll
+                for (int c = 0; c < CPT; c++) acc[c] = float4_t{0.f, 0.f, 0.f, 0.f};
+                for (int s0 = stripe; s0 < ns; s0 += SF * MC) {
+                    if (s0 != stripe) fetch(s0);
 #pragma unroll
                     for (int c = 0; c < CPT; c++) {
                         const int i = quad(c) / (HD / 4);

@@ -157,7 +157,7 @@ int32_t attn_params(const mx_paged_desc & d, const void * q, const void * k, con
 
 // ---- decode ----
 
-constexpr int kDecodeParts = 64;  // parts of a sequence at most (the merge takes one lane each)
+constexpr int kDecodeParts = 64;  // parts of a sequence at most: the join takes one lane each (131072 keys, Qwen2.5-7B heads, 54 us; with 33 67)
 constexpr int kCUs = 256;
 
 struct DecodePlan {
@@ -176,6 +176,8 @@ int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
     if ((int64_t)n_q * (d.n_head / d.n_head_kv) > 65536)
         return fail(MX_ATTN_UNSUPPORTED, "%d rows a sequence are a prompt (mx_paged_prefill)", n_q);
     plan.rows = n_q * (d.n_head / d.n_head_kv);
+    // A tile of 32 rows reads the keys once where two of 16 would twice (nine sequences of 201-5999 keys, 28 rows, 24 us against 31);
+    // at head dim 256 its registers do not fit.
     plan.rt = plan.rows > 16 && d.head_dim != 256 ? 32 : mx::decode_rows_per_tile(plan.rows);
     plan.n_rowtiles = (plan.rows + plan.rt - 1) / plan.rt;
     const int64_t per_seq = (int64_t)d.n_head_kv * plan.n_rowtiles, bound = kv_bound(d);
@@ -188,7 +190,10 @@ int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
         return fail(MX_ATTN_UNSUPPORTED, "%d sequences of up to %lld keys are more than one launch holds", d.n_seq,
                     (long long)std::max<int64_t>(bound, (int64_t)d.max_pages * d.page_size));
     plan.whole = bound <= 128;
-    // Ranges where the launch may hold several quanta of 128 keys for every workgroup, chunks below.
+    // Ranges where the launch may hold many quanta of 128 keys for every workgroup (64 sequences of 111-8191 keys, Llama-3-8B heads,
+    // 182 us against 227 of chunks), chunks below, where finding the range and joining over it cost more than its balance saves
+    // (64 of 100-2000, Qwen2.5-0.5B heads, 13.8 of chunks against 17.1; equal at 32 of 111-2000, Llama-3-8B heads, 33.7). Tiles of
+    // more rows join slower, so their bound is higher (32 rows, 32 sequences of 201-5999, 52 against 67).
     plan.by_ranges = d.n_seq > 1 && pairs * quanta(4) > (plan.rt <= 8 ? 16 : plan.rt == 16 ? 32 : 64) * kCUs;
     plan.fixed = 0;
     plan.whole_keys = 0;
@@ -196,10 +201,19 @@ int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
         plan.waves = 4;
         plan.ranges = (int32_t)std::max<int64_t>(1, (plan.rt <= 8 ? 2 : 1) * kCUs / per_seq);
     } else {
+        // A sequence of up to whole_keys keys is one chunk: joining costs 1 to 2 us more than the walk saves (513 keys, Qwen2.5-0.5B
+        // heads, 6.3 us against 7.4 split; 512 keys, Llama-3-8B heads, 8.2 against 8.6; 1000 keys 13.1 whole against 8.5). Beyond it
+        // 4 waves a workgroup, two on a CU, find the keys of a middling length on more CUs (1000 keys, Llama-3-8B heads, 7.35
+        // against 8.5 with 8 waves; 2000, Qwen2.5-0.5B heads, 7.2 against 7.6), and split shorter sequences too (8 of 100-1000 keys
+        // 9.5 against 10.4 with 512). Longer ones have fewer parts to join with 8 (4000 keys, Qwen2.5-7B heads, 9.8 against 10.6;
+        // 8192, Llama-3-8B heads, 11.3 against 14.8), and so have tiles of more rows. At head dim 256 the LDS holds 4 waves.
         plan.whole_keys = d.head_dim == 64 ? 640 : 512;
         plan.waves = d.head_dim == 256 || bound <= 128 || (plan.rt <= 8 && bound > plan.whole_keys && bound <= 2048) ? 4 : 8;
         if (plan.waves == 4) plan.whole_keys = 256;
         plan.ranges = (int32_t)std::max<int64_t>(d.n_seq, (plan.waves == 8 ? 1 : 2) * kCUs / per_seq);
+        // Where one round of workgroups has room for every quantum of every sequence the chunks need no planning from the lengths:
+        // one round trip less (8192 keys, Llama-3-8B heads, 11.3 us against 12.0). Beyond a round the empty ones cost more
+        // (16 sequences of 100-4000 keys, Qwen2.5-0.5B heads, 13.2 against 10.7 planned).
         const int64_t n = quanta(plan.waves);
         if (!plan.whole && n <= 32 && pairs * n <= (plan.waves == 8 ? 1 : 2) * kCUs) {
             plan.fixed = bound <= plan.whole_keys ? 1 : (int32_t)n;

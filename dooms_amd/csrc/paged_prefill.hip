@@ -5,7 +5,9 @@
 // times v, with the running maximum m and sum l of a row in f32: O <- O e^(m - m') + sum_j e^(s_j - m') v_j.
 //
 // What bounds it: 4 n_head head_dim flops per (row, key) pair on the matrix cores; the softmax's exponentials on the vector
-// ALUs fill most of the time between the products. Short prompts add what a tile costs beside its keys.
+// ALUs fill most of the time between the products (two chunks of 1.5k-2k rows behind 14k keys, Qwen2.5-7B heads, 735 GFLOP in 743 us,
+// 990 TFLOP/s; a large library product of the type reaches 1142). Short prompts add what a tile costs beside its keys, about 3 us
+// of queries, outputs and first loads (12 prompts of 65-1711 rows, Llama-3-8B heads, 104 GFLOP in 156 us).
 //
 //   * A tile is W waves of 32 query rows: W / HPW row tiles of each of HPW heads that share a kv head, so that a short or causal
 //     tile wastes few rows and the keys serve all of them. Steps are 64 keys; keys and values go straight into LDS

@@ -359,6 +359,8 @@ def _paged_desc(rows, k_pages, v_pages, page_table, kv_len, cu_q, n_head, max_q=
     if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
         raise ValueError("page_table must be an int32 [sequences][pages] tensor with unit stride along the pages")
     n_seq = page_table.shape[0]
+    if n_seq > 1 and page_table.stride(0) < page_table.shape[1]:
+        raise ValueError("the rows of page_table overlap")
     if kv_len.dtype != torch.int32 or kv_len.shape != (n_seq,) or not kv_len.is_contiguous():
         raise ValueError("kv_len must be a contiguous int32 tensor with an entry per sequence")
     if cu_q is not None and (cu_q.dtype != torch.int32 or cu_q.shape != (n_seq + 1,) or not cu_q.is_contiguous()):

@@ -400,6 +400,7 @@ struct Paged {
         need(k.dim() == 4 && k.stride(3) == 1 && (type == at::kHalf || type == at::kBFloat16));
         need(v.scalar_type() == type && v.sizes() == k.sizes() && v.strides() == k.strides());
         need(table.scalar_type() == at::kInt && (table.stride(1) == 1 || table.size(1) <= 1));
+        need(table.size(0) <= 1 || table.stride(0) >= table.size(1));
         for (int64_t n : {k.size(0), k.size(1), k.size(2), k.size(3), table.size(0), table.size(1), rows.size(0)}) need(n <= INT32_MAX);
         d.n_head = int32(n_head);
         d.n_head_kv = (int32_t)k.size(2);

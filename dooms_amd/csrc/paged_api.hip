@@ -215,7 +215,7 @@ int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
         // one round trip less (8192 keys, Llama-3-8B heads, 11.3 us against 12.0). Beyond a round the empty ones cost more
         // (16 sequences of 100-4000 keys, Qwen2.5-0.5B heads, 13.2 against 10.7 planned).
         const int64_t n = quanta(plan.waves);
-        if (!plan.whole && n <= 32 && pairs * n <= (plan.waves == 8 ? 1 : 2) * kCUs) {
+        if (bound <= plan.whole_keys || (n <= 32 && pairs * n <= (plan.waves == 8 ? 1 : 2) * kCUs)) {
             plan.fixed = bound <= plan.whole_keys ? 1 : (int32_t)n;
             plan.ranges = d.n_seq * plan.fixed;
         }

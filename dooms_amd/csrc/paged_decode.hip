@@ -116,22 +116,32 @@ struct Range {
     int32_t b, at;
 };
 
-// Range r: every wave sums all lengths (64 a step) and looks for the sequence that holds its first quantum.
+// Range r: every wave sums all lengths, each lane those of per_lane sequences in a row, and looks for the sequence that holds its
+// first quantum. lens: the lengths of the 64 sequences from lens0 on, that one among them.
 template <int QK>
-__device__ __forceinline__ Range find_range(const PagedAttnParams & p, int r, int lane, int & lens) {
-    const int n_seq = p.c.n_seq;
+__device__ __forceinline__ Range find_range(const PagedAttnParams & p, int r, int lane, int & lens, int & lens0) {
+    const int n_seq = p.c.n_seq, per_lane = (n_seq + kWave - 1) / kWave;
     lens = p.c.kv_len[min(lane, n_seq - 1)];
-    auto quanta = [&](int base) {
-        const int len = base == 0 ? lens : p.c.kv_len[min(base + lane, n_seq - 1)];
-        return base + lane < n_seq ? quanta_of<QK>(p, len) : 0;
-    };
-    int sum = 0, most = 0;
-    for (int base = 0; base < n_seq; base += kWave) {
-        const int n = quanta(base);
-        sum += n;
-        most = max(most, n);
+    lens0 = 0;
+    int mine = 0, most = 0;
+    if (per_lane == 1) {
+        mine = most = lane < n_seq ? quanta_of<QK>(p, lens) : 0;
+    } else {
+        constexpr int kAtOnce = 8;
+        for (int i0 = 0; i0 < per_lane; i0 += kAtOnce) {
+            int len[kAtOnce];
+#pragma unroll
+            for (int e = 0; e < kAtOnce; e++) len[e] = p.c.kv_len[min(lane * per_lane + i0 + e, n_seq - 1)];
+#pragma unroll
+            for (int e = 0; e < kAtOnce; e++) {
+                const bool in = i0 + e < per_lane && lane * per_lane + i0 + e < n_seq;
+                const int n = in ? quanta_of<QK>(p, len[e]) : 0;
+                mine += n;
+                most = max(most, n);
+            }
+        }
     }
-    sum = wave_isum(sum);
+    const int sum = wave_isum(mine);
     most = wave_imax(most);
     // an equal share each, and no more parts of a sequence than the merge takes (a part may start within a range: one more)
     Range x;
@@ -142,16 +152,25 @@ __device__ __forceinline__ Range find_range(const PagedAttnParams & p, int r, in
     x.b = -1;
     x.at = 0;
     if (x.lo >= x.hi) return x;
-    for (int base = 0; base < n_seq; base += kWave) {
-        const int n = quanta(base), upto = x.at + wave_iscan(n);
-        const uint64_t past = __builtin_amdgcn_ballot_w64(upto > x.lo);
+    const int upto = wave_iscan(mine);
+    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > x.lo));  // lo < sum: there is one
+    x.b = l * per_lane;
+    x.at = __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l);
+    const int end = min(x.b + per_lane, n_seq);
+    while (per_lane > 1) {  // among the lane's sequences
+        lens0 = x.b;
+        lens = p.c.kv_len[min(lens0 + lane, n_seq - 1)];
+        const int n = lens0 + lane < end ? quanta_of<QK>(p, lens) : 0, to = x.at + wave_iscan(n);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(to > x.lo);
         if (past) {
-            const int l = __builtin_ctzll(past);
-            x.b = base + l;
-            x.at = __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l);
-            return x;
+            const int i = __builtin_ctzll(past);
+            x.b = lens0 + i;
+            x.at = __builtin_amdgcn_readlane(to, i) - __builtin_amdgcn_readlane(n, i);
+            break;
         }
-        x.at = __builtin_amdgcn_readlane(upto, 63);
+        x.at = __builtin_amdgcn_readlane(to, 63);
+        x.b = min(lens0 + kWave, n_seq - 1);
+        if (lens0 + kWave >= end) break;  // only where lengths changed meanwhile
     }
     return x;
 }
@@ -263,12 +282,8 @@ void paged_decode_kernel(PagedAttnParams p) {
         s.b = -1;
     };
     if constexpr (RANGES) {
-        x = find_range<kStep>(p, r, lane, lens);
+        x = find_range<kStep>(p, r, lane, lens, lens0);
         if (x.b < 0) return;  // uniform over the workgroup
-        if (x.b >= kWave) {
-            lens0 = x.b;
-            lens = p.c.kv_len[min(lens0 + lane, n_seq - 1)];
-        }
         seg.b = x.b;
         seg.at = x.at;
         key0 = segment(seg, __builtin_amdgcn_readlane(lens, x.b - lens0));

@@ -68,17 +68,25 @@ __global__ __launch_bounds__(512) void paged_store_kernel(PagedStoreParams p) {
     // the row's sequence, its new rows and the row among them; a row behind the last sequence is left alone
     int b = -1, n = p.n_q, t = 0, len = 0;
     if (p.cu_q) {
-        for (int base = 0; base < p.c.n_seq; base += kWave) {
-            const int i = min(base + lane, p.c.n_seq - 1);
+        // 64 probes a step narrow many sequences to 64 (the offsets ascend)
+        int first = 0, left = p.c.n_seq;
+        while (left > kWave) {
+            const int step = (left + kWave - 1) / kWave;
+            const uint64_t below = __builtin_amdgcn_ballot_w64(lane * step < left && p.cu_q[min(first + lane * step, p.c.n_seq)] <= row);
+            const int skip = max(__builtin_popcountll(below) - 1, 0) * step;
+            first += skip;
+            left = min(step, left - skip);
+        }
+        {
+            const int i = min(first + lane, p.c.n_seq - 1);
             const int lo = min(max(p.cu_q[i], 0), p.n_rows), hi = min(max(p.cu_q[i + 1], 0), p.n_rows), ln = p.c.kv_len[i];
-            const uint64_t in = __builtin_amdgcn_ballot_w64(base + lane < p.c.n_seq && lo <= row && row < hi);
+            const uint64_t in = __builtin_amdgcn_ballot_w64(lane < left && lo <= row && row < hi);
             if (in) {
                 const int l = __builtin_ctzll(in);
-                b = base + l;
+                b = first + l;
                 t = row - __builtin_amdgcn_readlane(lo, l);
                 n = __builtin_amdgcn_readlane(hi, l) - __builtin_amdgcn_readlane(lo, l);
                 len = __builtin_amdgcn_readlane(ln, l);
-                break;
             }
         }
         if (b < 0) return;

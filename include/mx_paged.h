@@ -100,7 +100,7 @@ MX_ATTN_API int32_t mx_paged_store(const mx_paged_desc * desc, const mx_paged_ro
  *
  *   q          device, [n_rows][row_stride] of dtype, rotated; rows of sequence b start at b * n_rows / n_seq
  *   k, v       device, the pools
- *   out        device, [n_rows][out_stride] of row_dtype
+ *   out        device, [n_rows][out_stride] of row_dtype; must not overlap q
  *   lse        device f32, [n_rows][n_head], natural-log log-sum-exp of the scaled scores, or NULL
  *   workspace  device, 256-byte aligned, at least mx_paged_decode_workspace_bytes(desc) bytes, zeroed once by
  *              mx_attn_decode_workspace_init; every call leaves its counters at zero, and one workspace may serve this call,

@@ -108,6 +108,13 @@ def test_store_one_sequence_of_many(device):
     store_case(device, 11, 4, 2, 64, rows, [1 + b % 40 for b in range(200)], 16, F16, F32, 0)
 
 
+@pytest.mark.parametrize("n_seq", [64, 65, 129, 4097])
+def test_store_many_sequences(device, n_seq):
+    """The sequence of a row among many, runs of empty ones at the start, in between and at the end."""
+    rows = [0 if b < 5 or 30 <= b < 50 or b > n_seq - 7 else b % 3 for b in range(n_seq)]
+    store_case(device, 12, 2, 1, 64, rows, [n + b % 20 for b, n in enumerate(rows)], 16, BF16, F16, 1, tail=2)
+
+
 def test_store_many_rows(device):
     """More rows than a grid has workgroups along one dimension, and offsets past 2^32 bytes."""
     n = (1 << 22) + 5
@@ -211,6 +218,13 @@ def test_decode_long(device, max_kv_len):
     """Many splits, whatever the hint says of the length."""
     decode_case(device, 27, 8, 8, 128, [4000], 16, F16, max_kv_len=max_kv_len)
     decode_case(device, 28, 14, 2, 64, [9000, 100], 64, BF16, max_kv_len=max_kv_len)
+
+
+@pytest.mark.parametrize("longest", [100, 400])
+def test_decode_thousands_of_sequences(device, longest):
+    lens = [(b * 37) % 90 for b in range(4500)]
+    lens[7], lens[4499] = longest, longest - 3
+    decode_case(device, 36, 4, 2, 64, lens, 16, F16)
 
 
 @pytest.mark.parametrize("n_seq,n_q", [(65, 1), (130, 2), (700, 1)])
@@ -654,7 +668,7 @@ def test_front_end_refusals(device):
     cu = cu_of([1, 1], device)
     ws = A.new_workspace(64 << 20, device)
     bad = [dict(q=q.to(BF16)), dict(q=q.float()), dict(q=q[:, :128]), dict(q=q.cpu()), dict(q=q.t()), dict(v=v.to(BF16)), dict(v=v[:1]),
-           dict(k=k.cpu()), dict(k=k.transpose(2, 3)), dict(table=table.long()), dict(table=table[0]), dict(table=table.cpu()), dict(kv_len=kv_len[:1]),
+           dict(k=k.cpu()), dict(k=k.transpose(2, 3)), dict(table=table.long()), dict(table=table[0]), dict(table=table.cpu()), dict(table=table[:1].expand(2, -1)), dict(kv_len=kv_len[:1]),
            dict(kv_len=kv_len.long()), dict(kv_len=kv_len.cpu())]
     for wrong in bad:
         a = dict(dict(q=q, k=k, v=v, table=table, kv_len=kv_len), **wrong)

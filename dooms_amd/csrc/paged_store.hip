@@ -61,15 +61,10 @@ __global__ __launch_bounds__(512) void paged_store_kernel(PagedStoreParams p) {
         w[0] = load16(at);
         w[1] = load16(at + HALF * (IN == 0 ? 4 : 2));
     };
-    u32x4 w[AHEAD][2];
-#pragma unroll
-    for (int a = 0; a < AHEAD; a++) load(threadIdx.x + a * blockDim.x, w[a]);
-
-    // the row's sequence, its new rows and the row among them; a row behind the last sequence is left alone
-    int b = -1, n = p.n_q, t = 0, len = 0;
+    // the candidates for the row's sequence, one a lane: sent for ahead of the row itself, so that the wait for them leaves it in
+    // flight; 64 probes a step narrow many sequences to 64 (the offsets ascend)
+    int first = 0, left = p.c.n_seq, lo = 0, hi = 0, ln = 0;
     if (p.cu_q) {
-        // 64 probes a step narrow many sequences to 64 (the offsets ascend)
-        int first = 0, left = p.c.n_seq;
         while (left > kWave) {
             const int step = (left + kWave - 1) / kWave;
             const uint64_t below = __builtin_amdgcn_ballot_w64(lane * step < left && p.cu_q[min(first + lane * step, p.c.n_seq)] <= row);
@@ -77,17 +72,27 @@ __global__ __launch_bounds__(512) void paged_store_kernel(PagedStoreParams p) {
             first += skip;
             left = min(step, left - skip);
         }
-        {
-            const int i = min(first + lane, p.c.n_seq - 1);
-            const int lo = min(max(p.cu_q[i], 0), p.n_rows), hi = min(max(p.cu_q[i + 1], 0), p.n_rows), ln = p.c.kv_len[i];
-            const uint64_t in = __builtin_amdgcn_ballot_w64(lane < left && lo <= row && row < hi);
-            if (in) {
-                const int l = __builtin_ctzll(in);
-                b = first + l;
-                t = row - __builtin_amdgcn_readlane(lo, l);
-                n = __builtin_amdgcn_readlane(hi, l) - __builtin_amdgcn_readlane(lo, l);
-                len = __builtin_amdgcn_readlane(ln, l);
-            }
+        const int i = min(first + lane, p.c.n_seq - 1);
+        lo = p.cu_q[i];
+        hi = p.cu_q[i + 1];
+        ln = p.c.kv_len[i];
+    }
+    u32x4 w[AHEAD][2];
+#pragma unroll
+    for (int a = 0; a < AHEAD; a++) load(threadIdx.x + a * blockDim.x, w[a]);
+
+    // the row's sequence, its new rows and the row among them; a row behind the last sequence is left alone
+    int b = -1, n = p.n_q, t = 0, len = 0;
+    if (p.cu_q) {
+        lo = min(max(lo, 0), p.n_rows);
+        hi = min(max(hi, 0), p.n_rows);
+        const uint64_t in = __builtin_amdgcn_ballot_w64(lane < left && lo <= row && row < hi);
+        if (in) {
+            const int l = __builtin_ctzll(in);
+            b = first + l;
+            t = row - __builtin_amdgcn_readlane(lo, l);
+            n = __builtin_amdgcn_readlane(hi, l) - __builtin_amdgcn_readlane(lo, l);
+            len = __builtin_amdgcn_readlane(ln, l);
         }
         if (b < 0) return;
     } else {

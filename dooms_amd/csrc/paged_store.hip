@@ -6,9 +6,9 @@
 //
 // Byte work: each q|k|v element is read once and written once at half the width or the same. One workgroup per token row; a
 // thread holds two pieces of 16 bytes, half a head apart, so that both rotary layouts find their partners in one thread and
-// every load and store of a wave is contiguous. The row's loads go out first; behind them come the sequence, its length and
-// its page (three dependent reads), and the head_dim / 2 angles, turned into (cos, sin) once for all heads of the row. 179 MB of
-// packed prompts take 32.5 us (5.5 TB/s, a large copy reaches 5.0); a decode step's row 2.9 us, of which an empty launch is 2.
+// every load and store of a wave is contiguous. The sequence is looked up first, then the row's loads go out, behind them
+// the page, and the head_dim / 2 angles, turned into (cos, sin) once for all heads of the row. 179 MB of
+// packed prompts take 31.5 us (5.7 TB/s, a large copy reaches 5.0); a decode step's row 2.8 us, of which an empty launch is 2.
 #include "mx_paged.hpp"
 
 #include <algorithm>

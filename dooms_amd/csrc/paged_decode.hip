@@ -683,7 +683,10 @@ void paged_decode_kernel(PagedAttnParams p) {
                 // ---- join the parts: weights 2^(m - M) of every (part, row), one lane per part, then the accumulator's quads, each
                 // quad's parts striped over SF threads ----
                 constexpr int SF = kThreads >= NQ ? kThreads / NQ : 1, CPT = NQ > kThreads ? NQ / kThreads : 1;
-                constexpr int MC = CPT > 2 ? 4 : 8;  // parts of a quad in flight
+                // Parts of a quad in flight: as many as the registers hold (32 rows at head dim 128, 12 parts, 17.7 us with 8, 17.0
+                // with 12). Past the last part the lanes load it again, or at head dim 64, whose launches have fewer parts, nothing
+                // (7 parts 8.0 -> 7.55 us, but 32 parts at head dim 128 11.55 -> 11.75).
+                constexpr int MC = CPT > 2 ? 4 : CPT == 2 ? 12 : 8;
                 static_assert(kMaxParts <= kWave, "one lane per part");
                 static_assert((kMaxParts * RT + 2 * RT) * 4 + (SF - 1) * NQ * 16 <= (int64_t)sizeof(s_buf), "merge scratch");
                 float * s_w = reinterpret_cast<float *>(s_buf);                     // [part][row]
@@ -703,7 +706,10 @@ void paged_decode_kernel(PagedAttnParams p) {
                     for (int c = 0; c < CPT; c++) {
                         const int i = quad(c), at = i / (HD / 4) * PR + 4 * (i % (HD / 4));
 #pragma unroll
-                        for (int e = 0; e < MC; e++) w[c][e] = load16_dev(rsrc, 4 * (at + slot(min(s0 + SF * e, ns - 1))));
+                        for (int e = 0; e < MC; e++) {
+                            if (HD == 64 && s0 + SF * e >= ns) continue;
+                            w[c][e] = load16_dev(rsrc, 4 * (at + slot(min(s0 + SF * e, ns - 1))));
+                        }
                     }
                 };
                 fetch(stripe);

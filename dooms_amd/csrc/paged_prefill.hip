@@ -332,7 +332,8 @@ void paged_prefill_kernel(PagedAttnParams p) {
         int ahead;               // 1: it is of the tile behind the current one
     } fd;
     int bad = 0, bad_next = 0;  // a lane's sign bit: a page of the current tile's (the next one's) steps is none
-    int sent = 0, put = 0;      // steps in flight or unread, the buffer of the next
+    int sent = 0, put = 0;      // steps in flight or unread, the buffer of the next ...
+    int take = 0;               // ... and of the oldest
     auto feed_from = [&](const Tile & t, int ahead) __attribute__((always_inline)) {
         fd.head = 2 * (int64_t)t.kvh * p.c.head_stride;
         fd.table = p.c.table + t.b * p.c.table_stride;
@@ -396,6 +397,22 @@ void paged_prefill_kernel(PagedAttnParams p) {
         asm volatile("" ::: "memory");
     };
 
+    // The values that this wave loaded behind a sequence's last key (the loads repeat it) become zeros: its rows multiply them by
+    // probabilities of 0, which an infinity among them would turn into NaN. By asm, as the operands' reads are, so that no load in
+    // flight is waited for.
+    const uint32_t v_mine = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint16_t *)sm.v[0] + 1024 * wave + 16 * lane;
+    auto zero_behind = [&](int kb, int L) __attribute__((always_inline)) {
+        if (kb + my_rows + lrow >= L) {
+            const uint32_t at = v_mine + take * (uint32_t)sizeof(sm.v[0]);
+            static_for<0, NI>([&](auto I) __attribute__((always_inline)) {
+                const uint32_t a = at;
+                const u32x4 zero = {0u, 0u, 0u, 0u};
+                asm volatile("ds_write_b128 %0, %1 offset:%2" ::"v"(a), "v"(zero), "i"(1024 * W * decltype(I)::value) : "memory");
+            });
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    };
+
     // ---- the wave's rows of a tile ----
     const int l32 = lane % 32, hgrp = lane / 32;
     const int rt = wave % RPW;
@@ -417,7 +434,6 @@ void paged_prefill_kernel(PagedAttnParams p) {
     for (int b = 0; b < 2; b++) dl_k[b] = 512 * (l32 / 16) + 32 * (l32 % 16) + 8 * ((2 * b + hgrp) ^ ((l32 % 16) / 4));
     const int dl_v = (4 * hgrp + (lane % 16) / 4) * 32 + 16 * ((lane / 16) % 2) + 4 * (lane % 4);
     const float c = p.scale_log2;
-    int take = 0;          // the buffer of the oldest step
     bool waited = false;   // for its loads
 
     for (;;) {
@@ -460,6 +476,7 @@ void paged_prefill_kernel(PagedAttnParams p) {
             const int kb = ib * kBK;
             if (!waited) wait_step();
             waited = false;
+            if (kb + kBK > L) zero_behind(kb, L);
             __builtin_amdgcn_s_barrier();  // every wave's loads of the step are complete, and the buffer refilled below is read
             asm volatile("" ::: "memory");
             const int buf = take;

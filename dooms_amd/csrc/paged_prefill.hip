@@ -122,11 +122,12 @@ __device__ __forceinline__ void row_alone(const PagedAttnParams & p, const Tile 
 #pragma unroll
         for (int d = 0; d < HD / 64; d++) s += q[d] * one(p.c.k[at + 64 * d]);
         s = wave_sum(s) * p.scale_log2;
-        const float mn = fmaxf(m, s);
-        const float corr = m == kNegInf ? 0.f : exp2_fast(m - mn), w = exp2_fast(s - mn);
+        // scores of -inf alone (keys that hold an infinity) weigh 2^-inf = 0 each, and leave the maximum to the first finite one
+        const float mn = fmaxf(m, s), use = mn == kNegInf ? 0.f : mn;
+        const float corr = exp2_fast(m - use), w = exp2_fast(s - use);
         l = l * corr + w;
 #pragma unroll
-        for (int d = 0; d < HD / 64; d++) o[d] = (m == kNegInf ? 0.f : o[d] * corr) + w * one(p.c.v[at + 64 * d]);
+        for (int d = 0; d < HD / 64; d++) o[d] = o[d] * corr + w * one(p.c.v[at + 64 * d]);
         m = mn;
     }
     if (bad) l = __builtin_nanf("");

@@ -4,7 +4,9 @@ import math
 import pytest
 import torch
 
-from test_paged_gpu import BF16, F16, F32, poke, prefill_case
+from dooms_amd import attention as A
+from paged_helpers import Cache, attend, close
+from test_paged_gpu import BF16, F16, F32, cu_of, gen, poke, prefill_case
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +34,26 @@ def test_prefill_infinity_among_the_last_keys(device, hd, n_head, n_kv, long, va
         prefill_case(device, 120, n_head, n_kv, hd, [rows, 20], [L, 40], 16, F16, mutate=wide(m) if long else m, what=f"{rows} {L} {at}")
         prefill_case(device, 120, n_head, n_kv, hd, [rows, 20], [L, 40], 32, BF16, causal=False, mutate=wide(m) if long else m,
                      what=f"not causal {rows} {L} {at}")
+
+
+@pytest.mark.parametrize("hd,long", [(64, False), (128, False), (128, True), (256, False)])
+def test_prefill_scores_of_minus_infinity_first(device, hd, long):
+    """The first keys' scores are -inf, so they weigh nothing, and rows before an infinity among the values are computed by
+    themselves: the weights start at the first finite score. The definition is evaluated with finite keys whose weight is
+    below 10^-100 instead, as its tolerance knows no infinities."""
+    g = gen(121)
+    c = Cache(g, [75, 50], 1, hd, 16, F16)
+    (wide(poke(0, 74, 0, 5, math.inf)) if long else poke(0, 74, 0, 5, math.inf))(c)
+    q = torch.randn(80, 2 * hd, generator=g)
+    q[:, 3] = q[:, 3].abs().clamp_min(0.5)
+    q[:, hd + 3] = q[:, hd + 3].abs().clamp_min(0.5)
+    q = q.to(F16)
+    for pos in (0, 1, 2):
+        poke(0, pos, 0, 3, -math.inf, "k")(c)
+    k, v, table, kv_len = c.to(device)
+    out, lse = A.paged_prefill(q.to(device), k, v, table, kv_len, cu_of([60, 20], device), n_head=2, scale=0.125, want_lse=True)
+    for pos in (0, 1, 2):
+        poke(0, pos, 0, 3, -30000.0, "k")(c)
+    ref, rlse, tol, ltol = attend(c, q, [60, 20], 2, 0.125, True, True, F16)
+    close(out, ref, tol, "out")
+    close(lse, rlse, ltol, "lse")

@@ -345,7 +345,8 @@ void paged_prefill_kernel(PagedAttnParams p) {
     };
     auto ids_at = [&](int step) { return fd.table + (min(step * kBK + 16 * (lane % RB), fd.L - 1) >> shift); };
     // The page numbers of fd's step go to LDS on the same in-order queue as the steps, ahead of the loads of the step before: the
-    // wait for an older step then covers them, and no register waits for them.
+    // wait for an older step then covers them, and no register waits for them. Every take_ids() lies behind a wait issued after the
+    // request_ids() that it reads from.
     auto request_ids = [&]() __attribute__((always_inline)) {
         __builtin_amdgcn_global_load_lds(ids_at(fd.step), (__attribute__((address_space(3))) void *)&sm.ids[wave][0], 4, 0, 0);
     };
@@ -449,6 +450,7 @@ void paged_prefill_kernel(PagedAttnParams p) {
         // the first tile's steps, and what the tiles behind were too short for (the buffer read last is not among those filled)
         if (sent < NBUF - 1) {
             while (sent < NBUF - 1 && more()) {
+                waited = false;  // page numbers requested here are not covered by the wait at the last tile's end
                 // two steps' page numbers at once
                 const bool two = NBUF > 2 && sent == 0 && fd.step + 1 < fd.end;
                 int i0 = *ids_at(fd.step), i1 = *ids_at(two ? fd.step + 1 : fd.step);

@@ -57,3 +57,13 @@ def test_prefill_scores_of_minus_infinity_first(device, hd, long):
     ref, rlse, tol, ltol = attend(c, q, [60, 20], 2, 0.125, True, True, F16)
     close(out, ref, tol, "out")
     close(lse, rlse, ltol, "lse")
+
+
+@pytest.mark.parametrize("hd,n_head,n_kv,dtype,long", [(64, 4, 2, F16, False), (128, 2, 2, BF16, True), (128, 8, 2, F16, True), (128, 4, 1, F16, False),
+                                                       (256, 2, 1, BF16, False)])
+def test_prefill_tiles_of_one_step_before_longer_ones(device, hd, n_head, n_kv, dtype, long):
+    """Ranges whose tiles of one step leave the next tile's page numbers to be requested between two tiles: every step attends
+    the keys of its own pages."""
+    lens = [(60, 33, 200, 64, 500, 1)[b % 6] for b in range(330)]
+    prefill_case(device, 122, n_head, n_kv, hd, [min(L, 1 + b % 3) for b, L in enumerate(lens)], lens, 16, dtype,
+                 mutate=wide() if long else None)

@@ -714,8 +714,11 @@ int64_t prefill_split_keys(const mx_attn_desc & d) {
     if (d.causal) return (int64_t)d.p0 + d.n_q;
     return d.n_kv == 0 ? (int64_t)d.p0 + d.n_q : d.n_kv;
 }
-// workspace of the split route: the decode workspace, then (for mx_attn_prefill_rope_ws) the rotated f32 query rows
-size_t prefill_split_q_offset(const mx_attn_desc & d, int32_t L) { return (decode_ws_bytes(&d, 1, L) + 255) / 256 * 256; }
+// workspace of the split route: the decode workspace, then (for mx_attn_prefill_rope_ws) the rotated f32 query rows, behind
+// the counters also where this chunk's own plan needs none: the next call on the workspace may
+size_t prefill_split_q_offset(const mx_attn_desc & d, int32_t L) {
+    return (std::max(decode_ws_bytes(&d, 1, L), kCounterRegion) + 255) / 256 * 256;
+}
 
 // ---- IR SelfAttention (src/ir/op.h:31-32) ----
 

@@ -312,7 +312,8 @@ MX_ATTN_API size_t mx_self_attention_workspace_bytes(const mx_self_attn_desc * d
  *
  *   qkv        device, [batch][n_tok][3 embed] of desc->dtype, contiguous, 16-byte aligned
  *   y          device, [batch][n_tok][embed] of desc->dtype, contiguous, 16-byte aligned, not overlapping qkv
- *   workspace  device, 256-byte aligned, at least mx_self_attention_workspace_bytes(desc) bytes (NULL when that is 0)
+ *   workspace  device, 256-byte aligned, at least mx_self_attention_workspace_bytes(desc) bytes (NULL when that is 0). It
+ *              holds packed rows from its start on: not one whose counters a decode or prefill call relies on
  */
 MX_ATTN_API int32_t mx_self_attention(const mx_self_attn_desc * desc, const void * qkv, void * y, void * workspace,
                                       size_t ws_bytes, mx_attn_stream stream);

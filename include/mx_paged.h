@@ -104,8 +104,10 @@ MX_ATTN_API int32_t mx_paged_store(const mx_paged_desc * desc, const mx_paged_ro
  *   lse        device f32, [n_rows][n_head], natural-log log-sum-exp of the scaled scores, or NULL
  *   workspace  device, 256-byte aligned, at least mx_paged_decode_workspace_bytes(desc) bytes, zeroed once by
  *              mx_attn_decode_workspace_init; every call leaves its counters at zero, and one workspace may serve this call,
- *              mx_paged_prefill and the calls of mx_attn.h. Calls that share it (captured ones too) must be ordered.
- *              NULL is allowed when the size needed is 0.
+ *              mx_paged_prefill and the calls of mx_attn.h that keep such counters (mx_attn_decode, _decode_f32, _decode_rope,
+ *              _prefill_ws and _prefill_rope_ws), but not mx_self_attention or mx_linear, which write their rows where the
+ *              counters lie. Calls that share it (captured ones too) must be ordered. NULL is allowed when the size needed
+ *              is 0.
  */
 MX_ATTN_API int32_t mx_paged_decode(const mx_paged_desc * desc, const void * q, const void * k, const void * v,
                                     const int32_t * table, const int32_t * kv_len, void * out, float * lse, void * workspace,

@@ -38,3 +38,36 @@ def test_short_prompt_then_split_decode(device, n_head, n_kv, hd, n_q):
         assert torch.equal(out, alone)
         assert not ws[:COUNTERS].any()
         assert torch.equal(A.decode(q, [k], [v], [5000], workspace=ws, **heads)[0], want)
+
+
+@pytest.mark.gpu
+def test_every_call_that_keeps_counters(device):
+    """The calls that may share a workspace, each split, in turn on one: the results of a workspace of their own, and the counters
+    at zero behind each."""
+    g = torch.Generator().manual_seed(2)
+    n_head, n_kv, hd, L = 16, 4, 128, 3000
+    heads = dict(n_head=n_head, n_head_kv=n_kv, head_dim=hd)
+    rnd = lambda *s: torch.randn(*s, generator=g).to(device)
+    q, qkv = rnd(40, n_head * hd).half(), rnd(40, (n_head + 2 * n_kv) * hd)
+    k, v = rnd(L, n_kv * hd).half(), rnd(L, n_kv * hd).half()
+    pages = [rnd(400, 16, n_kv, hd).half() for _ in range(2)]
+    table = torch.randperm(400, generator=g).to(torch.int32).view(2, 200).to(device)
+    lens = torch.tensor([3200, 1500], dtype=torch.int32, device=device)
+    cu = torch.tensor([0, 30, 40], dtype=torch.int32, device=device)
+    calls = [
+        lambda ws: A.decode(q[:1], [k], [v], [L], workspace=ws, **heads)[0],
+        lambda ws: A.paged_decode(q[:2], *pages, table, lens, n_head=n_head, workspace=ws)[0],
+        lambda ws: A.decode(q[:1].float(), [k], [v], [L], workspace=ws, **heads)[0],
+        lambda ws: A.decode_rope(qkv[:1], [k.clone()], [v.clone()], [L], rope_mode=1, workspace=ws, **heads)[0],
+        lambda ws: A.paged_prefill(q, *pages, table, lens, cu, n_head=n_head, workspace=ws)[0],
+        lambda ws: A.prefill(q, k, v, p0=L - 40, workspace=ws, **heads)[0],
+        lambda ws: A.paged_decode(q[:16], *pages, table, lens, n_head=n_head, n_q=8, workspace=ws)[0],
+        lambda ws: A.prefill_rope(qkv, k.clone(), v.clone(), p0=L - 40, rope_mode=0, workspace=ws, **heads)[0],
+        lambda ws: A.prefill_rope(qkv[:9], k[:9].clone(), v[:9].clone(), rope_mode=0, workspace=ws, **heads)[0],
+    ]
+    want = [f(A.new_workspace(128 << 20, device)) for f in calls]
+    ws = A.new_workspace(128 << 20, device)
+    for _ in range(2):
+        for i, f in enumerate(calls):
+            assert torch.equal(f(ws), want[i]), i
+            assert not ws[:COUNTERS].any(), i

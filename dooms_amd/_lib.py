@@ -102,12 +102,15 @@ _lib = None
 
 
 def lib() -> ctypes.CDLL:
-    """The loaded library (raises FileNotFoundError if it was never built)."""
+    """The loaded library (raises FileNotFoundError if it was never built, ImportError if it lacks an entry point)."""
     global _lib
     if _lib is None:
         if not os.path.exists(LIB_PATH):
             raise FileNotFoundError(f"{LIB_PATH} is missing: build it with `python -m dooms_amd.build`")
         L = ctypes.CDLL(LIB_PATH)
+        missing = [f for f in EXPORTS if not hasattr(L, f)]
+        if missing:
+            raise ImportError(f"{LIB_PATH} was built from other sources (it has no {missing[0]}): build it with `python -m dooms_amd.build`")
         P = ctypes.c_void_p
         L.mx_attn_abi_version.restype = ctypes.c_int32
         L.mx_attn_abi_version.argtypes = []

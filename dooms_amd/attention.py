@@ -65,6 +65,8 @@ def _native():
         except ImportError as e:
             raise ImportError(f"{e}: build the extension for this torch with `python -m dooms_amd.build`") from e
         else:
+            if not hasattr(ext, "bind_paged"):
+                raise ImportError("dooms_amd._native was built from other sources: build it with `python -m dooms_amd.build`")
             ext.bind(L.mx_attn_abi_version(),
                      tuple(ctypes.sizeof(t) for t in (_lib.MxAttnDesc, _lib.MxAttnRope, _lib.MxLinearDesc, _lib.MxSelfAttnDesc)),
                      *[ctypes.cast(getattr(L, f), ctypes.c_void_p).value for f in (

@@ -260,14 +260,11 @@ mx::PagedPrefillPlan prefill_plan(const mx_paged_desc & d) {
     return r;
 }
 
-// The counters, and two partials of a tile for each of the workgroups that run at once, whichever plan runs.
+// The counters, and two partials of a tile for each of the workgroups that run at once: as many floats with 8 waves as with 4,
+// of which twice as many workgroups run, so that one workspace serves every plan of a head dim.
 size_t prefill_bytes(int head_dim) {
-    size_t floats = 0;
-    for (const int waves : {4, 8}) {
-        const mx::PagedPrefillPlan r{waves, 1};
-        if (waves == 4 || head_dim != 256) floats = std::max(floats, (size_t)(r.resident(head_dim) * r.part_floats(head_dim)));
-    }
-    return mx::kPagedCounterBytes + floats * sizeof(float);
+    const mx::PagedPrefillPlan r{4, 1};
+    return mx::kPagedCounterBytes + (size_t)(r.resident(head_dim) * r.part_floats(head_dim)) * sizeof(float);
 }
 
 }  // namespace

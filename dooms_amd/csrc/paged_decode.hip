@@ -773,7 +773,7 @@ void launch_rt(const PagedAttnParams & p, int rt, hipStream_t stream) {
     if (rt == 4) hipLaunchKernelGGL((paged_decode_kernel<HD, 4, T, NW, RANGES>), grid, block, 0, stream, p);
     else if (rt == 8) hipLaunchKernelGGL((paged_decode_kernel<HD, 8, T, NW, RANGES>), grid, block, 0, stream, p);
     else if (rt == 16) hipLaunchKernelGGL((paged_decode_kernel<HD, 16, T, NW, RANGES>), grid, block, 0, stream, p);
-    else if constexpr (NW <= 8 && HD != 256) hipLaunchKernelGGL((paged_decode_kernel<HD, 32, T, NW, RANGES>), grid, block, 0, stream, p);
+    else if constexpr (HD != 256) hipLaunchKernelGGL((paged_decode_kernel<HD, 32, T, NW, RANGES>), grid, block, 0, stream, p);
 }
 
 template <class T>

@@ -776,18 +776,18 @@ void launch_shape(const PagedAttnParams & p, hipStream_t stream) {
     hipLaunchKernelGGL((paged_prefill_kernel<HD, T, W, HPW>), dim3((uint32_t)p.ranges), dim3(W * kWave), 0, stream, p);
 }
 
+// The shapes that the plans take: 8 waves at head dim 128 only, several heads with 8 waves only.
 template <int HD, class T>
 void launch_plan(const PagedAttnParams & p, const PagedPrefillPlan & plan, hipStream_t stream) {
-    if constexpr (HD == 256) {
-        launch_shape<HD, T, 4, 1>(p, stream);
-    } else if (plan.waves == 8) {
-        if (plan.heads == 4) launch_shape<HD, T, 8, 4>(p, stream);
-        else if (plan.heads == 2) launch_shape<HD, T, 8, 2>(p, stream);
-        else launch_shape<HD, T, 8, 1>(p, stream);
-    } else {
-        if (plan.heads == 2) launch_shape<HD, T, 4, 2>(p, stream);
-        else launch_shape<HD, T, 4, 1>(p, stream);
+    if constexpr (HD == 128) {
+        if (plan.waves == 8) {
+            if (plan.heads == 4) launch_shape<HD, T, 8, 4>(p, stream);
+            else if (plan.heads == 2) launch_shape<HD, T, 8, 2>(p, stream);
+            else launch_shape<HD, T, 8, 1>(p, stream);
+            return;
+        }
     }
+    launch_shape<HD, T, 4, 1>(p, stream);
 }
 
 template <class T>

@@ -237,8 +237,8 @@ void decode_order(const int32_t * kv_len, int n_seq, bool xcd, int * order) {
 // every call leaves the ones it used at zero; the partials are left as they are. So the counter region has the same
 // place and size in every call, whatever its shape: a call of another shape on the same workspace must never write
 // partials where a counter lies. Launches of more sequences than fit run one after another and reuse both.
-constexpr int64_t kMaxTilesPerLaunch = 2048;
-constexpr size_t kCounterRegion = (size_t)kMaxTilesPerLaunch * mx::kCounterStride * 4;  // 512 KiB
+constexpr int64_t kMaxTilesPerLaunch = mx::kCounterLines;
+constexpr size_t kCounterRegion = mx::kCounterBytes;
 
 // Head dims below this run on the per-query kernel (small.hip), at and above it on the matrix-core kernels.
 constexpr int kMfmaMinHeadDim = 64;

@@ -53,18 +53,6 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 constexpr int kMergeChunk = 16;  // splits whose partials one thread has in flight at once during the merge
 constexpr int kMaxSplitsPerTile = 64;  // the host's split plan never makes more
 
-// Relaxed device-scope atomic accesses of float pairs: coherent across the XCDs without cache maintenance.
-__device__ __forceinline__ void publish2(float * p, float a, float b) {
-    const uint64_t v = (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
-    __hip_atomic_store(reinterpret_cast<uint64_t *>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ void collect2(const float * p, float & a, float & b) {
-    const uint64_t v = __hip_atomic_load(reinterpret_cast<uint64_t *>(const_cast<float *>(p)), __ATOMIC_RELAXED,
-                                         __HIP_MEMORY_SCOPE_AGENT);
-    a = __uint_as_float((uint32_t)v);
-    b = __uint_as_float((uint32_t)(v >> 32));
-}
-
 // XCD-local publishing (the XCD-mapped grid, where every split of a tile runs on one XCD): plain stores, complete once
 // they reach that XCD's L2, where the merging workgroup's device-scope loads find them (a store-load round trip on one
 // XCD: 0.96 us, against 1.50 us with device-scope stores). Batch 1 at 8192 keys 11.07-11.35 -> 10.70-10.89 us per

@@ -122,6 +122,25 @@ __device__ __forceinline__ half8_t as_half8(u32x4 v) { return __builtin_bit_cast
 // also counts against the LDS/scalar wait counter and so turns the waits for LDS into waits for memory.
 __device__ __forceinline__ u32x4 load16(const void * p) { return *(const __attribute__((address_space(1))) u32x4 *)(p); }
 
+// Relaxed device-scope accesses of partials, a float or a pair: coherent across the XCDs without cache maintenance.
+__device__ __forceinline__ void put_f32(float * a, float v) {
+    __hip_atomic_store(reinterpret_cast<uint32_t *>(a), __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float get_f32(const float * a) {
+    return __uint_as_float(__hip_atomic_load(reinterpret_cast<uint32_t *>(const_cast<float *>(a)), __ATOMIC_RELAXED,
+                                             __HIP_MEMORY_SCOPE_AGENT));
+}
+__device__ __forceinline__ void publish2(float * p, float a, float b) {
+    const uint64_t v = (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
+    __hip_atomic_store(reinterpret_cast<uint64_t *>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void collect2(const float * p, float & a, float & b) {
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<uint64_t *>(const_cast<float *>(p)), __ATOMIC_RELAXED,
+                                         __HIP_MEMORY_SCOPE_AGENT);
+    a = __uint_as_float((uint32_t)v);
+    b = __uint_as_float((uint32_t)(v >> 32));
+}
+
 // 16-byte device-scope (sc1) buffer loads: coherent across the XCDs, a quarter of the instructions of 4-byte atomic
 // loads. The resource is built from a wave-uniform base (a per-lane base would make the compiler loop over the distinct
 // descriptors of the wave); lanes differ in their byte offsets.

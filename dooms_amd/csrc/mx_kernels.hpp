@@ -19,6 +19,10 @@ constexpr int kDecodeChunkQuantum = 128;
 // Split counters kCounterStride uint32 (256 bytes) apart: each on a line of its own, so that the atomics of different
 // tiles do not serialize on one line.
 constexpr int kCounterStride = 64;
+// A workspace starts with so many of them (512 KiB), in every call that shares it; the partials lie behind. The torch front
+// end zeroes as many bytes.
+constexpr int kCounterLines = 2048;
+constexpr size_t kCounterBytes = (size_t)kCounterLines * kCounterStride * 4;
 
 struct DecodeSeq {
     const half_t * k;

@@ -157,7 +157,6 @@ int32_t attn_params(const mx_paged_desc & d, const void * q, const void * k, con
 
 // ---- decode ----
 
-constexpr int kDecodeParts = 64;  // parts of a sequence at most: the join takes one lane each (131072 keys, Qwen2.5-7B heads, 54 us; with 33 67)
 constexpr int kCUs = 256;
 
 struct DecodePlan {
@@ -182,7 +181,7 @@ int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
     plan.n_rowtiles = (plan.rows + plan.rt - 1) / plan.rt;
     const int64_t per_seq = (int64_t)d.n_head_kv * plan.n_rowtiles, bound = kv_bound(d);
     auto quanta = [&](int waves) { return (bound + mx::kPagedDecodeBlock * waves - 1) / (mx::kPagedDecodeBlock * waves); };
-    if (per_seq > mx::kPagedMaxSplitTiles)
+    if (per_seq > mx::kCounterLines)
         return fail(MX_ATTN_UNSUPPORTED, "%lld (kv head, row tile) pairs of a sequence are more than one launch holds", (long long)per_seq);
     const int64_t pairs = d.n_seq * per_seq;
     // the kernel counts the quanta of all sequences in 32 bits
@@ -224,7 +223,7 @@ int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
         return fail(MX_ATTN_UNSUPPORTED, "%d sequences of %lld (kv head, row tile) pairs are more than one launch holds", d.n_seq, (long long)per_seq);
     // Two partials a range and tile, or two chunks beyond one a sequence; sized for the most of any batch and length, so that one
     // workspace serves all calls of a head shape and row count.
-    plan.bytes = plan.whole ? 0 : mx::kPagedCounterBytes + (size_t)(2 * std::max<int64_t>(1, 2 * kCUs / per_seq) * per_seq * plan.rt * (d.head_dim + 4)) * sizeof(float);
+    plan.bytes = plan.whole ? 0 : mx::kCounterBytes + (size_t)(2 * std::max<int64_t>(1, 2 * kCUs / per_seq) * per_seq * plan.rt * (d.head_dim + 4)) * sizeof(float);
     return MX_ATTN_OK;
 }
 
@@ -264,7 +263,7 @@ mx::PagedPrefillPlan prefill_plan(const mx_paged_desc & d) {
 // of which twice as many workgroups run, so that one workspace serves every plan of a head dim.
 size_t prefill_bytes(int head_dim) {
     const mx::PagedPrefillPlan r{4, 1};
-    return mx::kPagedCounterBytes + (size_t)(r.resident(head_dim) * r.part_floats(head_dim)) * sizeof(float);
+    return mx::kCounterBytes + (size_t)(r.resident(head_dim) * r.part_floats(head_dim)) * sizeof(float);
 }
 
 }  // namespace
@@ -364,12 +363,11 @@ MX_ATTN_API int32_t mx_paged_decode(const mx_paged_desc * desc, const void * q, 
     p.by_ranges = plan.by_ranges;
     p.whole_keys = plan.whole_keys;
     p.ranges = plan.ranges;
-    p.max_parts = kDecodeParts;
     p.fixed = plan.fixed;
     p.whole = plan.whole;
     p.max_pages = d.max_pages;
     p.counters = static_cast<uint32_t *>(workspace);
-    p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + mx::kPagedCounterBytes);
+    p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + mx::kCounterBytes);
     const hipError_t e = mx::launch_paged_decode(p, d.head_dim, d.dtype, plan.rt, plan.waves, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return fail(MX_ATTN_INTERNAL, "paged decode launch: %s", hipGetErrorString(e));
     return MX_ATTN_OK;
@@ -402,7 +400,7 @@ MX_ATTN_API int32_t mx_paged_prefill(const mx_paged_desc * desc, const void * q,
     if (workspace && ws_bytes < prefill_bytes(d.head_dim))
         return fail(MX_ATTN_RESOURCE_EXHAUSTED, "workspace of %zu bytes is smaller than the %zu bytes needed", ws_bytes, prefill_bytes(d.head_dim));
     p.counters = static_cast<uint32_t *>(workspace);
-    p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + mx::kPagedCounterBytes);
+    p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + mx::kCounterBytes);
     const hipError_t e = mx::launch_paged_prefill(p, d.head_dim, d.dtype, plan, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return fail(MX_ATTN_INTERNAL, "paged prefill launch: %s", hipGetErrorString(e));
     return MX_ATTN_OK;

@@ -26,14 +26,9 @@ namespace mx {
 namespace {
 
 constexpr int kBlock = kPagedDecodeBlock;
-constexpr int kMaxParts = 64;   // parts of a sequence at most (p.max_parts): one lane each in the merge
 
 typedef short short4_t __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ void publish2(float * p, float a, float b) {
-    const uint64_t v = (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
-    __hip_atomic_store(reinterpret_cast<uint64_t *>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
 __device__ __forceinline__ u32x2 load8_dev(__amdgpu_buffer_rsrc_t r, int byte_off) {
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, byte_off, 0, kCpolSc1));
 }
@@ -82,7 +77,7 @@ __device__ __forceinline__ Chunk find_chunk(const PagedAttnParams & p, int j, in
     int c = most;
     if (longest > p.whole_keys) {
         const int share = __builtin_amdgcn_readfirstlane((int)fminf(ceilf(sum / (float)p.ranges), (float)most));
-        c = max((most + p.max_parts - 1) / p.max_parts, share);
+        c = max((most + kPagedMaxParts - 1) / kPagedMaxParts, share);
         for (int i = 0; c < most && count(c) > p.ranges; i++) c = i < 16 ? min(c + max(1, c / 8), most) : most;
     }
     Chunk x{-1, 0, 0, 1, c * QK, 0, 0};
@@ -145,7 +140,7 @@ __device__ __forceinline__ Range find_range(const PagedAttnParams & p, int r, in
     most = wave_imax(most);
     // an equal share each, and no more parts of a sequence than the merge takes (a part may start within a range: one more)
     Range x;
-    x.share = max((sum + p.ranges - 1) / p.ranges, (most + p.max_parts - 2) / (p.max_parts - 1));
+    x.share = max((sum + p.ranges - 1) / p.ranges, (most + kPagedMaxParts - 2) / (kPagedMaxParts - 1));
     const int64_t lo = (int64_t)r * x.share;
     x.lo = (int)min(lo, (int64_t)sum);
     x.hi = (int)min(lo + x.share, (int64_t)sum);
@@ -687,10 +682,10 @@ void paged_decode_kernel(PagedAttnParams p) {
                 // with 12). Past the last part the lanes load it again, or at head dim 64, whose launches have fewer parts, nothing
                 // (7 parts 8.0 -> 7.55 us, but 32 parts at head dim 128 11.55 -> 11.75).
                 constexpr int MC = CPT > 2 ? 4 : CPT == 2 ? 12 : 8;
-                static_assert(kMaxParts <= kWave, "one lane per part");
-                static_assert((kMaxParts * RT + 2 * RT) * 4 + (SF - 1) * NQ * 16 <= (int64_t)sizeof(s_buf), "merge scratch");
+                static_assert(kPagedMaxParts <= kWave, "one lane per part");
+                static_assert((kPagedMaxParts * RT + 2 * RT) * 4 + (SF - 1) * NQ * 16 <= (int64_t)sizeof(s_buf), "merge scratch");
                 float * s_w = reinterpret_cast<float *>(s_buf);                     // [part][row]
-                float2 * s_row = reinterpret_cast<float2 *>(s_w + kMaxParts * RT);  // (M, total)
+                float2 * s_row = reinterpret_cast<float2 *>(s_w + kPagedMaxParts * RT);  // (M, total)
                 float4_t * s_acc = reinterpret_cast<float4_t *>(s_row + RT);        // [stripe - 1][quad]
                 const int stripe = SF > 1 ? (int)threadIdx.x / NQ : 0;
                 auto quad = [&](int c) { return SF > 1 ? (int)threadIdx.x % NQ : (int)threadIdx.x + c * kThreads; };
@@ -722,7 +717,7 @@ void paged_decode_kernel(PagedAttnParams p) {
                     const float M = row16_max(xor16_max(xor32_max(m)));
                     const float w = exp2_fast(m - (M == kNegInf ? 0.f : M));
                     const float tot = row16_sum(xor16_add(xor32_add(lane < ns ? __uint_as_float(ml[r][1]) * w : 0.f)));
-                    if (lane < kMaxParts) s_w[lane * RT + i] = w;
+                    if (lane < kPagedMaxParts) s_w[lane * RT + i] = w;
                     if (lane == 0) s_row[i] = make_float2(M, tot);
                 }
                 lds_barrier();  // the weights

@@ -47,15 +47,6 @@ struct Smem {
     int32_t ids[W][kWave];  // page numbers of a wave's next step: its four 16-row blocks in lanes 0 .. 3 (and again above)
 };
 
-// Relaxed device-scope accesses of the partials: coherent across the XCDs without cache maintenance.
-__device__ __forceinline__ void put_f32(float * a, float v) {
-    __hip_atomic_store(reinterpret_cast<uint32_t *>(a), __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float get_f32(const float * a) {
-    return __uint_as_float(__hip_atomic_load(reinterpret_cast<uint32_t *>(const_cast<float *>(a)), __ATOMIC_RELAXED,
-                                             __HIP_MEMORY_SCOPE_AGENT));
-}
-
 // Inclusive prefix sums of values below 2^49 over a wave.
 __device__ __forceinline__ int64_t wave_scan64(int64_t v) {
     return ((int64_t)wave_iscan((int32_t)(v >> 24)) << 24) + wave_iscan((int32_t)(v & 0xffffff));

@@ -44,15 +44,6 @@ constexpr half2_t kOnes2 = {(half_t)1.f, (half_t)1.f};
 // exact update runs: below it every probability is below 2^8.
 constexpr float kProbSumMax = 256.f;
 
-// Relaxed device-scope accesses of the stream-K partials: coherent across the XCDs without cache maintenance.
-__device__ __forceinline__ void put_f32(float * a, float v) {
-    __hip_atomic_store(reinterpret_cast<uint32_t *>(a), __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float get_f32(const float * a) {
-    return __uint_as_float(__hip_atomic_load(reinterpret_cast<uint32_t *>(const_cast<float *>(a)), __ATOMIC_RELAXED,
-                                             __HIP_MEMORY_SCOPE_AGENT));
-}
-
 // LDS tiles are row-major with padded rows: K rows HD + 8 halves apart (the 16-byte reads of 16 consecutive rows at one
 // column land on 16 distinct 4-bank groups), V rows HD + 32 halves apart (a row step of 16 banks mod 64: the 4 rows x
 // 32 bytes that each 16-lane group reads through the transposing read, for both groups of a 32-lane phase, land on 64

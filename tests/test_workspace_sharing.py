@@ -71,3 +71,13 @@ def test_every_call_that_keeps_counters(device):
         for i, f in enumerate(calls):
             assert torch.equal(f(ws), want[i]), i
             assert not ws[:COUNTERS].any(), i
+
+
+def test_one_counter_region():
+    """Every call's partials lie behind the same counters, which the front end zeroes."""
+    paged = A.paged_decode_workspace_bytes(n_head=1, n_head_kv=1, head_dim=64, n_q=1, n_seq=1, max_kv_len=1 << 20)
+    assert paged - 2 * 512 * 4 * (64 + 4) * 4 == COUNTERS  # two partials of 4 rows for each of 512 workgroups
+    prompts = A.paged_prefill_workspace_bytes(n_head=1, n_head_kv=1, head_dim=64, n_rows=1, n_seq=1, max_q=1, max_kv_len=1)
+    assert prompts - 2 * 512 * 4 * 64 * (32 + 2) * 4 == COUNTERS  # of 4 waves, 32 outputs, m and l a lane
+    assert A.decode_workspace_bytes(n_head=1, n_head_kv=1, head_dim=64, n_q=1, batch=1, max_kv_len=256) - 2 * 4 * (64 + 4) * 4 == COUNTERS
+    assert A._PAGED_COUNTERS == COUNTERS

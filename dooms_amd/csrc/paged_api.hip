@@ -164,10 +164,12 @@ struct DecodePlan {
     size_t bytes;  // workspace
 };
 
-// Keys per sequence that the plan reckons with.
+// Keys per sequence that the plan reckons with: the hint's, or the table's, or what a launch holds where a workspace is
+// sized without either.
 int64_t kv_bound(const mx_paged_desc & d) {
-    const int64_t table = (int64_t)d.max_pages * d.page_size;
-    return std::max<int64_t>(1, d.max_kv_len > 0 && (table <= 0 || d.max_kv_len < table) ? d.max_kv_len : table);
+    int64_t table = (int64_t)d.max_pages * d.page_size;
+    if (table <= 0) table = std::min<int64_t>((int64_t)1 << 30, ((int64_t)1 << 36) / std::max(1, d.n_seq));
+    return d.max_kv_len > 0 && d.max_kv_len < table ? d.max_kv_len : table;
 }
 
 int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {

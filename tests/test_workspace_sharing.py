@@ -81,3 +81,10 @@ def test_one_counter_region():
     assert prompts - 2 * 512 * 4 * 64 * (32 + 2) * 4 == COUNTERS  # of 4 waves, 32 outputs, m and l a lane
     assert A.decode_workspace_bytes(n_head=1, n_head_kv=1, head_dim=64, n_q=1, batch=1, max_kv_len=256) - 2 * 4 * (64 + 4) * 4 == COUNTERS
     assert A._PAGED_COUNTERS == COUNTERS
+
+
+def test_workspace_without_a_length():
+    """No length and no table: room for any length, as the call that follows may be split."""
+    for n_seq in (1, 3, 200, 65535):
+        shape = dict(n_head=8, n_head_kv=2, head_dim=128, n_q=1, n_seq=n_seq)
+        assert A.paged_decode_workspace_bytes(max_kv_len=0, **shape) == A.paged_decode_workspace_bytes(max_kv_len=100000, **shape) > 0

@@ -356,7 +356,8 @@ def _paged_desc(rows, k_pages, v_pages, page_table, kv_len, cu_q, n_head, max_q=
     if k_pages.dim() != 4 or k_pages.stride(3) != 1 or k_pages.dtype not in _PAGE_DTYPES:
         raise ValueError("k_pages must be a float16 or bfloat16 [pages][page size][kv heads][head dim] tensor with unit stride along "
                          "the head dim")
-    if v_pages.shape != k_pages.shape or v_pages.stride() != k_pages.stride() or v_pages.dtype != k_pages.dtype:
+    if v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype or any(
+            n > 1 and a != b for n, a, b in zip(k_pages.shape, k_pages.stride(), v_pages.stride())):  # a lone page or head has no stride
         raise ValueError("v_pages must have the shape, strides and type of k_pages")
     if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
         raise ValueError("page_table must be an int32 [sequences][pages] tensor with unit stride along the pages")

@@ -398,7 +398,8 @@ struct Paged {
         type = k.scalar_type();
         need(rows.is_cuda() && k.device() == rows.device() && v.device() == rows.device() && table.device() == rows.device());
         need(k.dim() == 4 && k.stride(3) == 1 && (type == at::kHalf || type == at::kBFloat16));
-        need(v.scalar_type() == type && v.sizes() == k.sizes() && v.strides() == k.strides());
+        need(v.scalar_type() == type && v.sizes() == k.sizes());
+        for (int i = 0; i < 4; i++) need(k.size(i) <= 1 || v.stride(i) == k.stride(i));
         need(table.scalar_type() == at::kInt && (table.stride(1) == 1 || table.size(1) <= 1));
         need(table.size(0) <= 1 || table.stride(0) >= table.size(1));
         for (int64_t n : {k.size(0), k.size(1), k.size(2), k.size(3), table.size(0), table.size(1), rows.size(0)}) need(n <= INT32_MAX);

@@ -71,7 +71,7 @@ int32_t check_cache(const mx_paged_desc & d) {
         const char * name;
     } dim[3] = {{d.page_stride, d.n_pages, "page_stride"}, {d.kv_stride, d.page_size, "kv_stride"}, {d.head_stride, d.n_head_kv, "head_stride"}};
     for (const Dim & x : dim)
-        if (x.stride < 0 || x.stride % 8 || x.stride > (int64_t)1 << 46)
+        if (x.n > 1 && (x.stride < 0 || x.stride % 8 || x.stride > (int64_t)1 << 46))
             return fail(MX_ATTN_INVALID_ARGUMENT, "%s (%lld) must be a multiple of 8 elements, >= 0", x.name, (long long)x.stride);
     std::sort(dim, dim + 3, [](const Dim & a, const Dim & b) { return a.stride < b.stride; });
     int64_t span = d.head_dim;

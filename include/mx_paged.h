@@ -49,7 +49,7 @@ typedef struct mx_paged_desc {
     int32_t max_q;        /* mx_paged_prefill: the most rows of a sequence, 0: unknown. A hint for the plan, as is ... */
     int32_t max_kv_len;   /* ... the most keys of a sequence, 0: unknown (max_pages * page_size) */
     int32_t reserved;     /* must be 0 */
-    int64_t page_stride;  /* elements between pages, rows of a page and heads of a row: multiples of 8 */
+    int64_t page_stride;  /* elements between pages, rows of a page and heads of a row: multiples of 8 (any with one page or head) */
     int64_t kv_stride;
     int64_t head_stride;
     int64_t table_stride; /* entries between sequences of the page table (>= max_pages) */

@@ -67,3 +67,30 @@ def test_prefill_tiles_of_one_step_before_longer_ones(device, hd, n_head, n_kv, 
     lens = [(60, 33, 200, 64, 500, 1)[b % 6] for b in range(330)]
     prefill_case(device, 122, n_head, n_kv, hd, [min(L, 1 + b % 3) for b, L in enumerate(lens)], lens, 16, dtype,
                  mutate=wide() if long else None)
+
+
+# ---- layouts ----
+
+def test_one_page_and_one_head_have_no_stride(device):
+    """A pool with one kv head or one page, whose strides along them may be anything, each pool's its own."""
+    g = gen(123)
+    c = Cache(g, [30, 12], 1, 64, 16, F16)
+    k, v, table, kv_len = c.to(device)
+    last = k.squeeze(2).contiguous().unsqueeze(3).transpose(2, 3)  # stride 1 along the heads
+    assert last.stride(2) == 1 and v.stride(2) == 64
+    q = torch.randn(2, 4 * 64, generator=g).to(F16)
+    ref, _, tol, _ = attend(c, q, [1, 1], 4, 0.125, True, True, F16)
+    ws = A.new_workspace(64 << 20, device)
+    for w in (None, ws):
+        close(A.paged_decode(q.to(device), last, v, table, kv_len, n_head=4, workspace=w)[0], ref, tol, "decode")
+        close(A.paged_prefill(q.to(device), last, v, table, kv_len, cu_of([1, 1], device), n_head=4, workspace=w)[0], ref, tol, "prefill")
+    x = torch.randn(2, 6 * 64, generator=g).to(device)
+    for pools in ((k.clone(), v.clone()), (last.clone(memory_format=torch.preserve_format), v.clone())):
+        A.paged_store(x, *pools, table, kv_len, n_head=4, rope_mode=2)
+        assert torch.equal(pools[0][table[1, 0].long(), 11, 0], x[1, 256:320].to(F16))
+    one = Cache(g, [9], 2, 128, 16, BF16, spare=0)
+    k, v, table, kv_len = one.to(device)
+    k = torch.as_strided(k, k.shape, (3, *k.stride()[1:]))
+    q = torch.randn(1, 4 * 128, generator=g).to(BF16)
+    ref, _, tol, _ = attend(one, q, [1], 4, 128 ** -0.5, True, False, BF16)
+    close(A.paged_decode(q.to(device), k, v, table, kv_len, n_head=4)[0], ref, tol, "one page")

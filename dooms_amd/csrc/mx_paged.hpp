@@ -126,7 +126,7 @@ struct PagedAttnParams {
     int32_t by_ranges;     // decode: 1: workgroups walk ranges of the launch's keys, 0: a chunk of a sequence each
     int32_t ranges;        // decode: ranges, or chunks, that the launch has workgroups for, for each (kv head, row tile); prefill:
                            // workgroups, a multiple of 8
-    int32_t whole_keys;    // decode, chunks: sequences of up to so many keys are not split
+    int32_t whole_keys;    // decode, chunks: nothing is split where no sequence of the launch is longer (fixed: no such sequence is)
     int32_t fixed;         // decode, chunks: of every sequence, each a quantum (the last takes what is left); 0: the chunks follow
                            // from the lengths
     int32_t whole;         // 1: no sequence (prefill: no tile) is split, there is no workspace

@@ -538,9 +538,11 @@ void paged_prefill_kernel(PagedAttnParams p) {
                         sc[mt][v] = key > lim ? kNegInf : sc[mt][v];
                     }
             }
-            // Probabilities at the kept maximum, rounded to T (the P^T operand: step u takes values 8 (u % 2) .. + 8 of score tile
-            // u / 2), and the sum of the rounded ones, so that the weights of a row add up to 1. A lane's sum above 2^8 (or a row
-            // without a maximum yet) moves the maximum, rescales l and O, and computes the block again.
+            // Probabilities at the kept maximum, rounded to T as the product takes both operands in one type (the P^T operand: step u
+            // takes values 8 (u % 2) .. + 8 of score tile u / 2), and the sum of the rounded ones, so that the weights of a row add
+            // up to 1 (the outputs' error against 64 bits is 0.00196 in bf16 and 0.00028 in f16, where 32-bit probabilities and the
+            // output's rounding alone make 0.00164 and 0.00021). A lane's sum above 2^8 (or a row without a maximum yet) moves the
+            // maximum, rescales l and O, and computes the block again.
             u32x4 pb[4];
             auto settle = [&](auto H0C, auto H1C) __attribute__((always_inline)) {
                 constexpr int H0 = decltype(H0C)::value, H1 = decltype(H1C)::value;

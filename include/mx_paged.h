@@ -13,12 +13,16 @@
  * values alike. Any order of heads and rows within a page is a choice of the two strides. Sequences may share pages. Rows
  * that hold no key (behind a sequence's end, or in pages of no sequence) are never used, whatever they hold.
  *
+ * Arithmetic of the attention calls. Scores, running maxima and sums, accumulators and joins are f32. The probabilities are
+ * rounded to the pages' type for their product with the values, as the matrix cores take both operands in one type: half a step
+ * of that type on each key's weight, with row_dtype MX_ATTN_F32 too, whose rows are only stored wider. The output is rounded once.
+ *
  * Device metadata cannot be checked by the host, and no entry of it makes a call read or write outside the pool:
  *   - kv_len outside [0, max_pages * page_size] makes that sequence's outputs NaN, a page outside [0, n_pages) the rows that
  *     attend it (and rows of that sequence that are computed with them); mx_paged_store leaves out the keys and values of a row
  *     that such a page or length would take;
  *   - query rows that see no key (kv_len 0, or rows of a causal call at positions below 0) give zeros and an lse of -inf;
- *   - cu_q entries are clamped to [0, n_rows]; what overlapping ranges compute is undefined.
+ *   - cu_q entries are clamped to [0, n_rows] and have to ascend; what ranges that run backwards or overlap compute is undefined.
  *
  * Errors, streams and threading as mx_attn.h (the same codes and mx_attn_last_error()).
  */

@@ -204,9 +204,9 @@ int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
     } else {
         // Where no sequence is longer than whole_keys each is one chunk: joining costs 1 to 2 us more than the walk saves (513 keys,
         // Qwen2.5-0.5B heads, 6.3 us against 7.4 split; 512 keys, Llama-3-8B heads, 8.2 against 8.6; 1000 keys 13.1 whole against
-        // 8.5). Beyond it 4 waves a workgroup, two on a CU, find the keys of a middling length on more CUs (1000 keys, Llama-3-8B heads, 7.35
-        // against 8.5 with 8 waves; 2000, Qwen2.5-0.5B heads, 7.2 against 7.6), and split shorter sequences too (8 of 100-1000 keys
-        // 9.5 against 10.4 with 512). Longer ones have fewer parts to join with 8 (4000 keys, Qwen2.5-7B heads, 9.8 against 10.6;
+        // 8.5). Beyond it 4 waves a workgroup, two on a CU, find the keys of a middling length on more CUs (1000 keys, Llama-3-8B
+        // heads, 7.35 against 8.5 with 8 waves; 2000, Qwen2.5-0.5B heads, 7.2 against 7.6), and split shorter sequences too (8 of
+        // 100-1000 keys 9.5 against 10.4 with 512). Longer ones have fewer parts to join with 8 (4000 keys, Qwen2.5-7B heads, 9.8 against 10.6;
         // 8192, Llama-3-8B heads, 11.3 against 14.8), and so have tiles of more rows. At head dim 256 the LDS holds 4 waves.
         plan.whole_keys = d.head_dim == 64 ? 640 : 512;
         plan.waves = d.head_dim == 256 || bound <= 128 || (plan.rt <= 8 && bound > plan.whole_keys && bound <= 2048) ? 4 : 8;
@@ -407,5 +407,27 @@ MX_ATTN_API int32_t mx_paged_prefill(const mx_paged_desc * desc, const void * q,
     if (e != hipSuccess) return fail(MX_ATTN_INTERNAL, "paged prefill launch: %s", hipGetErrorString(e));
     return MX_ATTN_OK;
 }
+
+#ifdef MX_ATTN_TRACE
+// The diagnostic variant of the library tells how a call would run, so that tests know which kernels they reach. plan[0 .. 2]: rows
+// of a tile, waves, and for a decode how it is cut (0 chunks from the lengths, 1 a fixed count of each sequence, 2 ranges), for
+// prompts heads of a tile.
+__attribute__((visibility("default"))) int32_t mx_paged_trace_plan(const mx_paged_desc * d, int32_t prefill, int32_t * plan) {
+    if (int32_t rc = check_shape(d)) return rc;
+    if (prefill) {
+        const mx::PagedPrefillPlan r = prefill_plan(*d);
+        plan[0] = r.rows();
+        plan[1] = r.waves;
+        plan[2] = r.heads;
+        return MX_ATTN_OK;
+    }
+    DecodePlan r;
+    if (int32_t rc = decode_plan(*d, r)) return rc;
+    plan[0] = r.rt;
+    plan[1] = r.waves;
+    plan[2] = r.by_ranges ? 2 : r.fixed ? 1 : 0;
+    return MX_ATTN_OK;
+}
+#endif
 
 }  // extern "C"

@@ -392,18 +392,19 @@ void paged_prefill_kernel(PagedAttnParams p) {
 
     // The values that this wave loaded behind a sequence's last key (the loads repeat it) become zeros: its rows multiply them by
     // probabilities of 0, which an infinity among them would turn into NaN. By asm, as the operands' reads are, so that no load in
-    // flight is waited for.
-    const uint32_t v_mine = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint16_t *)sm.v[0] + 1024 * wave + 16 * lane;
+    // flight is waited for; from the thread's number alone, so that the steps before the last hold no registers for it.
     auto zero_behind = [&](int kb, int L) __attribute__((always_inline)) {
-        if (kb + my_rows + lrow >= L) {
-            const uint32_t at = v_mine + take * (uint32_t)sizeof(sm.v[0]);
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));
+        if (kb + my_rows + tid % kWave / 4 >= L) {
+            const uint32_t at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint16_t *)sm.v[take] + 16 * tid;
             static_for<0, NI>([&](auto I) __attribute__((always_inline)) {
                 const uint32_t a = at;
                 const u32x4 zero = {0u, 0u, 0u, 0u};
                 asm volatile("ds_write_b128 %0, %1 offset:%2" ::"v"(a), "v"(zero), "i"(1024 * W * decltype(I)::value) : "memory");
             });
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     };
 
     // ---- the wave's rows of a tile ----
@@ -441,7 +442,6 @@ void paged_prefill_kernel(PagedAttnParams p) {
         // the first tile's steps, and what the tiles behind were too short for (the buffer read last is not among those filled)
         if (sent < NBUF - 1) {
             while (sent < NBUF - 1 && more()) {
-                waited = false;  // page numbers requested here are not covered by the wait at the last tile's end
                 // two steps' page numbers at once
                 const bool two = NBUF > 2 && sent == 0 && fd.step + 1 < fd.end;
                 int i0 = *ids_at(fd.step), i1 = *ids_at(two ? fd.step + 1 : fd.step);
@@ -449,6 +449,7 @@ void paged_prefill_kernel(PagedAttnParams p) {
                 send(i0);
                 if (two) send(i1);
             }
+            if (waited) __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the wait at the last tile's end was before these
             asm volatile("" ::: "memory");
         }
 #pragma unroll

@@ -5,9 +5,10 @@
 // times v, with the running maximum m and sum l of a row in f32: O <- O e^(m - m') + sum_j e^(s_j - m') v_j.
 //
 // What bounds it: 4 n_head head_dim flops per (row, key) pair on the matrix cores; the softmax's exponentials on the vector
-// ALUs fill most of the time between the products (two chunks of 1.5k-2k rows behind 14k keys, Qwen2.5-7B heads, 735 GFLOP in 743 us,
-// 990 TFLOP/s; a large library product of the type reaches 1142). Short prompts add what a tile costs beside its keys, about 3 us
-// of queries, outputs and first loads (12 prompts of 65-1711 rows, Llama-3-8B heads, 104 GFLOP in 156 us).
+// ALUs fill most of the time between the products (two chunks of 1.5k-2k rows behind 14k keys, Qwen2.5-7B heads, 736 GFLOP in 735 to
+// 780 us from card to card, 945 to 1000 TFLOP/s; a large library product of the type reaches 1324, its right operand transposed
+// 1517). Short prompts add what a tile costs beside its keys, about 3 us of queries, outputs and first loads (12 prompts of 65-1711
+// rows, Llama-3-8B heads, 104 GFLOP in 152 to 160 us).
 //
 //   * A tile is W waves of 32 query rows: W / HPW row tiles of each of HPW heads that share a kv head, so that a short or causal
 //     tile wastes few rows and the keys serve all of them. Steps are 64 keys; keys and values go straight into LDS
@@ -392,7 +393,8 @@ void paged_prefill_kernel(PagedAttnParams p) {
 
     // The values that this wave loaded behind a sequence's last key (the loads repeat it) become zeros: its rows multiply them by
     // probabilities of 0, which an infinity among them would turn into NaN. By asm, as the operands' reads are, so that no load in
-    // flight is waited for; from the thread's number alone, so that the steps before the last hold no registers for it.
+    // flight is waited for; from the thread's number alone, so that the steps before the last hold no registers for it
+    // (0.5 % of 17 prompt batches' time; five prompts of 37-420 rows, Qwen2.5-0.5B heads, 11.8 -> 12.0 us).
     auto zero_behind = [&](int kb, int L) __attribute__((always_inline)) {
         int tid = threadIdx.x;
         asm volatile("" : "+v"(tid));

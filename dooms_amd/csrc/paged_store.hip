@@ -8,7 +8,7 @@
 // thread holds two pieces of 16 bytes, half a head apart, so that both rotary layouts find their partners in one thread and
 // every load and store of a wave is contiguous. The sequence is looked up first, then the row's loads go out, behind them
 // the page, and the head_dim / 2 angles, turned into (cos, sin) once for all heads of the row. 179 MB of
-// packed prompts take 31.5 us (5.7 TB/s, a large copy reaches 5.0); a decode step's row 2.8 us, of which an empty launch is 2.
+// packed prompts take 31.6 us (5.7 TB/s, a large copy reaches 5.2); a decode step's row 2.8 us, of which an empty launch is 2.
 #include "mx_paged.hpp"
 
 #include <algorithm>

@@ -16,6 +16,7 @@
  * Arithmetic of the attention calls. Scores, running maxima and sums, accumulators and joins are f32. The probabilities are
  * rounded to the pages' type for their product with the values, as the matrix cores take both operands in one type: half a step
  * of that type on each key's weight, with row_dtype MX_ATTN_F32 too, whose rows are only stored wider. The output is rounded once.
+ * A probability that rounds to 0 (in f16 below 2^-25 of the largest) makes NaN of an infinite value at its key.
  *
  * Device metadata cannot be checked by the host, and no entry of it makes a call read or write outside the pool:
  *   - kv_len outside [0, max_pages * page_size] makes that sequence's outputs NaN, a page outside [0, n_pages) the rows that

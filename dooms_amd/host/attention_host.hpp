@@ -164,27 +164,38 @@ public:
         if (c.head_dim < 4 || c.head_dim > 256 || (c.head_dim & (c.head_dim - 1)) != 0)  // metal_llama_decoder.mm:432-435
             return {Code::Unsupported, "head_dim must be a power of two in [4, 256], got " + std::to_string(c.head_dim)};
         std::unique_ptr<LlamaAttention> a(new LlamaAttention(c, k_cache, v_cache, stream));
-        // one workspace for the decode rows and for the prompt chunks of few rows that mx_attn_prefill_ws runs on the
-        // split-KV kernel (up to 512, or with a long enough cache 1024, rows per kv head), at the full context
-        mx_attn_desc d = a->desc(1, 0, 0);
-        size_t bytes = mx_attn_decode_workspace_bytes(&d, 1, c.n_ctx);
-        for (int32_t rows : {512, 1024}) {
-            const int32_t m_split = std::min<int32_t>(c.n_ctx, std::max(1, rows / (c.n_head / c.n_head_kv)));
-            mx_attn_desc dp = a->desc(m_split, 0, 0);
-            dp.p0 = c.n_ctx - m_split;
-            dp.causal = 1;
-            bytes = std::max(bytes, mx_attn_prefill_workspace_bytes(&dp));
-        }
-        // and the flash kernel's stream-K slots, when its plan splits the largest chunk over the CUs (at the end of the
-        // context, where its tiles are longest; a chunk that finds the workspace short of them runs unsplit)
-        const int32_t n_batch = std::min<int32_t>(c.n_ctx, c.n_batch > 0 ? c.n_batch : 2048);
-        mx_attn_desc db = a->desc(n_batch, 0, 0);
-        db.p0 = c.n_ctx - n_batch;
-        db.causal = 1;
-        bytes = std::max(bytes, mx_attn_prefill_workspace_bytes(&db));
+        const size_t bytes = workspace_bytes(c);
         if (Status st = a->ws_.reserve(bytes, stream); !st.is_ok()) return st;
         out = std::move(a);
         return {};
+    }
+
+    // Bytes of the one workspace for the decode rows and for the prompt chunks that mx_attn_prefill_ws runs on the split-KV kernel
+    // (up to 512, or with a long enough cache 1024, rows per kv head): chunks of so many rows anywhere in the context. A chunk
+    // needs more the more keys it has, but from some length on it runs on the flash kernel instead, which needs less, so each
+    // row count is asked for at the context's end and either side of the powers of two, where the route and the splits change
+    // (some 20 ms at most). A chunk of more rows that finds the workspace short of the flash kernel's stream-K slots runs unsplit.
+    static size_t workspace_bytes(const LlamaAttentionConfig & c) {
+        mx_attn_desc d = desc(c, 1, 0, 0);
+        size_t bytes = mx_attn_decode_workspace_bytes(&d, 1, c.n_ctx);
+        auto chunk = [&](int32_t rows, int64_t keys) {
+            if (keys < rows || keys > c.n_ctx) return;
+            mx_attn_desc p = desc(c, rows, 0, 0);
+            p.p0 = (int32_t)keys - rows;
+            p.causal = 1;
+            bytes = std::max(bytes, mx_attn_prefill_workspace_bytes(&p));
+        };
+        const int32_t most = std::min<int32_t>(c.n_ctx, std::max(1, 1024 / (c.n_head / c.n_head_kv)));
+        for (int32_t rows = 1; rows <= most; rows++) {
+            chunk(rows, c.n_ctx);
+            for (int64_t keys = 128; keys <= c.n_ctx; keys *= 2) {
+                chunk(rows, keys - 1);
+                chunk(rows, keys);
+            }
+        }
+        // the stream-K slots of the largest chunk, at the end of the context, where its tiles are longest
+        chunk(std::min<int32_t>(c.n_ctx, c.n_batch > 0 ? c.n_batch : 2048), c.n_ctx);
+        return bytes;
     }
 
     const LlamaAttentionConfig & config() const { return cfg_; }
@@ -280,17 +291,18 @@ public:
 
 private:
     LlamaAttention(const LlamaAttentionConfig & c, uint16_t * k, uint16_t * v, hipStream_t s) : cfg_(c), k_(k), v_(v), stream_(s) {}
-    mx_attn_desc desc(int32_t n_q, int64_t q_stride, int64_t out_stride) const {
+    mx_attn_desc desc(int32_t n_q, int64_t q_stride, int64_t out_stride) const { return desc(cfg_, n_q, q_stride, out_stride); }
+    static mx_attn_desc desc(const LlamaAttentionConfig & c, int32_t n_q, int64_t q_stride, int64_t out_stride) {
         mx_attn_desc d{};
-        d.n_head = cfg_.n_head;
-        d.n_head_kv = cfg_.n_head_kv;
-        d.head_dim = cfg_.head_dim;
+        d.n_head = c.n_head;
+        d.n_head_kv = c.n_head_kv;
+        d.head_dim = c.head_dim;
         d.n_q = n_q;
-        d.q_stride = q_stride ? q_stride : q_width();
-        d.kv_stride = kv_width();
-        d.out_stride = out_stride ? out_stride : q_width();
-        d.scale = 1.0f / std::sqrt((float)cfg_.head_dim);
-        d.tuning = &cfg_.tuning;
+        d.q_stride = q_stride ? q_stride : c.n_head * c.head_dim;
+        d.kv_stride = c.n_head_kv * c.head_dim;
+        d.out_stride = out_stride ? out_stride : c.n_head * c.head_dim;
+        d.scale = 1.0f / std::sqrt((float)c.head_dim);
+        d.tuning = &c.tuning;
         return d;
     }
     LlamaAttentionConfig cfg_;

@@ -206,8 +206,9 @@ int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
         // Qwen2.5-0.5B heads, 6.3 us against 7.4 split; 512 keys, Llama-3-8B heads, 8.2 against 8.6; 1000 keys 13.1 whole against
         // 8.5). Beyond it 4 waves a workgroup, two on a CU, find the keys of a middling length on more CUs (1000 keys, Llama-3-8B
         // heads, 7.35 against 8.5 with 8 waves; 2000, Qwen2.5-0.5B heads, 7.2 against 7.6), and split shorter sequences too (8 of
-        // 100-1000 keys 9.5 against 10.4 with 512). Longer ones have fewer parts to join with 8 (4000 keys, Qwen2.5-7B heads, 9.8 against 10.6;
-        // 8192, Llama-3-8B heads, 11.3 against 14.8), and so have tiles of more rows. At head dim 256 the LDS holds 4 waves.
+        // 100-1000 keys 9.5 against 10.4 with 512). Longer ones have fewer parts to join with 8 (4000 keys, Qwen2.5-7B heads, 9.8
+        // against 10.6; 8192, Llama-3-8B heads, 11.3 against 14.8), and so have tiles of more rows. At head dim 256 the LDS holds 4
+        // waves.
         plan.whole_keys = d.head_dim == 64 ? 640 : 512;
         plan.waves = d.head_dim == 256 || bound <= 128 || (plan.rt <= 8 && bound > plan.whole_keys && bound <= 2048) ? 4 : 8;
         if (plan.waves == 4) plan.whole_keys = 256;

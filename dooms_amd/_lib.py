@@ -26,7 +26,8 @@ EXPORTS = ("mx_attn_abi_version", "mx_attn_last_error", "mx_attn_prefill", "mx_a
            "mx_linear_call_workspace_bytes",
            "mx_attn_decode_workspace_bytes", "mx_attn_decode_workspace_init", "mx_self_attention",
            "mx_self_attention_workspace_bytes", "mx_paged_store", "mx_paged_decode", "mx_paged_decode_workspace_bytes",
-           "mx_paged_prefill", "mx_paged_prefill_workspace_bytes")
+           "mx_paged_prefill", "mx_paged_prefill_workspace_bytes", "mx_paged_store_e4m3", "mx_paged_decode_e4m3",
+           "mx_paged_prefill_e4m3")
 
 ROPE_NORMAL = 0  # adjacent pairs (2i, 2i + 1): llama
 ROPE_NEOX = 1    # split halves (i, i + head_dim / 2): qwen2
@@ -84,6 +85,12 @@ class MxPagedRope(ctypes.Structure):
     """mx_paged_rope (include/mx_paged.h)."""
     _fields_ = [("mode", ctypes.c_int32), ("n_axes", ctypes.c_int32), ("axis_pairs", ctypes.c_int32 * PAGED_MAX_AXES),
                 ("axis_restart", ctypes.c_int32), ("reserved", ctypes.c_int32), ("base", ctypes.c_double)]
+
+
+class MxPagedScales(ctypes.Structure):
+    """mx_paged_scales (include/mx_paged.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("reserved", ctypes.c_int32)]
 
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
@@ -161,6 +168,12 @@ def lib() -> ctypes.CDLL:
         L.mx_paged_decode.argtypes = [desc, P, P, P, P, P, P, P, P, ctypes.c_size_t, P]
         L.mx_paged_prefill.restype = ctypes.c_int32
         L.mx_paged_prefill.argtypes = [desc, P, P, P, P, P, P, P, P, P, ctypes.c_size_t, P]
+        for f in (L.mx_paged_store_e4m3, L.mx_paged_decode_e4m3, L.mx_paged_prefill_e4m3):
+            f.restype = ctypes.c_int32
+        scales = ctypes.POINTER(MxPagedScales)
+        L.mx_paged_store_e4m3.argtypes = [desc, rope, scales, *L.mx_paged_store.argtypes[2:]]
+        L.mx_paged_decode_e4m3.argtypes = [desc, scales, *L.mx_paged_decode.argtypes[1:]]
+        L.mx_paged_prefill_e4m3.argtypes = [desc, scales, *L.mx_paged_prefill.argtypes[1:]]
         for f in (L.mx_paged_decode_workspace_bytes, L.mx_paged_prefill_workspace_bytes):
             f.restype = ctypes.c_size_t
             f.argtypes = [desc]
@@ -318,24 +331,31 @@ def make_paged_rope(mode: int, base: float, axis_pairs, axis_restart: bool) -> M
 
 
 def paged_store_raw(desc: MxPagedDesc, rope: MxPagedRope, qkv: int, positions: int, k: int, v: int, table: int, kv_len: int,
-                    cu_q: int, q_out: int, stream: int) -> int:
-    """mx_paged_store on raw device addresses; returns the code."""
-    return lib().mx_paged_store(ctypes.byref(desc), ctypes.byref(rope), qkv or None, positions or None, k or None, v or None,
-                                table or None, kv_len or None, cu_q or None, q_out or None, stream or None)
+                    cu_q: int, q_out: int, stream: int, scales: MxPagedScales = None) -> int:
+    """mx_paged_store, or with scales mx_paged_store_e4m3, on raw device addresses; returns the code."""
+    rest = (qkv or None, positions or None, k or None, v or None, table or None, kv_len or None, cu_q or None, q_out or None, stream or None)
+    if scales is None:
+        return lib().mx_paged_store(ctypes.byref(desc), ctypes.byref(rope), *rest)
+    return lib().mx_paged_store_e4m3(ctypes.byref(desc), ctypes.byref(rope), ctypes.byref(scales), *rest)
 
 
 def paged_decode_raw(desc: MxPagedDesc, q: int, k: int, v: int, table: int, kv_len: int, out: int, lse: int, ws: int,
-                     ws_bytes: int, stream: int) -> int:
-    """mx_paged_decode on raw device addresses; returns the code."""
-    return lib().mx_paged_decode(ctypes.byref(desc), q or None, k or None, v or None, table or None, kv_len or None, out or None,
-                                 lse or None, ws or None, ws_bytes, stream or None)
+                     ws_bytes: int, stream: int, scales: MxPagedScales = None) -> int:
+    """mx_paged_decode, or with scales mx_paged_decode_e4m3, on raw device addresses; returns the code."""
+    rest = (q or None, k or None, v or None, table or None, kv_len or None, out or None, lse or None, ws or None, ws_bytes, stream or None)
+    if scales is None:
+        return lib().mx_paged_decode(ctypes.byref(desc), *rest)
+    return lib().mx_paged_decode_e4m3(ctypes.byref(desc), ctypes.byref(scales), *rest)
 
 
 def paged_prefill_raw(desc: MxPagedDesc, q: int, k: int, v: int, table: int, kv_len: int, cu_q: int, out: int, lse: int, ws: int,
-                      ws_bytes: int, stream: int) -> int:
-    """mx_paged_prefill on raw device addresses; returns the code."""
-    return lib().mx_paged_prefill(ctypes.byref(desc), q or None, k or None, v or None, table or None, kv_len or None, cu_q or None,
-                                  out or None, lse or None, ws or None, ws_bytes, stream or None)
+                      ws_bytes: int, stream: int, scales: MxPagedScales = None) -> int:
+    """mx_paged_prefill, or with scales mx_paged_prefill_e4m3, on raw device addresses; returns the code."""
+    rest = (q or None, k or None, v or None, table or None, kv_len or None, cu_q or None, out or None, lse or None, ws or None, ws_bytes,
+            stream or None)
+    if scales is None:
+        return lib().mx_paged_prefill(ctypes.byref(desc), *rest)
+    return lib().mx_paged_prefill_e4m3(ctypes.byref(desc), ctypes.byref(scales), *rest)
 
 
 def paged_decode_workspace_bytes(desc: MxPagedDesc) -> int:

@@ -65,7 +65,7 @@ def _native():
         except ImportError as e:
             raise ImportError(f"{e}: build the extension for this torch with `python -m dooms_amd.build`") from e
         else:
-            if not hasattr(ext, "bind_paged"):
+            if not hasattr(ext, "bind_paged_e4m3"):
                 raise ImportError("dooms_amd._native was built from other sources: build it with `python -m dooms_amd.build`")
             ext.bind(L.mx_attn_abi_version(),
                      tuple(ctypes.sizeof(t) for t in (_lib.MxAttnDesc, _lib.MxAttnRope, _lib.MxLinearDesc, _lib.MxSelfAttnDesc)),
@@ -76,6 +76,9 @@ def _native():
             ext.bind_paged(L.mx_attn_abi_version(), tuple(ctypes.sizeof(t) for t in (_lib.MxPagedDesc, _lib.MxPagedRope)),
                            *[ctypes.cast(getattr(L, f), ctypes.c_void_p).value
                              for f in ("mx_paged_store", "mx_paged_decode", "mx_paged_prefill")])
+            ext.bind_paged_e4m3(L.mx_attn_abi_version(), ctypes.sizeof(_lib.MxPagedScales),
+                                *[ctypes.cast(getattr(L, f), ctypes.c_void_p).value
+                                  for f in ("mx_paged_store_e4m3", "mx_paged_decode_e4m3", "mx_paged_prefill_e4m3")])
         _ext = ext   # before _bound: another thread that finds the library bound finds the extension too
         _bound = L
     return _ext
@@ -342,9 +345,28 @@ _PAGED_COUNTERS = 512 << 10  # bytes of counters at the start of a workspace
 _PAGE_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 
 
-def _paged_desc(rows, k_pages, v_pages, page_table, kv_len, cu_q, n_head, max_q=None, max_kv_len=None):
+def _paged_scales(scales, k_pages):
+    """The checked scales of pages in 8 bits, or None for pages in 16."""
+    if k_pages.dtype != torch.float8_e4m3fn:
+        if scales is not None:
+            raise ValueError("scales belong to float8_e4m3fn pages")
+        return None
+    if scales is None or len(scales) != 2:
+        raise ValueError("float8_e4m3fn pages need scales: those of the keys and those of the values")
+    n_pages, page_size, n_head_kv, _ = k_pages.shape
+    k, v = scales
+    for t in (k, v):
+        if t.device != k_pages.device or t.dtype != torch.float8_e8m0fnu or tuple(t.shape) != (n_pages, n_head_kv, page_size) or t.stride(2) != 1:
+            raise ValueError("scales must be float8_e8m0fnu [pages][kv heads][page size] tensors with unit stride along the page on the "
+                             "pages' device")
+    if any(n > 1 and a != b for n, a, b in zip(k.shape, k.stride(), v.stride())):
+        raise ValueError("the scales of the keys and of the values must share their strides")
+    return _lib.MxPagedScales(k=k.data_ptr(), v=v.data_ptr(), page_stride=k.stride(0), head_stride=k.stride(1))
+
+
+def _paged_desc(rows, k_pages, v_pages, page_table, kv_len, cu_q, n_head, max_q=None, max_kv_len=None, dtype=None):
     """The checked cache of a paged call as a descriptor (its rows' and outputs' types and strides are the caller's). Every
-    tensor has to be on the device of `rows`."""
+    tensor has to be on the device of `rows`. dtype: the queries' type, where the pages have 8 bits."""
     for t, name in ((rows, "rows"), (k_pages, "k_pages"), (v_pages, "v_pages"), (page_table, "page_table"), (kv_len, "kv_len"),
                     (cu_q, "cu_q")):
         if t is None:
@@ -353,9 +375,9 @@ def _paged_desc(rows, k_pages, v_pages, page_table, kv_len, cu_q, n_head, max_q=
             raise ValueError(f"{name} must be a device tensor")
         if t.device != rows.device:
             raise ValueError(f"{name} is on {t.device}, the rows on {rows.device}")
-    if k_pages.dim() != 4 or k_pages.stride(3) != 1 or k_pages.dtype not in _PAGE_DTYPES:
-        raise ValueError("k_pages must be a float16 or bfloat16 [pages][page size][kv heads][head dim] tensor with unit stride along "
-                         "the head dim")
+    if k_pages.dim() != 4 or k_pages.stride(3) != 1 or (k_pages.dtype not in _PAGE_DTYPES and k_pages.dtype != torch.float8_e4m3fn):
+        raise ValueError("k_pages must be a float16, bfloat16 or float8_e4m3fn [pages][page size][kv heads][head dim] tensor with unit "
+                         "stride along the head dim")
     if v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype or any(
             n > 1 and a != b for n, a, b in zip(k_pages.shape, k_pages.stride(), v_pages.stride())):  # a lone page or head has no stride
         raise ValueError("v_pages must have the shape, strides and type of k_pages")
@@ -369,7 +391,7 @@ def _paged_desc(rows, k_pages, v_pages, page_table, kv_len, cu_q, n_head, max_q=
     if cu_q is not None and (cu_q.dtype != torch.int32 or cu_q.shape != (n_seq + 1,) or not cu_q.is_contiguous()):
         raise ValueError("cu_q must be a contiguous int32 tensor of one entry more than sequences")
     n_pages, page_size, n_head_kv, head_dim = k_pages.shape
-    return _lib.MxPagedDesc(n_head=n_head, n_head_kv=n_head_kv, head_dim=head_dim, dtype=_PAGE_DTYPES[k_pages.dtype], n_seq=n_seq,
+    return _lib.MxPagedDesc(n_head=n_head, n_head_kv=n_head_kv, head_dim=head_dim, dtype=_PAGE_DTYPES[dtype or k_pages.dtype], n_seq=n_seq,
                             n_rows=rows.shape[0], page_size=page_size, n_pages=n_pages, max_pages=page_table.shape[1],
                             max_q=max_q or 0, max_kv_len=max_kv_len or 0, page_stride=k_pages.stride(0),
                             kv_stride=k_pages.stride(1), head_stride=k_pages.stride(2),
@@ -377,21 +399,33 @@ def _paged_desc(rows, k_pages, v_pages, page_table, kv_len, cu_q, n_head, max_q=
 
 
 def paged_store(qkv, k_pages, v_pages, page_table, kv_len, *, n_head, rope_mode, rope_base=10000.0, cu_q=None, positions=None,
-                axis_pairs=None, axis_restart=False, q=None, want_q=True):
+                axis_pairs=None, axis_restart=False, q=None, want_q=True, scales=None, q_dtype=None):
     """mx_paged_store, the append of a step's new tokens: qkv (f32, f16 or bf16) [rows][>= (n_head + 2 n_head_kv) hd] unrotated
     rows, each sequence's new tokens as cu_q has them (None: equally many each); kv_len counts them already. Their rotated keys
     and their values go into k_pages / v_pages ([pages][page size][kv heads][hd], f16 or bf16, any strides but the last). Returns
     the rotated queries, [rows][n_head hd] of the pages' type (None without want_q). positions: int32 [axes][rows] or [rows]
     (None: the cache positions); axis_pairs: rotary pairs of each axis (None: one axis); axis_restart: each axis has a frequency
-    ladder of its own."""
-    r = _native().paged_store(qkv, k_pages, v_pages, page_table, kv_len, n_head, rope_mode, rope_base, cu_q, positions, axis_pairs,
-                              axis_restart, q, want_q)
+    ladder of its own. Pages in 8 bits (mx_paged_store_e4m3): float8_e4m3fn pages with scales, those of the keys and of the values,
+    float8_e8m0fnu [pages][kv heads][page size]; the queries then have the type q_dtype, or that of q, or of qkv if it has 16 bits, or
+    float16."""
+    if scales is None:
+        r = _native().paged_store(qkv, k_pages, v_pages, page_table, kv_len, n_head, rope_mode, rope_base, cu_q, positions, axis_pairs,
+                                  axis_restart, q, want_q) if q_dtype is None else None
+    else:
+        r = _native().paged_store_e4m3(qkv, k_pages, v_pages, page_table, kv_len, n_head, rope_mode, rope_base, cu_q, positions,
+                                       axis_pairs, axis_restart, q, want_q, scales, q_dtype)
     if r is not None:
         return _result(r)
     if qkv.dtype not in _SA_DTYPES:
         raise ValueError("qkv must be float32, float16 or bfloat16")
     _rows(qkv, "qkv", qkv.dtype)
-    d = _paged_desc(qkv, k_pages, v_pages, page_table, kv_len, cu_q, n_head)
+    eight = k_pages.dtype == torch.float8_e4m3fn
+    if q_dtype is None:
+        q_dtype = k_pages.dtype if not eight else q.dtype if q is not None else qkv.dtype if qkv.dtype in _PAGE_DTYPES else torch.float16
+    if q_dtype not in _PAGE_DTYPES if eight else q_dtype != k_pages.dtype:
+        raise ValueError("the queries must have the pages' type, or be float16 or bfloat16 beside pages in 8 bits")
+    d = _paged_desc(qkv, k_pages, v_pages, page_table, kv_len, cu_q, n_head, dtype=q_dtype)
+    s = _paged_scales(scales, k_pages)
     d.row_dtype = _SA_DTYPES[qkv.dtype]
     if qkv.shape[1] < (n_head + 2 * d.n_head_kv) * d.head_dim:
         raise ValueError("qkv must be [rows][>= (n_head + 2 n_head_kv) head_dim]")
@@ -402,13 +436,13 @@ def paged_store(qkv, k_pages, v_pages, page_table, kv_len, *, n_head, rope_mode,
         if tuple(positions.shape) != (rope.n_axes, d.n_rows) and not (rope.n_axes == 1 and tuple(positions.shape) == (d.n_rows,)):
             raise ValueError("positions must be [axes][rows]")
     if want_q and q is None:
-        q = torch.empty(d.n_rows, n_head * d.head_dim, dtype=k_pages.dtype, device=qkv.device)
+        q = torch.empty(d.n_rows, n_head * d.head_dim, dtype=q_dtype, device=qkv.device)
     if q is not None:
-        _out_rows(q, "q", k_pages.dtype, d, qkv)
+        _out_rows(q, "q", q_dtype, d, qkv)
         d.out_stride = q.stride(0)
     with torch.cuda.device(qkv.device):
         _lib.check(_lib.paged_store_raw(d, rope, qkv.data_ptr(), _ptr(positions), k_pages.data_ptr(), v_pages.data_ptr(),
-                                        page_table.data_ptr(), kv_len.data_ptr(), _ptr(cu_q), _ptr(q), _stream()))
+                                        page_table.data_ptr(), kv_len.data_ptr(), _ptr(cu_q), _ptr(q), _stream(), s))
     return q
 
 
@@ -423,9 +457,12 @@ def _out_rows(out, name, dtype, d, like):
 
 
 def _paged_attend(q, k_pages, v_pages, page_table, kv_len, cu_q, n_head, causal, scale, out, out_dtype, lse, want_lse, max_q,
-                  max_kv_len, workspace, call, nbytes):
-    _rows(q, "q", k_pages.dtype)
-    d = _paged_desc(q, k_pages, v_pages, page_table, kv_len, cu_q, n_head, max_q, max_kv_len)
+                  max_kv_len, scales, workspace, call, nbytes):
+    if k_pages.dtype == torch.float8_e4m3fn and q.dtype not in _PAGE_DTYPES:
+        raise ValueError("q must be float16 or bfloat16 beside pages in 8 bits")
+    _rows(q, "q", q.dtype if k_pages.dtype == torch.float8_e4m3fn else k_pages.dtype)
+    d = _paged_desc(q, k_pages, v_pages, page_table, kv_len, cu_q, n_head, max_q, max_kv_len, q.dtype)
+    s = _paged_scales(scales, k_pages)
     if q.shape[1] < n_head * d.head_dim:
         raise ValueError("q must be [rows][>= n_head * head_dim]")
     if out_dtype is None:
@@ -452,32 +489,34 @@ def _paged_attend(q, k_pages, v_pages, page_table, kv_len, cu_q, n_head, causal,
                 _lib.check(_lib.decode_workspace_init(workspace.data_ptr(), min(need, _PAGED_COUNTERS), _stream()))
         elif workspace.device != q.device or not workspace.is_contiguous():
             raise ValueError("workspace must be a contiguous tensor on the rows' device")
-        rest = (out.data_ptr(), _ptr(lse), workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream())
+        rest = (out.data_ptr(), _ptr(lse), workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(), s)
         _lib.check(call(d, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), kv_len.data_ptr(),
                         *(() if cu_q is None else (cu_q.data_ptr(),)), *rest))
     return out, lse
 
 
 def paged_decode(q, k_pages, v_pages, page_table, kv_len, *, n_head, n_q=1, causal=True, scale=None, out=None, out_dtype=None, lse=None,
-                 want_lse=False, max_kv_len=None, workspace=None):
+                 want_lse=False, max_kv_len=None, scales=None, workspace=None):
     """mx_paged_decode: q [sequences * n_q][>= n_head hd], the n_q new rows of each sequence (rotated, of the pages' type), over
     its kv_len[b] keys in k_pages / v_pages; page_table int32 [sequences][pages] and kv_len int32 on the device. With causal, row
     t of the n_q sees the keys up to kv_len - n_q + t. max_kv_len: a length that no sequence is expected to pass, for the plan. The
-    output has the pages' type or out_dtype=torch.float32; workspace: paged_decode_workspace_bytes from new_workspace, kept by
-    the caller (None: made for this call). Returns (out, lse or None)."""
+    output has q's type or out_dtype=torch.float32; workspace: paged_decode_workspace_bytes from new_workspace, kept by
+    the caller (None: made for this call). Pages in 8 bits (mx_paged_decode_e4m3): float8_e4m3fn with scales as paged_store's, q
+    float16 or bfloat16. Returns (out, lse or None)."""
     if q.dim() == 2 and page_table.dim() == 2 and q.shape[0] != page_table.shape[0] * n_q:
         raise ValueError(f"q has {q.shape[0]} rows, not {n_q} for each of {page_table.shape[0]} sequences")
     if workspace is not None:
-        r = _native().paged_attend(q, k_pages, v_pages, page_table, kv_len, None, n_head, causal, scale, out, out_dtype, lse, want_lse,
-                                   None, max_kv_len, workspace)
+        args = (q, k_pages, v_pages, page_table, kv_len, None, n_head, causal, scale, out, out_dtype, lse, want_lse, None, max_kv_len,
+                workspace)
+        r = _native().paged_attend(*args) if scales is None else _native().paged_attend_e4m3(*args, scales)
         if r is not None:
             return _result(r)
     return _paged_attend(q, k_pages, v_pages, page_table, kv_len, None, n_head, causal, scale, out, out_dtype, lse, want_lse, None,
-                         max_kv_len, workspace, _lib.paged_decode_raw, _lib.paged_decode_workspace_bytes)
+                         max_kv_len, scales, workspace, _lib.paged_decode_raw, _lib.paged_decode_workspace_bytes)
 
 
 def paged_prefill(q, k_pages, v_pages, page_table, kv_len, cu_q, *, n_head, causal=True, scale=None, out=None, out_dtype=None,
-                  lse=None, want_lse=False, max_q=None, max_kv_len=None, workspace=None):
+                  lse=None, want_lse=False, max_q=None, max_kv_len=None, scales=None, workspace=None):
     """mx_paged_prefill: packed prompts, rows cu_q[b] .. cu_q[b + 1] - 1 (cu_q int32 on the device) the last of sequence b's
     kv_len[b] keys, which the pages hold already. max_q: the most rows of a sequence, for the plan. workspace:
     paged_prefill_workspace_bytes from new_workspace, kept by the caller; an empty tensor: no workgroups share a tile. Everything
@@ -485,12 +524,13 @@ def paged_prefill(q, k_pages, v_pages, page_table, kv_len, cu_q, *, n_head, caus
     if cu_q is None:
         raise ValueError("cu_q must be given")
     if workspace is not None:
-        r = _native().paged_attend(q, k_pages, v_pages, page_table, kv_len, cu_q, n_head, causal, scale, out, out_dtype, lse, want_lse,
-                                   max_q, max_kv_len, workspace)
+        args = (q, k_pages, v_pages, page_table, kv_len, cu_q, n_head, causal, scale, out, out_dtype, lse, want_lse, max_q, max_kv_len,
+                workspace)
+        r = _native().paged_attend(*args) if scales is None else _native().paged_attend_e4m3(*args, scales)
         if r is not None:
             return _result(r)
     return _paged_attend(q, k_pages, v_pages, page_table, kv_len, cu_q, n_head, causal, scale, out, out_dtype, lse, want_lse, max_q,
-                         max_kv_len, workspace, _lib.paged_prefill_raw, _lib.paged_prefill_workspace_bytes)
+                         max_kv_len, scales, workspace, _lib.paged_prefill_raw, _lib.paged_prefill_workspace_bytes)
 
 
 def paged_decode_workspace_bytes(*, n_head, n_head_kv, head_dim, n_q, n_seq, max_kv_len) -> int:

@@ -41,6 +41,9 @@ struct Api {
     decltype(&mx_paged_store) paged_store = nullptr;
     decltype(&mx_paged_decode) paged_decode = nullptr;
     decltype(&mx_paged_prefill) paged_prefill = nullptr;
+    decltype(&mx_paged_store_e4m3) paged_store_e4m3 = nullptr;
+    decltype(&mx_paged_decode_e4m3) paged_decode_e4m3 = nullptr;
+    decltype(&mx_paged_prefill_e4m3) paged_prefill_e4m3 = nullptr;
 };
 Api api;
 
@@ -388,17 +391,22 @@ const at::Tensor & ints(PyObject * o, int64_t n, const at::Tensor & like) {
     return t;
 }
 
-// k_pages, v_pages, page_table, kv_len at a; the rows' and outputs' types and strides are the caller's.
+// k_pages, v_pages, page_table, kv_len at a; the rows' and outputs' types and strides are the caller's, and where there are scales
+// (a pair for the keys and values, of pages in 8 bits) the queries' type.
 struct Paged {
     mx_paged_desc d{};
+    mx_paged_scales s{};
     const at::Tensor &k, &v, &table, &len;
-    at::ScalarType type;
-    Paged(PyObject * const * a, const at::Tensor & rows, PyObject * n_head)
+    at::ScalarType type;  // of the queries
+    Paged(PyObject * const * a, const at::Tensor & rows, PyObject * n_head, PyObject * scales = nullptr, at::ScalarType q_type = at::kHalf)
         : k(tensor(a[0])), v(tensor(a[1])), table(tensor(a[2])), len(ints(a[3], table.dim() == 2 ? table.size(0) : -1, rows)) {
-        type = k.scalar_type();
+        const at::ScalarType pages = k.scalar_type();
+        type = scales ? q_type : pages;
+        need(type == at::kHalf || type == at::kBFloat16);
+        need(!scales || pages == at::kFloat8_e4m3fn);
         need(rows.is_cuda() && k.device() == rows.device() && v.device() == rows.device() && table.device() == rows.device());
-        need(k.dim() == 4 && k.stride(3) == 1 && (type == at::kHalf || type == at::kBFloat16));
-        need(v.scalar_type() == type && v.sizes() == k.sizes());
+        need(k.dim() == 4 && k.stride(3) == 1);
+        need(v.scalar_type() == pages && v.sizes() == k.sizes());
         for (int i = 0; i < 4; i++) need(k.size(i) <= 1 || v.stride(i) == k.stride(i));
         need(table.scalar_type() == at::kInt && (table.stride(1) == 1 || table.size(1) <= 1));
         need(table.size(0) <= 1 || table.stride(0) >= table.size(1));
@@ -418,6 +426,19 @@ struct Paged {
         d.head_stride = k.stride(2);
         d.table_stride = std::max(table.stride(0), table.size(1));
         d.row_stride = rows.stride(0);
+        if (!scales) return;
+        const auto pair = items(scales);
+        need(pair.size() == 2);
+        const at::Tensor &sk = tensor(pair[0]), &sv = tensor(pair[1]);
+        for (const at::Tensor * t : {&sk, &sv}) {
+            need(t->device() == rows.device() && t->scalar_type() == at::kFloat8_e8m0fnu && t->dim() == 3 && t->stride(2) == 1);
+            need(t->size(0) == k.size(0) && t->size(1) == k.size(2) && t->size(2) == k.size(1));
+        }
+        for (int i = 0; i < 2; i++) need(sk.size(i) <= 1 || sk.stride(i) == sv.stride(i));
+        s.k = static_cast<uint8_t *>(sk.data_ptr());
+        s.v = static_cast<uint8_t *>(sv.data_ptr());
+        s.page_stride = sk.stride(0);
+        s.head_stride = sk.stride(1);
     }
     // the caller's rows of the output (checked) or new ones
     at::Tensor out(PyObject * o, at::ScalarType t, const at::Tensor & like) {
@@ -429,13 +450,24 @@ struct Paged {
     }
 };
 
-// qkv, k_pages, v_pages, page_table, kv_len, n_head, rope_mode, rope_base, cu_q, positions, axis_pairs, axis_restart, q, want_q
-PyObject * paged_store(PyObject * const * a) {
+// A type that the front end names, None: t.
+at::ScalarType dtype_or(PyObject * o, at::ScalarType t) {
+    if (o == Py_None) return t;
+    need(THPDtype_Check(o));
+    return reinterpret_cast<THPDtype *>(o)->scalar_type;
+}
+
+// qkv, k_pages, v_pages, page_table, kv_len, n_head, rope_mode, rope_base, cu_q, positions, axis_pairs, axis_restart, q, want_q; for
+// pages in 8 bits behind them scales and q_dtype
+template <bool Q8>
+PyObject * store(PyObject * const * a) {
     const at::Tensor & x0 = tensor(a[0]);
     const at::ScalarType t = x0.scalar_type();
     need(t == at::kFloat || t == at::kHalf || t == at::kBFloat16);
     const at::Tensor & x = rows(a[0], t);
-    Paged c(a + 1, x, a[5]);
+    at::ScalarType q_type = at::kHalf;
+    if constexpr (Q8) q_type = dtype_or(a[15], a[12] != Py_None ? tensor(a[12]).scalar_type() : t == at::kFloat ? at::kHalf : t);
+    Paged c(a + 1, x, a[5], Q8 ? a[14] : nullptr, q_type);
     c.d.row_dtype = element(t);
     need(x.size(1) >= ((int64_t)c.d.n_head + 2 * (int64_t)c.d.n_head_kv) * c.d.head_dim);
     const int32_t * cu = a[8] == Py_None ? nullptr : data<int32_t>(ints(a[8], c.d.n_seq + 1, x));
@@ -464,8 +496,12 @@ PyObject * paged_store(PyObject * const * a) {
     int32_t rc;
     {
         Unlocked u;
-        rc = api.paged_store(&c.d, &r, x.data_ptr(), pos, c.k.data_ptr(), c.v.data_ptr(), data<int32_t>(c.table), data<int32_t>(c.len),
-                             cu, q.data_ptr(), stream());
+        if constexpr (Q8)
+            rc = api.paged_store_e4m3(&c.d, &r, &c.s, x.data_ptr(), pos, c.k.data_ptr(), c.v.data_ptr(), data<int32_t>(c.table),
+                                      data<int32_t>(c.len), cu, q.data_ptr(), stream());
+        else
+            rc = api.paged_store(&c.d, &r, x.data_ptr(), pos, c.k.data_ptr(), c.v.data_ptr(), data<int32_t>(c.table),
+                                 data<int32_t>(c.len), cu, q.data_ptr(), stream());
     }
     if (rc) return code(rc);
     if (a[12] != Py_None) return Py_NewRef(a[12]);
@@ -473,19 +509,16 @@ PyObject * paged_store(PyObject * const * a) {
 }
 
 // q, k_pages, v_pages, page_table, kv_len, cu_q (None: as many rows for each sequence), n_head, causal, scale, out, out_dtype, lse,
-// want_lse, max_q, max_kv_len, workspace
-PyObject * paged_attend(PyObject * const * a) {
+// want_lse, max_q, max_kv_len, workspace; for pages in 8 bits behind them scales
+template <bool Q8>
+PyObject * attend(PyObject * const * a) {
     const at::Tensor & q0 = tensor(a[0]);
     const at::Tensor & q = rows(a[0], q0.scalar_type());
-    Paged c(a + 1, q, a[6]);
+    Paged c(a + 1, q, a[6], Q8 ? a[16] : nullptr, q.scalar_type());
     mx_paged_desc & d = c.d;
     need(q.scalar_type() == c.type && q.size(1) >= (int64_t)d.n_head * d.head_dim);
     const int32_t * cu = a[5] == Py_None ? nullptr : data<int32_t>(ints(a[5], d.n_seq + 1, q));
-    at::ScalarType t = a[9] == Py_None ? c.type : tensor(a[9]).scalar_type();
-    if (a[10] != Py_None) {
-        need(THPDtype_Check(a[10]));
-        t = reinterpret_cast<THPDtype *>(a[10])->scalar_type;
-    }
+    const at::ScalarType t = dtype_or(a[10], a[9] == Py_None ? c.type : tensor(a[9]).scalar_type());
     need(t == c.type || t == at::kFloat);
     d.row_dtype = element(t);
     d.causal = truth(a[7]);
@@ -504,13 +537,22 @@ PyObject * paged_attend(PyObject * const * a) {
     int32_t rc;
     {
         Unlocked u;
-        rc = cu ? api.paged_prefill(&d, q.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), data<int32_t>(c.table), data<int32_t>(c.len), cu,
-                                    out.data_ptr(), l, ws.data_ptr(), (size_t)ws.nbytes(), stream())
-                : api.paged_decode(&d, q.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), data<int32_t>(c.table), data<int32_t>(c.len),
-                                   out.data_ptr(), l, ws.data_ptr(), (size_t)ws.nbytes(), stream());
+        const void *x = q.data_ptr(), *k = c.k.data_ptr(), *v = c.v.data_ptr();
+        const int32_t *table = data<int32_t>(c.table), *len = data<int32_t>(c.len);
+        void *o = out.data_ptr(), *w = ws.data_ptr();
+        const size_t n = (size_t)ws.nbytes();
+        if constexpr (Q8)
+            rc = cu ? api.paged_prefill_e4m3(&d, &c.s, x, k, v, table, len, cu, o, l, w, n, stream())
+                    : api.paged_decode_e4m3(&d, &c.s, x, k, v, table, len, o, l, w, n, stream());
+        else
+            rc = cu ? api.paged_prefill(&d, x, k, v, table, len, cu, o, l, w, n, stream())
+                    : api.paged_decode(&d, x, k, v, table, len, o, l, w, n, stream());
     }
     return rc ? code(rc) : pair(out, a[9], lse, a[11]);
 }
+
+constexpr auto paged_store = store<false>, paged_store_e4m3 = store<true>;
+constexpr auto paged_attend = attend<false>, paged_attend_e4m3 = attend<true>;
 
 template <PyObject * (*F)(PyObject * const *), Py_ssize_t N>
 PyObject * entry(PyObject *, PyObject * const * args, Py_ssize_t n) {
@@ -580,12 +622,32 @@ PyObject * bind_paged(PyObject *, PyObject * args) {
     Py_RETURN_NONE;
 }
 
+// bind_paged_e4m3(version, size of mx_paged_scales, addresses of mx_paged_store_e4m3, _decode_e4m3, _prefill_e4m3): as bind.
+PyObject * bind_paged_e4m3(PyObject *, PyObject * args) {
+    int version;
+    Py_ssize_t scales;
+    unsigned long long p[3];
+    if (!PyArg_ParseTuple(args, "inKKK", &version, &scales, p, p + 1, p + 2)) return nullptr;
+    if (version != MX_ATTN_ABI_VERSION || (size_t)scales != sizeof(mx_paged_scales)) {
+        PyErr_SetString(PyExc_ImportError, "dooms_amd._native was built for other scales of pages: build both with `python -m dooms_amd.build`");
+        return nullptr;
+    }
+    auto set = [](auto & f, unsigned long long v) {
+        f = reinterpret_cast<std::remove_reference_t<decltype(f)>>((uintptr_t)v);
+    };
+    set(api.paged_store_e4m3, p[0]);
+    set(api.paged_decode_e4m3, p[1]);
+    set(api.paged_prefill_e4m3, p[2]);
+    Py_RETURN_NONE;
+}
+
 #define MX_ENTRY(name, n) \
     {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(entry<name, n>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     MX_ENTRY(decode, 14), MX_ENTRY(decode_rope, 14), MX_ENTRY(prefill, 14), MX_ENTRY(prefill_rope, 16), MX_ENTRY(linear, 8),
     MX_ENTRY(self_attention, 4), MX_ENTRY(paged_store, 14), MX_ENTRY(paged_attend, 16),
-    {"bind_paged", bind_paged, METH_VARARGS, nullptr}, {"bind", bind, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
+    MX_ENTRY(paged_store_e4m3, 16), MX_ENTRY(paged_attend_e4m3, 17),
+    {"bind_paged", bind_paged, METH_VARARGS, nullptr}, {"bind_paged_e4m3", bind_paged_e4m3, METH_VARARGS, nullptr}, {"bind", bind, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

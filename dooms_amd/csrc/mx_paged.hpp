@@ -23,6 +23,11 @@ struct F16 {
         const f16x2_t h = __builtin_bit_cast(f16x2_t, p);
         return make_float2((float)h[0], (float)h[1]);
     }
+    // two e4m3 codes (the lower or upper half of w) times the power of two `scale`; NaN codes and scales give NaN
+    template <bool HI>
+    static __device__ __forceinline__ uint32_t expand2(uint32_t w, float scale) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI));
+    }
     static constexpr uint32_t kExp = 0x7c00u;  // all exponent bits: infinities and NaN
 };
 struct BF16 {
@@ -39,6 +44,10 @@ struct BF16 {
     static __device__ __forceinline__ float2 unpack2(uint32_t p) {
         return make_float2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
     }
+    template <bool HI>
+    static __device__ __forceinline__ uint32_t expand2(uint32_t w, float scale) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
+    }
     static constexpr uint32_t kExp = 0x7f80u;
 };
 
@@ -51,6 +60,28 @@ __device__ __forceinline__ bool any_nonfinite(u32x4 w) {
         r |= (w[e] & T::kExp) == T::kExp || ((w[e] >> 16) & T::kExp) == T::kExp;
     return r;
 }
+
+// 8 codes of a row as T: exact where T holds the products (bf16 always, but for its smallest), else rounded to nearest even.
+template <class T>
+__device__ __forceinline__ u32x4 expand8(uint32_t lo, uint32_t hi, float scale) {
+    return u32x4{T::template expand2<false>(lo, scale), T::template expand2<true>(lo, scale), T::template expand2<false>(hi, scale),
+                 T::template expand2<true>(hi, scale)};
+}
+// Scale bytes of N rows in a row (N-byte aligned), and byte i of them as the float that the expansion takes: its exponent bits (255: NaN).
+template <int N>
+__device__ __forceinline__ uint32_t load_scales(const uint8_t * p) {
+    if constexpr (N == 1) return *(const __attribute__((address_space(1))) uint8_t *)(p);
+    else if constexpr (N == 2) return *(const __attribute__((address_space(1))) uint16_t *)(p);
+    else return *(const __attribute__((address_space(1))) uint32_t *)(p);
+}
+__device__ __forceinline__ float scale_of(uint32_t bytes, int i) { return __uint_as_float((bytes >> (8 * i) & 0xffu) << 23); }
+
+// Pages of e4m3 codes: a byte a row and kv head, the scale 2^(byte - 127), rows in a row.
+struct PagedScales {
+    uint8_t * k;
+    uint8_t * v;
+    int64_t page_stride, head_stride;
+};
 
 // Where the pages lie. `table` and `kv_len` are device memory that the host has not seen.
 struct PagedCache {
@@ -111,6 +142,7 @@ struct PagedStoreParams {
     int32_t n_head, n_head_kv, n_rows, n_q, rope_mode, n_axes;
     int32_t axis_end[kPagedMaxAxes];  // first pair behind each axis
     double freq[kMaxHeadDim / 2];
+    PagedScales s;  // pages of codes
 };
 
 struct PagedAttnParams {
@@ -135,6 +167,7 @@ struct PagedAttnParams {
     int32_t rows, n_rowtiles;  // decode: query rows that share a kv head, and their tiles
     float scale_log2;      // |scale| log2 e, or 1 with a scale of 0
     uint32_t q_xor, q_and; // scale < 0 turns the sign of the query rows, scale 0 makes them zero
+    PagedScales s;         // pages of codes
 };
 
 // Parts of a sequence in a decode at most: the join takes one lane each (131072 keys, Qwen2.5-7B heads, 54 us; with 33 67).
@@ -153,6 +186,10 @@ struct PagedPrefillPlan {
 
 hipError_t launch_paged_store(const PagedStoreParams & p, int head_dim, int in_dtype, int dtype, hipStream_t stream);
 hipError_t launch_paged_decode(const PagedAttnParams & p, int head_dim, int dtype, int rt, int waves, hipStream_t stream);
+// the same over pages of codes: the store's dtype is that of its queries
+hipError_t launch_paged_store_e4m3(const PagedStoreParams & p, int head_dim, int in_dtype, int dtype, hipStream_t stream);
+hipError_t launch_paged_decode_e4m3(const PagedAttnParams & p, int head_dim, int dtype, int rt, int waves, hipStream_t stream);
+hipError_t launch_paged_prefill_e4m3(const PagedAttnParams & p, int head_dim, int dtype, const PagedPrefillPlan & plan, hipStream_t stream);
 hipError_t launch_paged_prefill(const PagedAttnParams & p, int head_dim, int dtype, const PagedPrefillPlan & plan, hipStream_t stream);
 
 }  // namespace mx

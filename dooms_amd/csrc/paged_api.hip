@@ -52,8 +52,32 @@ int32_t check_uniform(const mx_paged_desc & d) {
     return MX_ATTN_OK;
 }
 
-// The pool, its strides and the table.
-int32_t check_cache(const mx_paged_desc & d) {
+// (page, row, head) rows of `width` elements apart from each other, strides in whole `unit`s: by ascending stride, each stride covers
+// what the smaller ones span.
+struct Dim {
+    int64_t stride, n;
+    const char * name;
+};
+int32_t check_strides(Dim * dim, int count, int64_t width, int unit) {
+    for (int i = 0; i < count; i++)
+        if (dim[i].n > 1 && (dim[i].stride < 0 || dim[i].stride % unit || dim[i].stride > (int64_t)1 << 46))
+            return fail(MX_ATTN_INVALID_ARGUMENT, "%s (%lld) must be a multiple of %d elements, >= 0", dim[i].name, (long long)dim[i].stride, unit);
+    std::sort(dim, dim + count, [](const Dim & a, const Dim & b) { return a.stride < b.stride; });
+    int64_t span = width;
+    for (int i = 0; i < count; i++) {
+        const Dim & x = dim[i];
+        if (x.n == 1) continue;
+        if (x.stride < span)
+            return fail(MX_ATTN_INVALID_ARGUMENT, "%s (%lld) makes rows of the pool overlap (%lld elements lie below it)", x.name,
+                        (long long)x.stride, (long long)span);
+        if (x.stride > ((int64_t)1 << 62) / x.n) return fail(MX_ATTN_INVALID_ARGUMENT, "%s (%lld) is out of range", x.name, (long long)x.stride);
+        span += x.stride * (x.n - 1);
+    }
+    return MX_ATTN_OK;
+}
+
+// The pool, its strides and the table; s: the scales of pages of codes, whose rows are loaded 16 bytes at a time as others are.
+int32_t check_cache(const mx_paged_desc & d, const mx_paged_scales * s) {
     if (d.page_size < 16 || d.page_size > 65536 || (d.page_size & (d.page_size - 1)))
         return fail(MX_ATTN_UNSUPPORTED, "page_size (%d) must be a power of two in [16, 65536]", d.page_size);
     if (d.n_pages < 1 || d.max_pages < 1)
@@ -64,25 +88,23 @@ int32_t check_cache(const mx_paged_desc & d) {
         return fail(MX_ATTN_INVALID_ARGUMENT, "table_stride (%lld) < max_pages (%d)", (long long)d.table_stride, d.max_pages);
     if (d.kv_stride > (int64_t)1 << 26)
         return fail(MX_ATTN_UNSUPPORTED, "kv_stride (%lld) beyond 2^26 elements", (long long)d.kv_stride);
-    // (page, row, head) rows of head_dim elements apart from each other: by ascending stride, each stride covers what the
-    // smaller ones span
-    struct Dim {
-        int64_t stride, n;
-        const char * name;
-    } dim[3] = {{d.page_stride, d.n_pages, "page_stride"}, {d.kv_stride, d.page_size, "kv_stride"}, {d.head_stride, d.n_head_kv, "head_stride"}};
-    for (const Dim & x : dim)
-        if (x.n > 1 && (x.stride < 0 || x.stride % 8 || x.stride > (int64_t)1 << 46))
-            return fail(MX_ATTN_INVALID_ARGUMENT, "%s (%lld) must be a multiple of 8 elements, >= 0", x.name, (long long)x.stride);
-    std::sort(dim, dim + 3, [](const Dim & a, const Dim & b) { return a.stride < b.stride; });
-    int64_t span = d.head_dim;
-    for (const Dim & x : dim) {
-        if (x.n == 1) continue;
-        if (x.stride < span)
-            return fail(MX_ATTN_INVALID_ARGUMENT, "%s (%lld) makes rows of the pool overlap (%lld elements lie below it)", x.name,
-                        (long long)x.stride, (long long)span);
-        if (x.stride > ((int64_t)1 << 62) / x.n) return fail(MX_ATTN_INVALID_ARGUMENT, "%s (%lld) is out of range", x.name, (long long)x.stride);
-        span += x.stride * (x.n - 1);
-    }
+    Dim dim[3] = {{d.page_stride, d.n_pages, "page_stride"}, {d.kv_stride, d.page_size, "kv_stride"}, {d.head_stride, d.n_head_kv, "head_stride"}};
+    if (int32_t rc = check_strides(dim, 3, d.head_dim, s ? 16 : 8)) return rc;
+    if (!s) return MX_ATTN_OK;
+    if (s->reserved != 0) return fail(MX_ATTN_INVALID_ARGUMENT, "scales->reserved must be 0");
+    Dim of_scales[2] = {{s->page_stride, d.n_pages, "scales->page_stride"}, {s->head_stride, d.n_head_kv, "scales->head_stride"}};
+    return check_strides(of_scales, 2, d.page_size, 16);
+}
+
+// The scales of a call that has work to do.
+int32_t scales_of(const mx_paged_scales * s, mx::PagedScales & to) {
+    if (!s) return MX_ATTN_OK;
+    if (!s->k || !s->v || !aligned(s->k, 16) || !aligned(s->v, 16))
+        return fail(MX_ATTN_INVALID_ARGUMENT, "scales->k and scales->v must be 16-byte aligned pointers");
+    to.k = s->k;
+    to.v = s->v;
+    to.page_stride = s->page_stride;
+    to.head_stride = s->head_stride;
     return MX_ATTN_OK;
 }
 
@@ -119,13 +141,13 @@ int32_t check_rows(const char * name, int64_t stride, int64_t width, int unit) {
 }
 
 // Checks of an attention call, and its parameters but for the plan.
-int32_t attn_params(const mx_paged_desc & d, const void * q, const void * k, const void * v, const int32_t * table,
+int32_t attn_params(const mx_paged_desc & d, const mx_paged_scales * s, const void * q, const void * k, const void * v, const int32_t * table,
                     const int32_t * kv_len, const int32_t * cu_q, void * out, float * lse, mx::PagedAttnParams & p) {
     if (d.row_dtype != d.dtype && d.row_dtype != MX_ATTN_F32)
         return fail(MX_ATTN_INVALID_ARGUMENT, "row_dtype (%d) must be MX_ATTN_F32 or dtype (%d)", d.row_dtype, d.dtype);
     if (d.causal != 0 && d.causal != 1) return fail(MX_ATTN_INVALID_ARGUMENT, "causal must be 0 or 1");
     if (!std::isfinite(d.scale)) return fail(MX_ATTN_INVALID_ARGUMENT, "scale is not finite");
-    if (int32_t rc = check_cache(d)) return rc;
+    if (int32_t rc = check_cache(d, s)) return rc;
     const int64_t wide = (int64_t)d.n_head * d.head_dim;
     const bool out32 = d.row_dtype == MX_ATTN_F32;
     if (int32_t rc = check_rows("row_stride", d.row_stride, wide, 8)) return rc;
@@ -135,6 +157,7 @@ int32_t attn_params(const mx_paged_desc & d, const void * q, const void * k, con
     if (!aligned(q, 16) || !aligned(out, 16)) return fail(MX_ATTN_INVALID_ARGUMENT, "q and out must be 16-byte aligned");
     if (!aligned(lse, 4)) return fail(MX_ATTN_INVALID_ARGUMENT, "lse must be 4-byte aligned");
     if (int32_t rc = check_pointers(k, v, table, kv_len, cu_q)) return rc;
+    if (int32_t rc = scales_of(s, p.s)) return rc;
     p.c = cache_of(d, k, v, table, kv_len);
     p.q = static_cast<const uint16_t *>(q);
     p.out = out;
@@ -269,13 +292,11 @@ size_t prefill_bytes(int head_dim) {
     return mx::kCounterBytes + (size_t)(r.resident(head_dim) * r.part_floats(head_dim)) * sizeof(float);
 }
 
-}  // namespace
+// ---- the calls, over pages of the queries' type (s null) or of codes ----
 
-extern "C" {
-
-MX_ATTN_API int32_t mx_paged_store(const mx_paged_desc * desc, const mx_paged_rope * rope, const void * qkv,
-                                   const int32_t * positions, void * k, void * v, const int32_t * table,
-                                   const int32_t * kv_len, const int32_t * cu_q, void * q_out, mx_attn_stream stream) {
+int32_t store(const mx_paged_desc * desc, const mx_paged_rope * rope, const mx_paged_scales * s, const void * qkv,
+              const int32_t * positions, void * k, void * v, const int32_t * table, const int32_t * kv_len, const int32_t * cu_q,
+              void * q_out, mx_attn_stream stream) {
     if (int32_t rc = check_shape(desc)) return rc;
     const mx_paged_desc & d = *desc;
     if (d.row_dtype != MX_ATTN_F32 && d.row_dtype != MX_ATTN_F16 && d.row_dtype != MX_ATTN_BF16)
@@ -312,7 +333,7 @@ MX_ATTN_API int32_t mx_paged_store(const mx_paged_desc * desc, const mx_paged_ro
         if (!positions && rope->n_axes > 1) return fail(MX_ATTN_INVALID_ARGUMENT, "positions must be given for more than one axis");
         if (!aligned(positions, 4)) return fail(MX_ATTN_INVALID_ARGUMENT, "positions must be 4-byte aligned");
     }
-    if (int32_t rc = check_cache(d)) return rc;
+    if (int32_t rc = check_cache(d, s)) return rc;
     const int64_t wide = (int64_t)d.n_head * d.head_dim, all = wide + 2 * (int64_t)d.n_head_kv * d.head_dim;
     if (int32_t rc = check_rows("row_stride", d.row_stride, all, d.row_dtype == MX_ATTN_F32 ? 4 : 8)) return rc;
     if (q_out)
@@ -323,6 +344,7 @@ MX_ATTN_API int32_t mx_paged_store(const mx_paged_desc * desc, const mx_paged_ro
     if (!qkv || !aligned(qkv, 16)) return fail(MX_ATTN_INVALID_ARGUMENT, "qkv must be a 16-byte aligned pointer");
     if (!aligned(q_out, 16)) return fail(MX_ATTN_INVALID_ARGUMENT, "q_out must be 16-byte aligned");
     if (int32_t rc = check_pointers(k, v, table, kv_len, cu_q)) return rc;
+    if (int32_t rc = scales_of(s, p.s)) return rc;
     p.c = cache_of(d, k, v, table, kv_len);
     p.qkv = qkv;
     p.positions = rope->mode == 2 ? nullptr : positions;
@@ -334,25 +356,19 @@ MX_ATTN_API int32_t mx_paged_store(const mx_paged_desc * desc, const mx_paged_ro
     p.n_head_kv = d.n_head_kv;
     p.n_rows = d.n_rows;
     p.n_q = d.n_rows / d.n_seq;
-    const hipError_t e = mx::launch_paged_store(p, d.head_dim, d.row_dtype, d.dtype, static_cast<hipStream_t>(stream));
+    const auto launch = s ? mx::launch_paged_store_e4m3 : mx::launch_paged_store;
+    const hipError_t e = launch(p, d.head_dim, d.row_dtype, d.dtype, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return fail(MX_ATTN_INTERNAL, "paged store launch: %s", hipGetErrorString(e));
     return MX_ATTN_OK;
 }
 
-MX_ATTN_API size_t mx_paged_decode_workspace_bytes(const mx_paged_desc * desc) {
-    if (check_shape(desc) || check_uniform(*desc) || desc->n_seq == 0 || desc->n_rows == 0) return 0;
-    DecodePlan plan;
-    return decode_plan(*desc, plan) ? 0 : plan.bytes;
-}
-
-MX_ATTN_API int32_t mx_paged_decode(const mx_paged_desc * desc, const void * q, const void * k, const void * v,
-                                    const int32_t * table, const int32_t * kv_len, void * out, float * lse, void * workspace,
-                                    size_t ws_bytes, mx_attn_stream stream) {
+int32_t decode(const mx_paged_desc * desc, const mx_paged_scales * s, const void * q, const void * k, const void * v, const int32_t * table,
+               const int32_t * kv_len, void * out, float * lse, void * workspace, size_t ws_bytes, mx_attn_stream stream) {
     if (int32_t rc = check_shape(desc)) return rc;
     const mx_paged_desc & d = *desc;
     if (int32_t rc = check_uniform(d)) return rc;
     mx::PagedAttnParams p{};
-    if (int32_t rc = attn_params(d, q, k, v, table, kv_len, nullptr, out, lse, p)) return rc;
+    if (int32_t rc = attn_params(d, s, q, k, v, table, kv_len, nullptr, out, lse, p)) return rc;
     if (d.n_seq == 0 || d.n_rows == 0) return MX_ATTN_OK;
     DecodePlan plan;
     if (int32_t rc = decode_plan(d, plan)) return rc;
@@ -371,23 +387,19 @@ MX_ATTN_API int32_t mx_paged_decode(const mx_paged_desc * desc, const void * q, 
     p.max_pages = d.max_pages;
     p.counters = static_cast<uint32_t *>(workspace);
     p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + mx::kCounterBytes);
-    const hipError_t e = mx::launch_paged_decode(p, d.head_dim, d.dtype, plan.rt, plan.waves, static_cast<hipStream_t>(stream));
+    const auto launch = s ? mx::launch_paged_decode_e4m3 : mx::launch_paged_decode;
+    const hipError_t e = launch(p, d.head_dim, d.dtype, plan.rt, plan.waves, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return fail(MX_ATTN_INTERNAL, "paged decode launch: %s", hipGetErrorString(e));
     return MX_ATTN_OK;
 }
 
-MX_ATTN_API size_t mx_paged_prefill_workspace_bytes(const mx_paged_desc * desc) {
-    if (check_shape(desc) || desc->n_seq == 0 || desc->n_rows == 0) return 0;
-    return prefill_bytes(desc->head_dim);
-}
-
-MX_ATTN_API int32_t mx_paged_prefill(const mx_paged_desc * desc, const void * q, const void * k, const void * v,
-                                     const int32_t * table, const int32_t * kv_len, const int32_t * cu_q, void * out, float * lse,
-                                     void * workspace, size_t ws_bytes, mx_attn_stream stream) {
+int32_t prefill(const mx_paged_desc * desc, const mx_paged_scales * s, const void * q, const void * k, const void * v, const int32_t * table,
+                const int32_t * kv_len, const int32_t * cu_q, void * out, float * lse, void * workspace, size_t ws_bytes,
+                mx_attn_stream stream) {
     if (int32_t rc = check_shape(desc)) return rc;
     const mx_paged_desc & d = *desc;
     mx::PagedAttnParams p{};
-    if (int32_t rc = attn_params(d, q, k, v, table, kv_len, cu_q, out, lse, p)) return rc;
+    if (int32_t rc = attn_params(d, s, q, k, v, table, kv_len, cu_q, out, lse, p)) return rc;
     if (d.n_seq == 0 || d.n_rows == 0) return MX_ATTN_OK;
     if (!cu_q) return fail(MX_ATTN_INVALID_ARGUMENT, "cu_q must not be null");
     const mx::PagedPrefillPlan plan = prefill_plan(d);
@@ -404,9 +416,64 @@ MX_ATTN_API int32_t mx_paged_prefill(const mx_paged_desc * desc, const void * q,
         return fail(MX_ATTN_RESOURCE_EXHAUSTED, "workspace of %zu bytes is smaller than the %zu bytes needed", ws_bytes, prefill_bytes(d.head_dim));
     p.counters = static_cast<uint32_t *>(workspace);
     p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + mx::kCounterBytes);
-    const hipError_t e = mx::launch_paged_prefill(p, d.head_dim, d.dtype, plan, static_cast<hipStream_t>(stream));
+    const auto launch = s ? mx::launch_paged_prefill_e4m3 : mx::launch_paged_prefill;
+    const hipError_t e = launch(p, d.head_dim, d.dtype, plan, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return fail(MX_ATTN_INTERNAL, "paged prefill launch: %s", hipGetErrorString(e));
     return MX_ATTN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+MX_ATTN_API int32_t mx_paged_store(const mx_paged_desc * desc, const mx_paged_rope * rope, const void * qkv,
+                                   const int32_t * positions, void * k, void * v, const int32_t * table,
+                                   const int32_t * kv_len, const int32_t * cu_q, void * q_out, mx_attn_stream stream) {
+    return store(desc, rope, nullptr, qkv, positions, k, v, table, kv_len, cu_q, q_out, stream);
+}
+
+MX_ATTN_API int32_t mx_paged_store_e4m3(const mx_paged_desc * desc, const mx_paged_rope * rope, const mx_paged_scales * scales,
+                                        const void * qkv, const int32_t * positions, void * k, void * v, const int32_t * table,
+                                        const int32_t * kv_len, const int32_t * cu_q, void * q_out, mx_attn_stream stream) {
+    if (!scales) return fail(MX_ATTN_INVALID_ARGUMENT, "scales is null");
+    return store(desc, rope, scales, qkv, positions, k, v, table, kv_len, cu_q, q_out, stream);
+}
+
+MX_ATTN_API size_t mx_paged_decode_workspace_bytes(const mx_paged_desc * desc) {
+    if (check_shape(desc) || check_uniform(*desc) || desc->n_seq == 0 || desc->n_rows == 0) return 0;
+    DecodePlan plan;
+    return decode_plan(*desc, plan) ? 0 : plan.bytes;
+}
+
+MX_ATTN_API int32_t mx_paged_decode(const mx_paged_desc * desc, const void * q, const void * k, const void * v,
+                                    const int32_t * table, const int32_t * kv_len, void * out, float * lse, void * workspace,
+                                    size_t ws_bytes, mx_attn_stream stream) {
+    return decode(desc, nullptr, q, k, v, table, kv_len, out, lse, workspace, ws_bytes, stream);
+}
+
+MX_ATTN_API int32_t mx_paged_decode_e4m3(const mx_paged_desc * desc, const mx_paged_scales * scales, const void * q, const void * k,
+                                         const void * v, const int32_t * table, const int32_t * kv_len, void * out, float * lse,
+                                         void * workspace, size_t ws_bytes, mx_attn_stream stream) {
+    if (!scales) return fail(MX_ATTN_INVALID_ARGUMENT, "scales is null");
+    return decode(desc, scales, q, k, v, table, kv_len, out, lse, workspace, ws_bytes, stream);
+}
+
+MX_ATTN_API size_t mx_paged_prefill_workspace_bytes(const mx_paged_desc * desc) {
+    if (check_shape(desc) || desc->n_seq == 0 || desc->n_rows == 0) return 0;
+    return prefill_bytes(desc->head_dim);
+}
+
+MX_ATTN_API int32_t mx_paged_prefill(const mx_paged_desc * desc, const void * q, const void * k, const void * v,
+                                     const int32_t * table, const int32_t * kv_len, const int32_t * cu_q, void * out, float * lse,
+                                     void * workspace, size_t ws_bytes, mx_attn_stream stream) {
+    return prefill(desc, nullptr, q, k, v, table, kv_len, cu_q, out, lse, workspace, ws_bytes, stream);
+}
+
+MX_ATTN_API int32_t mx_paged_prefill_e4m3(const mx_paged_desc * desc, const mx_paged_scales * scales, const void * q, const void * k,
+                                          const void * v, const int32_t * table, const int32_t * kv_len, const int32_t * cu_q,
+                                          void * out, float * lse, void * workspace, size_t ws_bytes, mx_attn_stream stream) {
+    if (!scales) return fail(MX_ATTN_INVALID_ARGUMENT, "scales is null");
+    return prefill(desc, scales, q, k, v, table, kv_len, cu_q, out, lse, workspace, ws_bytes, stream);
 }
 
 #ifdef MX_ATTN_TRACE

@@ -1,0 +1,10 @@
+// The append to pages of e4m3 codes.
+#include "paged_store_kernel.hpp"
+
+namespace mx {
+
+hipError_t launch_paged_store_e4m3(const PagedStoreParams & p, int head_dim, int in_dtype, int dtype, hipStream_t stream) {
+    return dtype == 1 ? launch_hd<F16, true>(p, head_dim, in_dtype, stream) : launch_hd<BF16, true>(p, head_dim, in_dtype, stream);
+}
+
+}  // namespace mx

@@ -25,6 +25,13 @@
  *   - query rows that see no key (kv_len 0, or rows of a causal call at positions below 0) give zeros and an lse of -inf;
  *   - cu_q entries are clamped to [0, n_rows] and have to ascend; what ranges that run backwards or overlap compute is undefined.
  *
+ * Pages in 8 bits. The calls named _e4m3 keep each row of a kv head as head_dim codes of the 8-bit float e4m3 (no infinities,
+ * largest 448) and one scale byte e, and the row stands for code x 2^(e - 127): half the memory of 16-bit pages and half the
+ * bytes of a decode, at half a step of 2^-4 on each element. The scale is a power of two: quantising and expanding round once and
+ * not twice, and a row's values do not depend on how a quotient is rounded. desc->dtype is then the type of the query rows, to which
+ * codes are expanded for the matrix cores: exact in bf16, and in f16 as a cache of f16 values would hold them (products past 65504
+ * are infinite, below 2^-14 they lose digits). A NaN code, or scale byte 255, stands for NaN.
+ *
  * Errors, streams and threading as mx_attn.h (the same codes and mx_attn_last_error()).
  */
 #ifndef MX_PAGED_H
@@ -64,6 +71,19 @@ typedef struct mx_paged_desc {
 } mx_paged_desc;
 
 /*
+ * The scales of pages in 8 bits: that of row `row` of page `page`, kv head g is the byte at page * page_stride + g * head_stride +
+ * row (rows of a page lie in a row) of k for the keys, v for the values. The pools' strides in mx_paged_desc count codes, and
+ * are multiples of 16 there.
+ */
+typedef struct mx_paged_scales {
+    uint8_t * k;          /* device, 16-byte aligned; written by mx_paged_store_e4m3 */
+    uint8_t * v;
+    int64_t page_stride;  /* bytes between pages and heads: multiples of 16 (any with one page or head) */
+    int64_t head_stride;
+    int32_t reserved;     /* must be 0 */
+} mx_paged_scales;
+
+/*
  * Rotary embedding. The head_dim / 2 pairs of a head are dealt to 1 .. 4 position axes in order, axis_pairs[a] pairs to axis a,
  * and pair i turns by positions[axis of i] * f(i). One axis is the ordinary embedding; several place image patches or video
  * frames (time, height, width).
@@ -100,6 +120,16 @@ MX_ATTN_API int32_t mx_paged_store(const mx_paged_desc * desc, const mx_paged_ro
                                    const int32_t * kv_len, const int32_t * cu_q, void * q_out, mx_attn_stream stream);
 
 /*
+ * mx_paged_store into pages in 8 bits. The scale of a row is 2^e with e the least (from -127 on) for which its largest finite
+ * magnitude, rotated in f32, is at most 448 x 2^e; each element is divided by it, which is exact, and rounded to nearest even. A
+ * row of zeros has scale byte 0. An infinity or NaN becomes a NaN code, and leaves the scale to the others. The queries are rounded
+ * to desc->dtype.
+ */
+MX_ATTN_API int32_t mx_paged_store_e4m3(const mx_paged_desc * desc, const mx_paged_rope * rope, const mx_paged_scales * scales,
+                                        const void * qkv, const int32_t * positions, void * k, void * v, const int32_t * table,
+                                        const int32_t * kv_len, const int32_t * cu_q, void * q_out, mx_attn_stream stream);
+
+/*
  * Attention of n_rows / n_seq new rows of each sequence (one: a decode step; a few: drafted tokens) over its pages. The work is
  * cut over the sequences' lengths on the device, read by each call (and each replay of a captured one).
  *
@@ -118,6 +148,11 @@ MX_ATTN_API int32_t mx_paged_decode(const mx_paged_desc * desc, const void * q, 
                                     const int32_t * table, const int32_t * kv_len, void * out, float * lse, void * workspace,
                                     size_t ws_bytes, mx_attn_stream stream);
 
+/* mx_paged_decode over pages in 8 bits, with the same workspace. */
+MX_ATTN_API int32_t mx_paged_decode_e4m3(const mx_paged_desc * desc, const mx_paged_scales * scales, const void * q, const void * k,
+                                         const void * v, const int32_t * table, const int32_t * kv_len, void * out, float * lse,
+                                         void * workspace, size_t ws_bytes, mx_attn_stream stream);
+
 /* Workspace bytes mx_paged_decode needs for desc (the strides and pools do not matter). 0 and the last error set for an
  * invalid descriptor. */
 MX_ATTN_API size_t mx_paged_decode_workspace_bytes(const mx_paged_desc * desc);
@@ -132,6 +167,11 @@ MX_ATTN_API size_t mx_paged_decode_workspace_bytes(const mx_paged_desc * desc);
 MX_ATTN_API int32_t mx_paged_prefill(const mx_paged_desc * desc, const void * q, const void * k, const void * v,
                                      const int32_t * table, const int32_t * kv_len, const int32_t * cu_q, void * out, float * lse,
                                      void * workspace, size_t ws_bytes, mx_attn_stream stream);
+
+/* mx_paged_prefill over pages in 8 bits, with the same workspace. */
+MX_ATTN_API int32_t mx_paged_prefill_e4m3(const mx_paged_desc * desc, const mx_paged_scales * scales, const void * q, const void * k,
+                                          const void * v, const int32_t * table, const int32_t * kv_len, const int32_t * cu_q,
+                                          void * out, float * lse, void * workspace, size_t ws_bytes, mx_attn_stream stream);
 
 /* Workspace bytes mx_paged_prefill needs for desc; 0 and the last error set for an invalid descriptor. */
 MX_ATTN_API size_t mx_paged_prefill_workspace_bytes(const mx_paged_desc * desc);

@@ -27,7 +27,7 @@ EXPORTS = ("mx_attn_abi_version", "mx_attn_last_error", "mx_attn_prefill", "mx_a
            "mx_attn_decode_workspace_bytes", "mx_attn_decode_workspace_init", "mx_self_attention",
            "mx_self_attention_workspace_bytes", "mx_paged_store", "mx_paged_decode", "mx_paged_decode_workspace_bytes",
            "mx_paged_prefill", "mx_paged_prefill_workspace_bytes", "mx_paged_store_e4m3", "mx_paged_decode_e4m3",
-           "mx_paged_prefill_e4m3")
+           "mx_paged_prefill_e4m3", "mx_paged_decode_shared", "mx_paged_decode_shared_workspace_bytes")
 
 ROPE_NORMAL = 0  # adjacent pairs (2i, 2i + 1): llama
 ROPE_NEOX = 1    # split halves (i, i + head_dim / 2): qwen2
@@ -91,6 +91,11 @@ class MxPagedScales(ctypes.Structure):
     """mx_paged_scales (include/mx_paged.h)."""
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
                 ("reserved", ctypes.c_int32)]
+
+
+class MxPagedPrefix(ctypes.Structure):
+    """mx_paged_prefix (include/mx_paged.h)."""
+    _fields_ = [("n_groups", ctypes.c_int32), ("reserved", ctypes.c_int32), ("cu_seq", ctypes.c_void_p), ("prefix_len", ctypes.c_void_p)]
 
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
@@ -174,6 +179,10 @@ def lib() -> ctypes.CDLL:
         L.mx_paged_store_e4m3.argtypes = [desc, rope, scales, *L.mx_paged_store.argtypes[2:]]
         L.mx_paged_decode_e4m3.argtypes = [desc, scales, *L.mx_paged_decode.argtypes[1:]]
         L.mx_paged_prefill_e4m3.argtypes = [desc, scales, *L.mx_paged_prefill.argtypes[1:]]
+        L.mx_paged_decode_shared.restype = ctypes.c_int32
+        L.mx_paged_decode_shared.argtypes = [desc, scales, ctypes.POINTER(MxPagedPrefix), *L.mx_paged_decode.argtypes[1:]]
+        L.mx_paged_decode_shared_workspace_bytes.restype = ctypes.c_size_t
+        L.mx_paged_decode_shared_workspace_bytes.argtypes = [desc, ctypes.c_int32]
         for f in (L.mx_paged_decode_workspace_bytes, L.mx_paged_prefill_workspace_bytes):
             f.restype = ctypes.c_size_t
             f.argtypes = [desc]
@@ -356,6 +365,18 @@ def paged_prefill_raw(desc: MxPagedDesc, q: int, k: int, v: int, table: int, kv_
     if scales is None:
         return lib().mx_paged_prefill(ctypes.byref(desc), *rest)
     return lib().mx_paged_prefill_e4m3(ctypes.byref(desc), ctypes.byref(scales), *rest)
+
+
+def paged_decode_shared_raw(desc: MxPagedDesc, prefix: MxPagedPrefix, q: int, k: int, v: int, table: int, kv_len: int, out: int,
+                            lse: int, ws: int, ws_bytes: int, stream: int, scales: MxPagedScales = None) -> int:
+    """mx_paged_decode_shared on raw device addresses; returns the code."""
+    return lib().mx_paged_decode_shared(ctypes.byref(desc), ctypes.byref(scales) if scales is not None else None,
+                                        ctypes.byref(prefix) if prefix is not None else None, q or None, k or None, v or None,
+                                        table or None, kv_len or None, out or None, lse or None, ws or None, ws_bytes, stream or None)
+
+
+def paged_decode_shared_workspace_bytes(desc: MxPagedDesc, n_groups: int) -> int:
+    return lib().mx_paged_decode_shared_workspace_bytes(ctypes.byref(desc), n_groups)
 
 
 def paged_decode_workspace_bytes(desc: MxPagedDesc) -> int:

@@ -65,7 +65,7 @@ def _native():
         except ImportError as e:
             raise ImportError(f"{e}: build the extension for this torch with `python -m dooms_amd.build`") from e
         else:
-            if not hasattr(ext, "bind_paged_e4m3"):
+            if not hasattr(ext, "bind_paged_more"):
                 raise ImportError("dooms_amd._native was built from other sources: build it with `python -m dooms_amd.build`")
             ext.bind(L.mx_attn_abi_version(),
                      tuple(ctypes.sizeof(t) for t in (_lib.MxAttnDesc, _lib.MxAttnRope, _lib.MxLinearDesc, _lib.MxSelfAttnDesc)),
@@ -76,9 +76,10 @@ def _native():
             ext.bind_paged(L.mx_attn_abi_version(), tuple(ctypes.sizeof(t) for t in (_lib.MxPagedDesc, _lib.MxPagedRope)),
                            *[ctypes.cast(getattr(L, f), ctypes.c_void_p).value
                              for f in ("mx_paged_store", "mx_paged_decode", "mx_paged_prefill")])
-            ext.bind_paged_e4m3(L.mx_attn_abi_version(), ctypes.sizeof(_lib.MxPagedScales),
+            ext.bind_paged_more(L.mx_attn_abi_version(), tuple(ctypes.sizeof(t) for t in (_lib.MxPagedScales, _lib.MxPagedPrefix)),
                                 *[ctypes.cast(getattr(L, f), ctypes.c_void_p).value
-                                  for f in ("mx_paged_store_e4m3", "mx_paged_decode_e4m3", "mx_paged_prefill_e4m3")])
+                                  for f in ("mx_paged_store_e4m3", "mx_paged_decode_e4m3", "mx_paged_prefill_e4m3",
+                                            "mx_paged_decode_shared")])
         _ext = ext   # before _bound: another thread that finds the library bound finds the extension too
         _bound = L
     return _ext
@@ -515,6 +516,31 @@ def paged_decode(q, k_pages, v_pages, page_table, kv_len, *, n_head, n_q=1, caus
                          max_kv_len, scales, workspace, _lib.paged_decode_raw, _lib.paged_decode_workspace_bytes)
 
 
+def paged_decode_shared(q, k_pages, v_pages, page_table, kv_len, cu_seq, prefix_len, *, n_head, n_q=1, causal=True, scale=None, out=None,
+                        out_dtype=None, lse=None, want_lse=False, max_own_len=None, scales=None, workspace=None):
+    """mx_paged_decode_shared: paged_decode of sequences that come in groups which share their first keys. cu_seq int32 [groups + 1]
+    and prefix_len int32 [groups] on the device: sequences cu_seq[g] .. cu_seq[g + 1] - 1 have the first prefix_len[g] keys in common,
+    in the pages that the group's first sequence has for them; kv_len counts them too, and every new row has to see them all. The
+    shared keys are read once for a group. max_own_len: the most keys of a sequence behind its prefix, for the plan. workspace:
+    paged_shared_workspace_bytes from new_workspace. Everything else as paged_decode. Returns (out, lse or None)."""
+    if q.dim() == 2 and page_table.dim() == 2 and q.shape[0] != page_table.shape[0] * n_q:
+        raise ValueError(f"q has {q.shape[0]} rows, not {n_q} for each of {page_table.shape[0]} sequences")
+    if workspace is not None:
+        r = _native().paged_attend_shared(q, k_pages, v_pages, page_table, kv_len, None, n_head, causal, scale, out, out_dtype, lse,
+                                          want_lse, None, max_own_len, workspace, scales, cu_seq, prefix_len)
+        if r is not None:
+            return _result(r)
+    for t, name in ((cu_seq, "cu_seq"), (prefix_len, "prefix_len")):
+        if t.device != q.device or t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor of one dimension on the rows' device")
+    if cu_seq.shape[0] != prefix_len.shape[0] + 1:
+        raise ValueError("cu_seq must have one entry more than prefix_len")
+    prefix = _lib.MxPagedPrefix(n_groups=prefix_len.shape[0], cu_seq=cu_seq.data_ptr(), prefix_len=prefix_len.data_ptr())
+    return _paged_attend(q, k_pages, v_pages, page_table, kv_len, None, n_head, causal, scale, out, out_dtype, lse, want_lse, None,
+                         max_own_len, scales, workspace, lambda d, *rest: _lib.paged_decode_shared_raw(d, prefix, *rest),
+                         lambda d: _lib.paged_decode_shared_workspace_bytes(d, prefix.n_groups))
+
+
 def paged_prefill(q, k_pages, v_pages, page_table, kv_len, cu_q, *, n_head, causal=True, scale=None, out=None, out_dtype=None,
                   lse=None, want_lse=False, max_q=None, max_kv_len=None, scales=None, workspace=None):
     """mx_paged_prefill: packed prompts, rows cu_q[b] .. cu_q[b + 1] - 1 (cu_q int32 on the device) the last of sequence b's
@@ -544,3 +570,11 @@ def paged_prefill_workspace_bytes(*, n_head, n_head_kv, head_dim, n_rows, n_seq,
     return _lib.paged_prefill_workspace_bytes(_lib.MxPagedDesc(
         n_head=n_head, n_head_kv=n_head_kv, head_dim=head_dim, dtype=_lib.DTYPE_F16, n_seq=n_seq, n_rows=n_rows, max_q=max_q,
         max_kv_len=max_kv_len))
+
+
+def paged_shared_workspace_bytes(*, n_head, n_head_kv, head_dim, n_q, n_seq, n_groups, max_own_len) -> int:
+    """Bytes of a workspace for paged_decode_shared of n_seq sequences of n_q rows in n_groups groups, with at most max_own_len keys
+    each behind the prefix."""
+    return _lib.paged_decode_shared_workspace_bytes(_lib.MxPagedDesc(
+        n_head=n_head, n_head_kv=n_head_kv, head_dim=head_dim, dtype=_lib.DTYPE_F16, n_seq=n_seq, n_rows=n_seq * n_q,
+        max_kv_len=max_own_len), n_groups)

@@ -44,6 +44,7 @@ struct Api {
     decltype(&mx_paged_store_e4m3) paged_store_e4m3 = nullptr;
     decltype(&mx_paged_decode_e4m3) paged_decode_e4m3 = nullptr;
     decltype(&mx_paged_prefill_e4m3) paged_prefill_e4m3 = nullptr;
+    decltype(&mx_paged_decode_shared) paged_decode_shared = nullptr;
 };
 Api api;
 
@@ -509,12 +510,14 @@ PyObject * store(PyObject * const * a) {
 }
 
 // q, k_pages, v_pages, page_table, kv_len, cu_q (None: as many rows for each sequence), n_head, causal, scale, out, out_dtype, lse,
-// want_lse, max_q, max_kv_len, workspace; for pages in 8 bits behind them scales
-template <bool Q8>
+// want_lse, max_q, max_kv_len, workspace; for pages in 8 bits behind them scales, for shared prefixes scales or None, cu_seq, prefix_len
+enum Attend { kPlain, kE4m3, kShared };
+template <Attend KIND>
 PyObject * attend(PyObject * const * a) {
     const at::Tensor & q0 = tensor(a[0]);
     const at::Tensor & q = rows(a[0], q0.scalar_type());
-    Paged c(a + 1, q, a[6], Q8 ? a[16] : nullptr, q.scalar_type());
+    PyObject * const scales = KIND == kPlain || a[16] == Py_None ? nullptr : a[16];
+    Paged c(a + 1, q, a[6], scales, q.scalar_type());
     mx_paged_desc & d = c.d;
     need(q.scalar_type() == c.type && q.size(1) >= (int64_t)d.n_head * d.head_dim);
     const int32_t * cu = a[5] == Py_None ? nullptr : data<int32_t>(ints(a[5], d.n_seq + 1, q));
@@ -534,6 +537,14 @@ PyObject * attend(PyObject * const * a) {
         need(lse.scalar_type() == at::kFloat && lse.device() == q.device() && lse.dim() == 2 && lse.size(0) == d.n_rows &&
              lse.size(1) == d.n_head && lse.is_contiguous());
     float * l = lse.defined() ? data<float>(lse) : nullptr;
+    [[maybe_unused]] mx_paged_prefix prefix{};
+    if constexpr (KIND == kShared) {
+        const at::Tensor & n = tensor(a[18]);
+        need(n.dim() == 1 && n.size(0) <= d.n_seq);
+        prefix.n_groups = (int32_t)n.size(0);
+        prefix.prefix_len = data<int32_t>(ints(a[18], n.size(0), q));
+        prefix.cu_seq = data<int32_t>(ints(a[17], n.size(0) + 1, q));
+    }
     int32_t rc;
     {
         Unlocked u;
@@ -541,7 +552,9 @@ PyObject * attend(PyObject * const * a) {
         const int32_t *table = data<int32_t>(c.table), *len = data<int32_t>(c.len);
         void *o = out.data_ptr(), *w = ws.data_ptr();
         const size_t n = (size_t)ws.nbytes();
-        if constexpr (Q8)
+        if constexpr (KIND == kShared)
+            rc = api.paged_decode_shared(&d, scales ? &c.s : nullptr, &prefix, x, k, v, table, len, o, l, w, n, stream());
+        else if constexpr (KIND == kE4m3)
             rc = cu ? api.paged_prefill_e4m3(&d, &c.s, x, k, v, table, len, cu, o, l, w, n, stream())
                     : api.paged_decode_e4m3(&d, &c.s, x, k, v, table, len, o, l, w, n, stream());
         else
@@ -552,7 +565,7 @@ PyObject * attend(PyObject * const * a) {
 }
 
 constexpr auto paged_store = store<false>, paged_store_e4m3 = store<true>;
-constexpr auto paged_attend = attend<false>, paged_attend_e4m3 = attend<true>;
+constexpr auto paged_attend = attend<kPlain>, paged_attend_e4m3 = attend<kE4m3>, paged_attend_shared = attend<kShared>;
 
 template <PyObject * (*F)(PyObject * const *), Py_ssize_t N>
 PyObject * entry(PyObject *, PyObject * const * args, Py_ssize_t n) {
@@ -622,14 +635,15 @@ PyObject * bind_paged(PyObject *, PyObject * args) {
     Py_RETURN_NONE;
 }
 
-// bind_paged_e4m3(version, size of mx_paged_scales, addresses of mx_paged_store_e4m3, _decode_e4m3, _prefill_e4m3): as bind.
-PyObject * bind_paged_e4m3(PyObject *, PyObject * args) {
+// bind_paged_more(version, (sizes of mx_paged_scales, mx_paged_prefix), addresses of mx_paged_store_e4m3, _decode_e4m3, _prefill_e4m3,
+// _decode_shared): as bind.
+PyObject * bind_paged_more(PyObject *, PyObject * args) {
     int version;
-    Py_ssize_t scales;
-    unsigned long long p[3];
-    if (!PyArg_ParseTuple(args, "inKKK", &version, &scales, p, p + 1, p + 2)) return nullptr;
-    if (version != MX_ATTN_ABI_VERSION || (size_t)scales != sizeof(mx_paged_scales)) {
-        PyErr_SetString(PyExc_ImportError, "dooms_amd._native was built for other scales of pages: build both with `python -m dooms_amd.build`");
+    Py_ssize_t scales, prefix;
+    unsigned long long p[4];
+    if (!PyArg_ParseTuple(args, "i(nn)KKKK", &version, &scales, &prefix, p, p + 1, p + 2, p + 3)) return nullptr;
+    if (version != MX_ATTN_ABI_VERSION || (size_t)scales != sizeof(mx_paged_scales) || (size_t)prefix != sizeof(mx_paged_prefix)) {
+        PyErr_SetString(PyExc_ImportError, "dooms_amd._native was built for other scales or prefixes: build both with `python -m dooms_amd.build`");
         return nullptr;
     }
     auto set = [](auto & f, unsigned long long v) {
@@ -638,6 +652,7 @@ PyObject * bind_paged_e4m3(PyObject *, PyObject * args) {
     set(api.paged_store_e4m3, p[0]);
     set(api.paged_decode_e4m3, p[1]);
     set(api.paged_prefill_e4m3, p[2]);
+    set(api.paged_decode_shared, p[3]);
     Py_RETURN_NONE;
 }
 
@@ -646,8 +661,8 @@ PyObject * bind_paged_e4m3(PyObject *, PyObject * args) {
 PyMethodDef methods[] = {
     MX_ENTRY(decode, 14), MX_ENTRY(decode_rope, 14), MX_ENTRY(prefill, 14), MX_ENTRY(prefill_rope, 16), MX_ENTRY(linear, 8),
     MX_ENTRY(self_attention, 4), MX_ENTRY(paged_store, 14), MX_ENTRY(paged_attend, 16),
-    MX_ENTRY(paged_store_e4m3, 16), MX_ENTRY(paged_attend_e4m3, 17),
-    {"bind_paged", bind_paged, METH_VARARGS, nullptr}, {"bind_paged_e4m3", bind_paged_e4m3, METH_VARARGS, nullptr}, {"bind", bind, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
+    MX_ENTRY(paged_store_e4m3, 16), MX_ENTRY(paged_attend_e4m3, 17), MX_ENTRY(paged_attend_shared, 19),
+    {"bind_paged", bind_paged, METH_VARARGS, nullptr}, {"bind_paged_more", bind_paged_more, METH_VARARGS, nullptr}, {"bind", bind, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -145,6 +145,24 @@ struct PagedStoreParams {
     PagedScales s;  // pages of codes
 };
 
+// Sequences that share their first keys: groups of them, and what the prefixes' kernel leaves for the decode behind it.
+struct PagedPrefix {
+    const int32_t * cu_seq;      // [n_groups + 1]: sequences cu_seq[g] .. cu_seq[g + 1] - 1 are group g's
+    const int32_t * prefix_len;  // [n_groups]
+    int32_t n_groups;
+    int64_t max_rows;            // rows that `part` has room for
+    float * part;                // partials: head_dim + 4 floats a row
+    int32_t * rows;              // rows of the partials of a kv head
+    int32_t * start;             // [n_seq]: keys that are shared
+    int32_t * own_len;           // [n_seq]: keys from the multiple of 16 at or below them on; -1: a length that is none
+    int4 * info;                 // [n_seq]: the group's first row among the partials, its rows, parts, the sequence's row among them
+};
+struct PagedPrefixPart {  // of a workgroup
+    int64_t first;  // first row
+    int32_t rows;
+};
+constexpr int kPagedPrefixWaves = 4;
+
 struct PagedAttnParams {
     PagedCache c;
     const uint16_t * q;
@@ -168,6 +186,7 @@ struct PagedAttnParams {
     float scale_log2;      // |scale| log2 e, or 1 with a scale of 0
     uint32_t q_xor, q_and; // scale < 0 turns the sign of the query rows, scale 0 makes them zero
     PagedScales s;         // pages of codes
+    PagedPrefix x;         // shared prefixes
 };
 
 // Parts of a sequence in a decode at most: the join takes one lane each (131072 keys, Qwen2.5-7B heads, 54 us; with 33 67).
@@ -191,5 +210,9 @@ hipError_t launch_paged_store_e4m3(const PagedStoreParams & p, int head_dim, int
 hipError_t launch_paged_decode_e4m3(const PagedAttnParams & p, int head_dim, int dtype, int rt, int waves, hipStream_t stream);
 hipError_t launch_paged_prefill_e4m3(const PagedAttnParams & p, int head_dim, int dtype, const PagedPrefillPlan & plan, hipStream_t stream);
 hipError_t launch_paged_prefill(const PagedAttnParams & p, int head_dim, int dtype, const PagedPrefillPlan & plan, hipStream_t stream);
+
+hipError_t launch_paged_prefix(const PagedAttnParams & p, int head_dim, int dtype, bool e4m3, uint32_t grid, hipStream_t stream);
+hipError_t launch_paged_decode_shared(const PagedAttnParams & p, int head_dim, int dtype, int rt, hipStream_t stream);
+hipError_t launch_paged_decode_shared_e4m3(const PagedAttnParams & p, int head_dim, int dtype, int rt, hipStream_t stream);
 
 }  // namespace mx

@@ -195,7 +195,8 @@ int64_t kv_bound(const mx_paged_desc & d) {
     return d.max_kv_len > 0 && d.max_kv_len < table ? d.max_kv_len : table;
 }
 
-int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
+// four: the kernels have 4 waves only.
+int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan, bool four = false) {
     const int n_q = d.n_rows / d.n_seq;
     if ((int64_t)n_q * (d.n_head / d.n_head_kv) > 65536)
         return fail(MX_ATTN_UNSUPPORTED, "%d rows a sequence are a prompt (mx_paged_prefill)", n_q);
@@ -233,7 +234,7 @@ int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
         // against 10.6; 8192, Llama-3-8B heads, 11.3 against 14.8), and so have tiles of more rows. At head dim 256 the LDS holds 4
         // waves.
         plan.whole_keys = d.head_dim == 64 ? 640 : 512;
-        plan.waves = d.head_dim == 256 || bound <= 128 || (plan.rt <= 8 && bound > plan.whole_keys && bound <= 2048) ? 4 : 8;
+        plan.waves = four || d.head_dim == 256 || bound <= 128 || (plan.rt <= 8 && bound > plan.whole_keys && bound <= 2048) ? 4 : 8;
         if (plan.waves == 4) plan.whole_keys = 256;
         plan.ranges = (int32_t)std::max<int64_t>(d.n_seq, (plan.waves == 8 ? 1 : 2) * kCUs / per_seq);
         // Where one round of workgroups has room for every quantum of every sequence the chunks need no planning from the lengths:
@@ -251,6 +252,20 @@ int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
     // workspace serves all calls of a head shape and row count.
     plan.bytes = plan.whole ? 0 : mx::kCounterBytes + (size_t)(2 * std::max<int64_t>(1, 2 * kCUs / per_seq) * per_seq * plan.rt * (d.head_dim + 4)) * sizeof(float);
     return MX_ATTN_OK;
+}
+
+void decode_params(const mx_paged_desc & d, const DecodePlan & plan, void * workspace, mx::PagedAttnParams & p) {
+    p.n_q = d.n_rows / d.n_seq;
+    p.rows = plan.rows;
+    p.n_rowtiles = plan.n_rowtiles;
+    p.by_ranges = plan.by_ranges;
+    p.whole_keys = plan.whole_keys;
+    p.ranges = plan.ranges;
+    p.fixed = plan.fixed;
+    p.whole = plan.whole;
+    p.max_pages = d.max_pages;
+    p.counters = static_cast<uint32_t *>(workspace);
+    p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + mx::kCounterBytes);
 }
 
 // ---- prefill ----
@@ -290,6 +305,41 @@ mx::PagedPrefillPlan prefill_plan(const mx_paged_desc & d) {
 size_t prefill_bytes(int head_dim) {
     const mx::PagedPrefillPlan r{4, 1};
     return mx::kCounterBytes + (size_t)(r.resident(head_dim) * r.part_floats(head_dim)) * sizeof(float);
+}
+
+// ---- shared prefixes ----
+
+// How the two launches run, and where in the workspace their data lies: the decode's part as it is, then what the first leaves.
+struct SharedPlan {
+    DecodePlan own;
+    uint32_t grid;     // of the prefixes' launch
+    int32_t resident;  // its workgroups that run at once
+    int64_t max_rows;  // rows of its partials
+    size_t rows, start, own_len, info, part, bytes;  // offsets
+};
+
+int32_t shared_plan(const mx_paged_desc & d, int64_t n_groups, SharedPlan & plan) {
+    if (n_groups < 0 || n_groups > d.n_seq) return fail(MX_ATTN_INVALID_ARGUMENT, "n_groups (%lld) must be in [0, n_seq]", (long long)n_groups);
+    if ((int64_t)d.n_rows * d.n_head > (int64_t)1 << 26)
+        return fail(MX_ATTN_UNSUPPORTED, "%d rows of %d heads are more than one launch holds", d.n_rows, d.n_head);
+    // a sequence's own keys are walked from a multiple of 16 on: up to 15 more than it has
+    mx_paged_desc own = d;
+    own.max_kv_len = d.max_kv_len ? (int32_t)std::min<int64_t>((int64_t)d.max_kv_len + 15, INT32_MAX) : 0;
+    if (int32_t rc = decode_plan(own, plan.own, true)) return rc;
+    // groups of one sequence have no part here: at most n_seq / 2 tiles are not full
+    constexpr int kTile = 32 * mx::kPagedPrefixWaves;
+    const int64_t rows = (int64_t)d.n_rows * (d.n_head / d.n_head_kv), tiles = rows / kTile + std::min<int64_t>(n_groups, d.n_seq / 2) + 1;
+    plan.resident = d.head_dim == 256 ? kCUs : 2 * kCUs;
+    plan.grid = (uint32_t)std::max<int64_t>(plan.resident, tiles * d.n_head_kv);
+    plan.max_rows = std::max<int64_t>((int64_t)plan.resident * kTile, (int64_t)d.n_rows * d.n_head);
+    auto round = [](size_t n) { return (n + 255) / 256 * 256; };
+    plan.rows = round(std::max<size_t>(plan.own.bytes, mx::kCounterBytes));
+    plan.start = plan.rows + 256;
+    plan.own_len = plan.start + round(4 * (size_t)d.n_seq);
+    plan.info = plan.own_len + round(4 * (size_t)d.n_seq);
+    plan.part = plan.info + round(16 * (size_t)d.n_seq);
+    plan.bytes = plan.part + (size_t)plan.max_rows * (d.head_dim + 4) * sizeof(float);
+    return MX_ATTN_OK;
 }
 
 // ---- the calls, over pages of the queries' type (s null) or of codes ----
@@ -376,17 +426,7 @@ int32_t decode(const mx_paged_desc * desc, const mx_paged_scales * s, const void
         return fail(MX_ATTN_INVALID_ARGUMENT, "a 256-byte aligned workspace of %zu bytes is needed", plan.bytes);
     if (ws_bytes < plan.bytes)
         return fail(MX_ATTN_RESOURCE_EXHAUSTED, "workspace of %zu bytes is smaller than the %zu bytes needed", ws_bytes, plan.bytes);
-    p.n_q = d.n_rows / d.n_seq;
-    p.rows = plan.rows;
-    p.n_rowtiles = plan.n_rowtiles;
-    p.by_ranges = plan.by_ranges;
-    p.whole_keys = plan.whole_keys;
-    p.ranges = plan.ranges;
-    p.fixed = plan.fixed;
-    p.whole = plan.whole;
-    p.max_pages = d.max_pages;
-    p.counters = static_cast<uint32_t *>(workspace);
-    p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + mx::kCounterBytes);
+    decode_params(d, plan, workspace, p);
     const auto launch = s ? mx::launch_paged_decode_e4m3 : mx::launch_paged_decode;
     const hipError_t e = launch(p, d.head_dim, d.dtype, plan.rt, plan.waves, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return fail(MX_ATTN_INTERNAL, "paged decode launch: %s", hipGetErrorString(e));
@@ -474,6 +514,55 @@ MX_ATTN_API int32_t mx_paged_prefill_e4m3(const mx_paged_desc * desc, const mx_p
                                           void * out, float * lse, void * workspace, size_t ws_bytes, mx_attn_stream stream) {
     if (!scales) return fail(MX_ATTN_INVALID_ARGUMENT, "scales is null");
     return prefill(desc, scales, q, k, v, table, kv_len, cu_q, out, lse, workspace, ws_bytes, stream);
+}
+
+MX_ATTN_API size_t mx_paged_decode_shared_workspace_bytes(const mx_paged_desc * desc, int32_t n_groups) {
+    if (check_shape(desc) || check_uniform(*desc) || desc->n_seq == 0 || desc->n_rows == 0) return 0;
+    SharedPlan plan;
+    return shared_plan(*desc, n_groups, plan) ? 0 : plan.bytes;
+}
+
+MX_ATTN_API int32_t mx_paged_decode_shared(const mx_paged_desc * desc, const mx_paged_scales * scales, const mx_paged_prefix * prefix,
+                                           const void * q, const void * k, const void * v, const int32_t * table,
+                                           const int32_t * kv_len, void * out, float * lse, void * workspace, size_t ws_bytes,
+                                           mx_attn_stream stream) {
+    if (int32_t rc = check_shape(desc)) return rc;
+    const mx_paged_desc & d = *desc;
+    if (int32_t rc = check_uniform(d)) return rc;
+    if (!prefix) return fail(MX_ATTN_INVALID_ARGUMENT, "prefix is null");
+    if (prefix->reserved != 0) return fail(MX_ATTN_INVALID_ARGUMENT, "prefix->reserved must be 0");
+    mx::PagedAttnParams p{};
+    if (int32_t rc = attn_params(d, scales, q, k, v, table, kv_len, nullptr, out, lse, p)) return rc;
+    if (d.n_seq == 0 || d.n_rows == 0) return MX_ATTN_OK;
+    SharedPlan plan;
+    if (int32_t rc = shared_plan(d, prefix->n_groups, plan)) return rc;
+    if (!workspace || !aligned(workspace, 256))
+        return fail(MX_ATTN_INVALID_ARGUMENT, "a 256-byte aligned workspace of %zu bytes is needed", plan.bytes);
+    if (ws_bytes < plan.bytes)
+        return fail(MX_ATTN_RESOURCE_EXHAUSTED, "workspace of %zu bytes is smaller than the %zu bytes needed", ws_bytes, plan.bytes);
+    if (prefix->n_groups == 0) return decode(desc, scales, q, k, v, table, kv_len, out, lse, workspace, ws_bytes, stream);
+    if (!prefix->cu_seq || !prefix->prefix_len || !aligned(prefix->cu_seq, 4) || !aligned(prefix->prefix_len, 4))
+        return fail(MX_ATTN_INVALID_ARGUMENT, "prefix->cu_seq and prefix->prefix_len must be 4-byte aligned pointers");
+    char * const ws = static_cast<char *>(workspace);
+    p.x.cu_seq = prefix->cu_seq;
+    p.x.prefix_len = prefix->prefix_len;
+    p.x.n_groups = prefix->n_groups;
+    p.x.max_rows = plan.max_rows;
+    p.x.part = reinterpret_cast<float *>(ws + plan.part);
+    p.x.rows = reinterpret_cast<int32_t *>(ws + plan.rows);
+    p.x.start = reinterpret_cast<int32_t *>(ws + plan.start);
+    p.x.own_len = reinterpret_cast<int32_t *>(ws + plan.own_len);
+    p.x.info = reinterpret_cast<int4 *>(ws + plan.info);
+    p.n_q = d.n_rows / d.n_seq;
+    p.ranges = plan.resident;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    hipError_t e = mx::launch_paged_prefix(p, d.head_dim, d.dtype, scales != nullptr, plan.grid, s);
+    if (e != hipSuccess) return fail(MX_ATTN_INTERNAL, "shared prefix launch: %s", hipGetErrorString(e));
+    decode_params(d, plan.own, workspace, p);
+    p.c.kv_len = p.x.own_len;
+    e = (scales ? mx::launch_paged_decode_shared_e4m3 : mx::launch_paged_decode_shared)(p, d.head_dim, d.dtype, plan.own.rt, s);
+    if (e != hipSuccess) return fail(MX_ATTN_INTERNAL, "shared decode launch: %s", hipGetErrorString(e));
+    return MX_ATTN_OK;
 }
 
 #ifdef MX_ATTN_TRACE

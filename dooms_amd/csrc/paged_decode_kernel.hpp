@@ -188,8 +188,10 @@ __device__ __forceinline__ u32x4 load_kv(const char * a) {
 
 // HD: head_dim. RT: query rows per tile (4, 8, 16 or 32; the matrix products have 16 or 32, the others are zero). T: type of
 // query rows and pages. NW: waves. RANGES: a workgroup walks a range of the launch's keys over the sequences in it, else one chunk.
-// Q8: the pages hold e4m3 codes with a scale a row, expanded to T on their way to LDS.
-template <int HD, int RT, class T, int NW, bool RANGES, bool Q8>
+// Q8: the pages hold e4m3 codes with a scale a row, expanded to T on their way to LDS. SHARED: the sequences' first keys are done
+// already (PagedPrefix): positions count from the multiple of 16 at or below the first other key, and the prefix's partials are joined
+// in behind the sequence's own.
+template <int HD, int RT, class T, int NW, bool RANGES, bool Q8, bool SHARED>
 __global__ __launch_bounds__(NW * kWave) __attribute__((amdgpu_waves_per_eu(HD == 256 || RANGES ? 1 : 2)))
 void paged_decode_kernel(PagedAttnParams p) {
     constexpr int QT = RT > 16 ? 2 : 1;  // 16-row product tiles
@@ -242,8 +244,9 @@ void paged_decode_kernel(PagedAttnParams p) {
     const uint32_t kv_stride = (uint32_t)p.c.kv_stride;
     // page numbers of the two halves of the block at key jb, in lanes 0 and 1 (past the table: its last entry; numbers behind the
     // last key are not used)
-    auto read_ids = [&](int b, int jb) {
-        return p.c.table[b * p.c.table_stride + min((uint32_t)(jb + 16 * (lane & 1)) >> shift, (uint32_t)p.max_pages - 1)];
+    auto read_ids = [&](int b, int jb, int start) {
+        const int from = SHARED ? start & ~15 : 0;
+        return p.c.table[b * p.c.table_stride + min((uint32_t)(from + jb + 16 * (lane & 1)) >> shift, (uint32_t)p.max_pages - 1)];
     };
 
     // this lane's rows of a product tile: local row, sequence row, head, last visible key
@@ -262,12 +265,17 @@ void paged_decode_kernel(PagedAttnParams p) {
     // is number at
     struct Seg {
         int b, at, L, k1;
+        int start;  // SHARED: keys in common with other sequences
     };
     Seg seg;
     int key0, ids[D];
     Range x{};
     Chunk ch{};
     int lens = 0, lens0 = 0;  // RANGES: the lengths of 64 sequences from lens0 on
+    int starts = 0;           // RANGES and SHARED: where they start
+    auto read_starts = [&]() __attribute__((always_inline)) {
+        if constexpr (SHARED) starts = p.x.start[min(lens0 + lane, n_seq - 1)];
+    };
     auto segment = [&](Seg & s, int len) __attribute__((always_inline)) {  // of s.b and s.at; returns its first key
         s.L = length_ok(p.c, len) ? len : -1;
         const int q1 = x.hi - s.at;
@@ -282,7 +290,9 @@ void paged_decode_kernel(PagedAttnParams p) {
                 if ((uint32_t)(s.b - lens0) >= (uint32_t)kWave) {
                     lens0 = s.b;
                     lens = p.c.kv_len[min(lens0 + lane, n_seq - 1)];
+                    read_starts();
                 }
+                s.start = SHARED ? __builtin_amdgcn_readlane(starts, s.b - lens0) : 0;
                 segment(s, __builtin_amdgcn_readlane(lens, s.b - lens0));
                 return;
             }
@@ -292,8 +302,10 @@ void paged_decode_kernel(PagedAttnParams p) {
     if constexpr (RANGES) {
         x = find_range<kStep>(p, r, lane, lens, lens0);
         if (x.b < 0) return;  // uniform over the workgroup
+        read_starts();
         seg.b = x.b;
         seg.at = x.at;
+        seg.start = SHARED ? __builtin_amdgcn_readlane(starts, x.b - lens0) : 0;
         key0 = segment(seg, __builtin_amdgcn_readlane(lens, x.b - lens0));
     } else {
         if (p.fixed) {
@@ -302,7 +314,7 @@ void paged_decode_kernel(PagedAttnParams p) {
             ch.i = (uint32_t)r / (uint32_t)n_seq;
             ch.b = r - ch.i * n_seq;
 #pragma unroll
-            for (int i = 0; i < D; i++) ids[i] = read_ids(ch.b, (ch.i + i) * kStep + kBlock * wave);
+            for (int i = 0; i < D && !SHARED; i++) ids[i] = read_ids(ch.b, (ch.i + i) * kStep + kBlock * wave, 0);
             ch.len = __builtin_amdgcn_readfirstlane(p.c.kv_len[ch.b]);
             ch.keys = kStep;
             ch.n = min(p.fixed, quanta_of<kStep>(p, ch.len));
@@ -314,10 +326,16 @@ void paged_decode_kernel(PagedAttnParams p) {
             ch = find_chunk<kStep>(p, r, lane);
             if (ch.b < 0) return;  // uniform over the workgroup
 #pragma unroll
-            for (int i = 0; i < D; i++) ids[i] = read_ids(ch.b, ch.i * ch.keys + i * kStep + kBlock * wave);
+            for (int i = 0; i < D && !SHARED; i++) ids[i] = read_ids(ch.b, ch.i * ch.keys + i * kStep + kBlock * wave, 0);
         }
         seg.b = ch.b;
         seg.at = 0;
+        seg.start = 0;
+        if constexpr (SHARED) {
+            seg.start = __builtin_amdgcn_readfirstlane(p.x.start[ch.b]);
+#pragma unroll
+            for (int i = 0; i < D; i++) ids[i] = read_ids(ch.b, ch.i * ch.keys + i * kStep + kBlock * wave, seg.start);
+        }
         seg.L = length_ok(p.c, ch.len) ? ch.len : -1;
         key0 = ch.i * ch.keys;
         seg.k1 = ch.i == ch.n - 1 ? max(seg.L, 0) : key0 + ch.keys;
@@ -330,9 +348,10 @@ void paged_decode_kernel(PagedAttnParams p) {
         int last[2];
     };
     bool bad_page = false;  // whether a page of the last block placed is none
-    auto place = [&](int L, int jb, int ids) __attribute__((always_inline)) {
+    auto place = [&](int L, int jb, int ids, int start) __attribute__((always_inline)) {
         Place a;
         bad_page = false;
+        const int from = SHARED ? start & ~15 : 0;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const bool in = jb + 16 * h < L;  // a half behind the last key repeats the half before it
@@ -341,8 +360,8 @@ void paged_decode_kernel(PagedAttnParams p) {
             bad_page |= !ok;
             id = ok ? id : 0;
             const int k16 = jb + (in ? 16 * h : 0);
-            a.base[h] = ES * (head + (int64_t)id * p.c.page_stride + (int64_t)(k16 & page_mask) * p.c.kv_stride);
-            if constexpr (Q8) a.scale[h] = (int64_t)id * p.s.page_stride + (int64_t)g * p.s.head_stride + (k16 & page_mask);
+            a.base[h] = ES * (head + (int64_t)id * p.c.page_stride + (int64_t)((from + k16) & page_mask) * p.c.kv_stride);
+            if constexpr (Q8) a.scale[h] = (int64_t)id * p.s.page_stride + (int64_t)g * p.s.head_stride + ((from + k16) & page_mask);
             a.last[h] = L - 1 - k16;
         }
         return a;
@@ -390,12 +409,12 @@ void paged_decode_kernel(PagedAttnParams p) {
         jseq = ahead.b;
         jb = jb_after;
         if (jseq >= 0) {
-            ids[0] = read_ids(jseq, jb);
-            const int L = ahead.L;
+            ids[0] = read_ids(jseq, jb, ahead.start);
+            const int L = ahead.L, start = ahead.start;
             jb_after += kStep;
             settle();
-            if (ahead.b >= 0) ids_after = read_ids(ahead.b, jb_after);
-            const Place a = place(L, jb, ids[0]);
+            if (ahead.b >= 0) ids_after = read_ids(ahead.b, jb_after, ahead.start);
+            const Place a = place(L, jb, ids[0], start);
             load(p.c.k, p.s.k, a, kr[0]);
             load(p.c.v, p.s.v, a, vr[0]);
         }
@@ -404,11 +423,11 @@ void paged_decode_kernel(PagedAttnParams p) {
         for (int i = 0; i < D; i++) {
             const int key = key0 + kBlock * wave + i * kStep;
             if (key < seg.k1) {
-                const Place a = place(seg.L, key, ids[i]);
+                const Place a = place(seg.L, key, ids[i], seg.start);
                 bad |= bad_page;
                 load(p.c.k, p.s.k, a, kr[i]);
                 load(p.c.v, p.s.v, a, vr[i]);
-                ids[i] = read_ids(seg.b, key + D * kStep);
+                ids[i] = read_ids(seg.b, key + D * kStep, seg.start);
             }
         }
     }
@@ -423,6 +442,9 @@ void paged_decode_kernel(PagedAttnParams p) {
 
     for (;;) {
         const int L = max(seg.L, 0);
+        const int skip = SHARED ? seg.start & 15 : 0;  // keys of the first 16 that the prefix has
+        [[maybe_unused]] int4 pre{};                   // the prefix's partials of the sequence
+        if constexpr (SHARED) pre = p.x.info[seg.b];
         int lim[QT];  // last key that the lane's row sees
 #pragma unroll
         for (int t = 0; t < QT; t++)
@@ -453,7 +475,7 @@ void paged_decode_kernel(PagedAttnParams p) {
             }
             wave_sync();
             // S^T = K Q^T, two tiles of 16 keys: lane holds keys 16 mt + 4 sgrp + v of its row
-            const bool edge = key + kBlock > seg.k1 || (p.causal && key + kBlock > L - n_q + 1);
+            const bool edge = key + kBlock > seg.k1 || (p.causal && key + kBlock > L - n_q + 1) || (SHARED && key < skip);
             float4_t sc[QT][2];
 #pragma unroll
             for (int mt = 0; mt < 2; mt++) {
@@ -475,7 +497,7 @@ void paged_decode_kernel(PagedAttnParams p) {
 #pragma unroll
                     for (int v = 0; v < 4; v++) {
                         const int j = key + 16 * mt + 4 * sgrp + v;
-                        sc[t][mt][v] = !edge || j <= lim[t] ? sc[t][mt][v] * p.scale_log2 : kNegInf;
+                        sc[t][mt][v] = !edge || (j <= lim[t] && (!SHARED || j >= skip)) ? sc[t][mt][v] * p.scale_log2 : kNegInf;
                         bmax = fmaxf(bmax, sc[t][mt][v]);
                     }
                 bmax = xor32_max(xor16_max(bmax));
@@ -522,7 +544,7 @@ void paged_decode_kernel(PagedAttnParams p) {
                 bool odd = false;
 #pragma unroll
                 for (int j = 0; j < NX; j++) {
-                    if (key + piece_row(j) >= L) vx[j] = u32x4{0u, 0u, 0u, 0u};
+                    if (key + piece_row(j) >= L || (SHARED && key + piece_row(j) < skip)) vx[j] = u32x4{0u, 0u, 0u, 0u};
                     odd |= any_nonfinite<T>(vx[j]);
                 }
                 if (p.causal && n_q > 1 && __builtin_amdgcn_ballot_w64(odd)) {
@@ -592,10 +614,10 @@ void paged_decode_kernel(PagedAttnParams p) {
                     key, kr[0], vr[0],
                     [&]() __attribute__((always_inline)) {
                         if (!more) return;
-                        a = place(ahead.L, jb, ids_after);
+                        a = place(ahead.L, jb, ids_after, ahead.start);
                         jb_after += kStep;
                         settle();
-                        if (ahead.b >= 0) ids_after = read_ids(ahead.b, jb_after);
+                        if (ahead.b >= 0) ids_after = read_ids(ahead.b, jb_after, ahead.start);
                         __builtin_amdgcn_sched_barrier(0);
                         load(p.c.k, p.s.k, a, kr[0]);
                     },
@@ -614,9 +636,9 @@ void paged_decode_kernel(PagedAttnParams p) {
                         key, kr[i], vr[i],
                         [&]() __attribute__((always_inline)) {
                             if (next >= seg.k1) return;
-                            a = place(seg.L, next, ids[i]);
+                            a = place(seg.L, next, ids[i], seg.start);
                             bad |= bad_page;
-                            ids[i] = read_ids(seg.b, next + D * kStep);
+                            ids[i] = read_ids(seg.b, next + D * kStep, seg.start);
                             __builtin_amdgcn_sched_barrier(0);
                             load(p.c.k, p.s.k, a, kr[i]);
                         },
@@ -652,7 +674,37 @@ void paged_decode_kernel(PagedAttnParams p) {
             const int rr = rt * RT + i;
             if (rr >= p.rows) return;
             const int t = rr / G, h = g * G + rr % G;
-            const bool empty = p.causal ? L - n_q + t < 0 : L == 0;  // no key: zeros (a length that is none: NaN)
+            if constexpr (SHARED) {
+                // the prefix's parts, a few in flight, each at its maximum
+                constexpr int AT_ONCE = 8;
+                const int64_t row = pre.w + rr, rows = pre.y;
+                for (int k0 = 0; k0 < pre.z; k0 += AT_ONCE) {
+                    float4_t w[AT_ONCE];
+                    float2 ml[AT_ONCE];
+                    float top = M;
+#pragma unroll
+                    for (int e = 0; e < AT_ONCE; e++) {
+                        const int64_t first = (int64_t)g * *p.x.rows + pre.x + (int64_t)min(k0 + e, pre.z - 1) * rows;
+                        const float * x = p.x.part + first * (HD + 4);
+                        w[e] = *reinterpret_cast<const float4_t *>(x + (d / 4 * rows + row) * 4);
+                        ml[e] = *reinterpret_cast<const float2 *>(x + HD * rows + 2 * row);
+                    }
+#pragma unroll
+                    for (int e = 0; e < AT_ONCE; e++) top = fmaxf(top, ml[e].x);
+                    const float use = top == kNegInf ? 0.f : top, corr = exp2_fast(M - use);
+                    a *= corr;
+                    tot *= corr;
+#pragma unroll
+                    for (int e = 0; e < AT_ONCE; e++) {
+                        if (k0 + e >= pre.z) break;
+                        const float y = exp2_fast(ml[e].x - use);
+                        a += w[e] * y;
+                        tot += ml[e].y * y;
+                    }
+                    M = top;
+                }
+            }
+            const bool empty = !(SHARED && pre.z > 0) && (p.causal ? L - n_q + t < 0 : L == 0);  // no key: zeros (a length that is none: NaN)
             const float inv = 1.f / tot;
             float4_t w = empty ? float4_t{0.f, 0.f, 0.f, 0.f} : a * inv;
             if (bad_len) w = float4_t{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
@@ -806,30 +858,34 @@ void paged_decode_kernel(PagedAttnParams p) {
     }
 }
 
-template <int HD, class T, int NW, bool RANGES, bool Q8>
+template <int HD, class T, int NW, bool RANGES, bool Q8, bool SHARED>
 void launch_rt(const PagedAttnParams & p, int rt, hipStream_t stream) {
     const int64_t groups = (int64_t)p.ranges * p.n_head_kv;
     const dim3 grid((uint32_t)(p.n_rowtiles == 1 ? groups : (groups + 7) / 8 * 8 * p.n_rowtiles)), block(NW * kWave);
-    if (rt == 4) hipLaunchKernelGGL((paged_decode_kernel<HD, 4, T, NW, RANGES, Q8>), grid, block, 0, stream, p);
-    else if (rt == 8) hipLaunchKernelGGL((paged_decode_kernel<HD, 8, T, NW, RANGES, Q8>), grid, block, 0, stream, p);
-    else if (rt == 16) hipLaunchKernelGGL((paged_decode_kernel<HD, 16, T, NW, RANGES, Q8>), grid, block, 0, stream, p);
-    else if constexpr (HD != 256) hipLaunchKernelGGL((paged_decode_kernel<HD, 32, T, NW, RANGES, Q8>), grid, block, 0, stream, p);
+    if (rt == 4) hipLaunchKernelGGL((paged_decode_kernel<HD, 4, T, NW, RANGES, Q8, SHARED>), grid, block, 0, stream, p);
+    else if (rt == 8) hipLaunchKernelGGL((paged_decode_kernel<HD, 8, T, NW, RANGES, Q8, SHARED>), grid, block, 0, stream, p);
+    else if (rt == 16) hipLaunchKernelGGL((paged_decode_kernel<HD, 16, T, NW, RANGES, Q8, SHARED>), grid, block, 0, stream, p);
+    else if constexpr (HD != 256) hipLaunchKernelGGL((paged_decode_kernel<HD, 32, T, NW, RANGES, Q8, SHARED>), grid, block, 0, stream, p);
 }
 
-template <class T, bool Q8>
-void launch_hd(const PagedAttnParams & p, int head_dim, int rt, int waves, hipStream_t stream) {
-    if (head_dim == 256) {
-        if (p.by_ranges) launch_rt<256, T, 4, true, Q8>(p, rt, stream);
-        else launch_rt<256, T, 4, false, Q8>(p, rt, stream);
-    } else if (head_dim == 64) {
-        if (p.by_ranges) launch_rt<64, T, 4, true, Q8>(p, rt, stream);
-        else if (waves == 8) launch_rt<64, T, 8, false, Q8>(p, rt, stream);
-        else launch_rt<64, T, 4, false, Q8>(p, rt, stream);
-    } else {
-        if (p.by_ranges) launch_rt<128, T, 4, true, Q8>(p, rt, stream);
-        else if (waves == 8) launch_rt<128, T, 8, false, Q8>(p, rt, stream);
-        else launch_rt<128, T, 4, false, Q8>(p, rt, stream);
+// SHARED runs 4 waves: what sequences have of their own is seldom long.
+template <int HD, class T, bool Q8, bool SHARED>
+void launch_waves(const PagedAttnParams & p, int rt, int waves, hipStream_t stream) {
+    if constexpr (HD != 256 && !SHARED) {
+        if (!p.by_ranges && waves == 8) {
+            launch_rt<HD, T, 8, false, Q8, SHARED>(p, rt, stream);
+            return;
+        }
     }
+    if (p.by_ranges) launch_rt<HD, T, 4, true, Q8, SHARED>(p, rt, stream);
+    else launch_rt<HD, T, 4, false, Q8, SHARED>(p, rt, stream);
+}
+
+template <class T, bool Q8, bool SHARED>
+void launch_hd(const PagedAttnParams & p, int head_dim, int rt, int waves, hipStream_t stream) {
+    if (head_dim == 256) launch_waves<256, T, Q8, SHARED>(p, rt, waves, stream);
+    else if (head_dim == 64) launch_waves<64, T, Q8, SHARED>(p, rt, waves, stream);
+    else launch_waves<128, T, Q8, SHARED>(p, rt, waves, stream);
 }
 
 }  // namespace

@@ -175,9 +175,158 @@ __device__ __forceinline__ bool odd_values(const PagedAttnParams & p, const Tile
     return __builtin_amdgcn_ballot_w64(odd) != 0;
 }
 
+// ---- shared prefixes: the rows of a group's sequences are one tile list over the keys they share ----
+
+// Rows of R a tile: the tile, and the part of its keys, that workgroup o of the launch computes (b -1: none), with the group's row of
+// the page table in t.b and its first query row in t.row0. Every part takes the same count of steps, the least for which the chip
+// holds all parts of the launch at once, and no fewer than a tile has waves with rows: with fewer, writing the partial and
+// reading it back costs more than the shorter walk saves. The waves of the last workgroups also write what the kernel behind this
+// one needs to know of each sequence.
+template <int R, int W>
+__device__ __forceinline__ Tile plan_prefix(const PagedAttnParams & p, int wave, PagedPrefixPart & part) {
+    const PagedPrefix & x = p.x;
+    const int lane = threadIdx.x % kWave, n_seq = p.c.n_seq, per_seq = p.n_q * p.group;
+    struct Group {
+        int s0, n, keys, rows, steps, tiles, least;  // rows 0: nothing is shared
+    };
+    auto clamp = [&](int s) { return min(max(s, 0), n_seq); };
+    auto group_at = [&](int base) {
+        Group r;
+        const int i = min(base + lane, x.n_groups - 1);
+        r.s0 = clamp(x.cu_seq[i]);
+        r.n = base + lane < x.n_groups ? max(clamp(x.cu_seq[i + 1]) - r.s0, 0) : 0;
+        r.keys = x.prefix_len[i];
+        const bool shared = r.n > 1 && r.keys > 0 && r.keys <= p.c.capacity;
+        r.rows = shared ? r.n * per_seq : 0;
+        r.steps = shared ? (r.keys + kBK - 1) / kBK : 0;
+        r.tiles = (r.rows + R - 1) / R;
+        r.least = min(W, (r.rows + 31) / 32);
+        return r;
+    };
+    const Group first = group_at(0);
+    auto at = [&](int base) { return base == 0 ? first : group_at(base); };
+    auto parts = [&](const Group & r, int c) { return r.rows ? (r.steps + max(c, r.least) - 1) / max(c, r.least) : 0; };
+    float sum = 0.f;
+    int longest = 1;
+    for (int base = 0; base < x.n_groups; base += kWave) {
+        const Group r = at(base);
+        sum += (float)r.tiles * (float)r.steps;
+        longest = max(longest, r.steps);
+    }
+    longest = wave_imax(longest);
+    sum = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_sum(sum))));
+    const int room = max(1, p.ranges / p.n_head_kv);
+    auto count = [&](int c) {  // parts of a kv head, at most 2^30
+        int r = 0;
+        for (int base = 0; base < x.n_groups; base += kWave) {
+            const Group y = at(base);
+            r = min(r + wave_isum((int)min((int64_t)y.tiles * parts(y, c), (int64_t)1 << 23)), 1 << 29);
+        }
+        return r;
+    };
+    int c = __builtin_amdgcn_readfirstlane((int)fminf(ceilf(sum / (float)room), (float)longest));
+    c = max(c, (longest + kPagedMaxParts - 1) / kPagedMaxParts);
+    for (int i = 0; c < longest && count(c) > room; i++) c = i < 16 ? min(c + max(1, c / 8), longest) : longest;
+    const int per_kv = count(c);
+    int64_t rows = 0;  // of the partials of a kv head
+    for (int base = 0; base < x.n_groups; base += kWave) {
+        const Group r = at(base);
+        rows += read_lane64(wave_scan64((int64_t)r.rows * parts(r, c)), 63);
+    }
+    // only ranges of cu_seq that overlap have more parts or rows than the launch
+    const int64_t all = (int64_t)per_kv * p.n_head_kv;
+    const bool fits = all <= (int64_t)gridDim.x && rows * p.n_head_kv <= x.max_rows;
+
+    // ---- the sequences: where their own keys start, how many they are, and where the partials lie ----
+    if (blockIdx.x == 0 && threadIdx.x == 0) *x.rows = fits ? (int32_t)rows : 0;
+    for (int64_t b0 = ((int64_t)(gridDim.x - 1 - blockIdx.x) * W + wave) * kWave; b0 < n_seq; b0 += (int64_t)gridDim.x * W * kWave) {
+        const int b = min((int)b0 + lane, n_seq - 1);
+        int g = 0, end = x.n_groups;  // the last group that does not start behind b
+        while (__builtin_amdgcn_ballot_w64(end - g > 1)) {
+            const int mid = (g + end) / 2;
+            if (end - g > 1) {
+                if (x.cu_seq[mid] <= b) g = mid;
+                else end = mid;
+            }
+        }
+        const int s0 = clamp(x.cu_seq[g]), s1 = clamp(x.cu_seq[g + 1]), len = p.c.kv_len[b];
+        const bool in = s0 <= b && b < s1;
+        const int keys = in ? x.prefix_len[g] : 0;
+        const bool shared = in && s1 - s0 > 1 && keys > 0 && keys <= p.c.capacity;
+        int start = 0, own = len, np = 0, group_rows = 0;
+        int64_t first_row = 0;
+        for (int base = 0; base < x.n_groups; base += kWave) {
+            const Group r = at(base);
+            const int n = parts(r, c);
+            const int64_t mine = (int64_t)r.rows * n, upto = wave_scan64(mine) - mine;
+            const int from = (g - base) & (kWave - 1);
+            const int lo = __builtin_amdgcn_ds_bpermute(4 * from, (int32_t)upto), n_of = __builtin_amdgcn_ds_bpermute(4 * from, n);
+            const int rows_of = __builtin_amdgcn_ds_bpermute(4 * from, r.rows);
+            const int last = __builtin_amdgcn_readlane((int32_t)(upto + mine), 63);
+            if (g - base >= 0 && g - base < kWave) {
+                first_row += (uint32_t)lo;
+                np = n_of;
+                group_rows = rows_of;
+            } else if (g >= base + kWave) {
+                first_row += (uint32_t)last;
+            }
+        }
+        if (shared && len != 0) {
+            // a row has to see the keys of the prefix, every one
+            const bool ok = fits && length_ok(p.c, len) && len >= keys + (p.causal ? p.n_q - 1 : 0);
+            start = ok ? keys : 0;
+            own = ok ? len - (keys & ~15) : -1;
+            if (!ok) np = 0;
+        } else {
+            np = 0;
+            if (in && (keys < 0 || keys > p.c.capacity) && len != 0) own = -1;
+        }
+        if ((int)b0 + lane < n_seq) {
+            x.own_len[b] = own;
+            x.start[b] = start;
+            x.info[b] = make_int4((int)first_row, group_rows, np, (b - s0) * per_seq);
+        }
+    }
+
+    // ---- the workgroup's part: by kv head, group, keys, then tiles, neighbours on one XCD ----
+    Tile t{};
+    t.b = -1;
+    if (!fits || blockIdx.x >= (uint32_t)all) return t;
+    int o = (int)xcd_remap(blockIdx.x, (uint32_t)all);
+    t.kvh = o / per_kv;
+    o -= t.kvh * per_kv;
+    int64_t before = 0;
+    for (int base = 0; base < x.n_groups; base += kWave) {
+        const Group r = at(base);
+        const int n = parts(r, c), mine = r.tiles * n, upto = wave_iscan(mine);
+        const int64_t of_rows = wave_scan64((int64_t)r.rows * n);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(upto > o);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            o -= __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l);
+            const int tiles = __builtin_amdgcn_readlane(r.tiles, l), k = o / tiles, each = max(c, __builtin_amdgcn_readlane(r.least, l));
+            t.b = __builtin_amdgcn_readlane(r.s0, l);
+            t.row0 = t.b * p.n_q;
+            t.n = __builtin_amdgcn_readlane(r.rows, l);
+            t.len = __builtin_amdgcn_readlane(r.keys, l);
+            t.i = o - k * tiles;
+            t.steps = __builtin_amdgcn_readlane(r.steps, l);
+            t.s0 = k * each;
+            t.s1 = min(t.s0 + each, t.steps);
+            part.rows = t.n;
+            part.first = t.kvh * rows + before + read_lane64(of_rows, l) - (int64_t)t.n * __builtin_amdgcn_readlane(n, l) + (int64_t)k * t.n;
+            return t;
+        }
+        o -= __builtin_amdgcn_readlane(upto, 63);
+        before += read_lane64(of_rows, 63);
+    }
+    return t;
+}
+
 // HD: head_dim. T: type of query rows and pages. W: waves. HPW: query heads of a group that a workgroup takes, W / HPW row tiles of
-// each. Q8: the pages hold e4m3 codes with a scale a row, expanded to T in LDS.
-template <int HD, class T, int W, int HPW, bool Q8>
+// each. Q8: the pages hold e4m3 codes with a scale a row, expanded to T in LDS. PREFIX: the keys that groups of sequences share, for all
+// rows of a group; a row is one of a query head then, and a workgroup computes one part of a tile and leaves it to the next kernel.
+template <int HD, class T, int W, int HPW, bool Q8, bool PREFIX>
 __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(HD <= 128 ? 2 : 1, HD <= 128 ? 2 : 1)))
 void paged_prefill_kernel(PagedAttnParams p) {
     constexpr int RPW = W / HPW, R = 32 * RPW;  // row tiles of a head, and rows
@@ -197,7 +346,8 @@ void paged_prefill_kernel(PagedAttnParams p) {
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x % kWave;
-    const int n_seq = p.c.n_seq, sets = (p.group + HPW - 1) / HPW;
+    const int n_seq = p.c.n_seq, sets = PREFIX ? 1 : (p.group + HPW - 1) / HPW;
+    [[maybe_unused]] PagedPrefixPart prefix_part;
 
     // ---- the sequences, 64 in lanes: rows lo .. lo + n - 1, kv_len ----
     int lo = 0, nq = 0, len = 0, first_seq = -1;
@@ -222,7 +372,7 @@ void paged_prefill_kernel(PagedAttnParams p) {
     // ---- the workgroup's range of units, or its tile ----
     int tiles = 0, longest = 0;  // of one kv head and set
     int64_t units = 0;
-    for (int base = 0; base < n_seq; base += kWave) {
+    for (int base = 0; !PREFIX && base < n_seq; base += kWave) {
         read(base);
         const Rows<R> s = rows_of(nq, len);
         // more than p.max_tiles only where ranges of cu_q overlap
@@ -231,13 +381,16 @@ void paged_prefill_kernel(PagedAttnParams p) {
         longest = max(longest, wave_imax(s.n ? s.steps(s.nt - 1) : 0));
     }
     const int all = tiles * sets * p.n_head_kv;
-    const bool direct = all <= p.ranges && longest <= kDirectSteps;
+    const bool direct = PREFIX || (all <= p.ranges && longest <= kDirectSteps);
     const int64_t per_kv = units * sets, total = per_kv * p.n_head_kv;
     Tile t{};
     t.b = -1;
     int64_t hi_unit = 0, share = 1;
     int range = 0;
-    if (direct) {
+    if constexpr (PREFIX) {
+        t = plan_prefix<R, W>(p, wave, prefix_part);
+        if (t.b < 0) return;
+    } else if (direct) {
         if (blockIdx.x >= (uint32_t)all) return;
         int o = (int)xcd_remap(blockIdx.x, (uint32_t)all);
         t.kvh = o / (tiles * sets);
@@ -512,10 +665,11 @@ void paged_prefill_kernel(PagedAttnParams p) {
     const int l32 = lane % 32, hgrp = lane / 32;
     const int rt = wave % RPW;
     u32x4 qb[KS];  // lane holds Q[row][16 ks + 8 hgrp .. + 8]; rows past the sequence's read its last one, zeroed before use
-    auto head_of = [&](const Tile & t) { return t.kvh * p.group + min(t.set * HPW + wave / RPW, p.group - 1); };
+    auto head_of = [&](const Tile & t) { return PREFIX ? t.kvh * p.group : t.kvh * p.group + min(t.set * HPW + wave / RPW, p.group - 1); };
     auto load_q = [&](const Tile & t) __attribute__((always_inline)) {
         const int row = min(t.i * R + 32 * rt + l32, t.n - 1);
-        const uint16_t * qr = p.q + (int64_t)(t.row0 + row) * p.q_stride + (int64_t)head_of(t) * HD + 8 * hgrp;
+        const int tok = PREFIX ? row / p.group : row, h = PREFIX ? row - tok * p.group : 0;
+        const uint16_t * qr = p.q + (int64_t)(t.row0 + tok) * p.q_stride + (int64_t)(head_of(t) + h) * HD + 8 * hgrp;
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) qb[ks] = load16(qr + 16 * ks);
     };
@@ -537,9 +691,10 @@ void paged_prefill_kernel(PagedAttnParams p) {
         const int off = L - t.n;                           // key that row 0 sits at (below 0: rows without one)
         const int first_row = t.i * R + 32 * rt, row = first_row + l32;  // among the sequence's
         const int h = head_of(t);
-        const bool idle = t.set * HPW + wave / RPW >= p.group || first_row >= t.n;  // heads past the group, rows past the end
-        const int wave_end = idle ? 0 : p.causal ? off + min(first_row + 32, t.n) : L;  // keys that this wave's rows see at most
-        const int lim = p.causal ? min(off + row, L - 1) : L - 1;  // last key the row sees
+        const bool idle = (!PREFIX && t.set * HPW + wave / RPW >= p.group) || first_row >= t.n;  // heads past the group, rows past the end
+        const bool causal = !PREFIX && p.causal;
+        const int wave_end = idle ? 0 : causal ? off + min(first_row + 32, t.n) : L;  // keys that this wave's rows see at most
+        const int lim = causal ? min(off + row, L - 1) : L - 1;  // last key the row sees
         // the first tile's steps, and what the tiles behind were too short for (the buffer read last is not among those filled)
         if (sent < AHEAD) {
             while (sent < AHEAD && more()) {
@@ -633,7 +788,7 @@ void paged_prefill_kernel(PagedAttnParams p) {
             };
             static_for<0, VA>(vread);
             // the mask only where a block crosses the diagonal or the end (wave-uniform)
-            if (p.causal ? kb + kBK - 1 > off + first_row : kb + kBK > L) {
+            if (causal ? kb + kBK - 1 > off + first_row : kb + kBK > L) {
 #pragma unroll
                 for (int mt = 0; mt < 2; mt++)
 #pragma unroll
@@ -714,6 +869,21 @@ void paged_prefill_kernel(PagedAttnParams p) {
             });
         }
 
+        if constexpr (PREFIX) {
+            // ---- the partial of this part: O in quads [HD / 4][rows], so that lanes of neighbouring rows store side by side, then (m, l) ----
+            const float l = __builtin_amdgcn_ballot_w64(bad != 0) ? __builtin_nanf("") : xor32_add(l_run);
+            if (row < t.n) {
+                float * d = p.x.part + prefix_part.first * (HD + 4);
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                    for (int gq = 0; gq < 4; gq++)
+                        *reinterpret_cast<float4_t *>(d + ((int64_t)(8 * dt + 2 * gq + hgrp) * prefix_part.rows + row) * 4) =
+                            float4_t{o[dt][4 * gq], o[dt][4 * gq + 1], o[dt][4 * gq + 2], o[dt][4 * gq + 3]};
+                if (hgrp == 0) *reinterpret_cast<float2 *>(d + (int64_t)HD * prefix_part.rows + 2 * row) = make_float2(m_run, l);
+            }
+            return;
+        }
         // ---- the tile (or this part of it) is done: the next one's query goes out ----
         const Tile done = t;
         const bool poison = bad_len || __builtin_amdgcn_ballot_w64(bad != 0) != 0;
@@ -870,7 +1040,7 @@ void paged_prefill_kernel(PagedAttnParams p) {
 
 template <int HD, class T, int W, int HPW, bool Q8>
 void launch_shape(const PagedAttnParams & p, hipStream_t stream) {
-    hipLaunchKernelGGL((paged_prefill_kernel<HD, T, W, HPW, Q8>), dim3((uint32_t)p.ranges), dim3(W * kWave), 0, stream, p);
+    hipLaunchKernelGGL((paged_prefill_kernel<HD, T, W, HPW, Q8, false>), dim3((uint32_t)p.ranges), dim3(W * kWave), 0, stream, p);
 }
 
 // The shapes that the plans take: 8 waves at head dim 128 only, several heads with 8 waves only.
@@ -892,6 +1062,14 @@ void launch_hd(const PagedAttnParams & p, int head_dim, const PagedPrefillPlan &
     if (head_dim == 64) launch_plan<64, T, Q8>(p, plan, stream);
     else if (head_dim == 128) launch_plan<128, T, Q8>(p, plan, stream);
     else launch_plan<256, T, Q8>(p, plan, stream);
+}
+
+template <class T, bool Q8>
+void launch_prefix(const PagedAttnParams & p, int head_dim, uint32_t grid, hipStream_t stream) {
+    const dim3 block(kPagedPrefixWaves * kWave);
+    if (head_dim == 64) hipLaunchKernelGGL((paged_prefill_kernel<64, T, kPagedPrefixWaves, 1, Q8, true>), dim3(grid), block, 0, stream, p);
+    else if (head_dim == 128) hipLaunchKernelGGL((paged_prefill_kernel<128, T, kPagedPrefixWaves, 1, Q8, true>), dim3(grid), block, 0, stream, p);
+    else hipLaunchKernelGGL((paged_prefill_kernel<256, T, kPagedPrefixWaves, 1, Q8, true>), dim3(grid), block, 0, stream, p);
 }
 
 }  // namespace

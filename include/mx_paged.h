@@ -2,7 +2,8 @@
  * mx_paged.h — C ABI of the paged key/value cache: keys and values of many sequences in fixed-size pages of one pool,
  * lengths and page tables in device memory, so that a step captured in a HIP graph replays while its sequences grow.
  * Three calls serve a decoder's layer: mx_paged_store writes a step's new keys and values, mx_paged_decode attends a few
- * new rows of each sequence, mx_paged_prefill attends packed prompts.
+ * new rows of each sequence, mx_paged_prefill attends packed prompts. Each has a form for pages in 8 bits, and the decode one for
+ * sequences that share their first keys.
  *
  * The reference has no paged cache: it keeps one contiguous cache per sequence (metal_llama_decoder.mm:664), which
  * mx_attn.h serves. The arithmetic is that of rope_store (src/backend/metal/llama_kernels.h:520-545) and of the attention
@@ -156,6 +157,46 @@ MX_ATTN_API int32_t mx_paged_decode_e4m3(const mx_paged_desc * desc, const mx_pa
 /* Workspace bytes mx_paged_decode needs for desc (the strides and pools do not matter). 0 and the last error set for an
  * invalid descriptor. */
 MX_ATTN_API size_t mx_paged_decode_workspace_bytes(const mx_paged_desc * desc);
+
+/*
+ * Sequences whose first keys are the same: a batch of answers to one prompt, of users behind one system prompt, of questions about one
+ * document. The sequences come in n_groups groups, one behind the other, each with a prefix that its sequences share; sequences
+ * that no group has share nothing.
+ */
+typedef struct mx_paged_prefix {
+    int32_t n_groups;           /* 0 .. n_seq (0: nothing is shared) */
+    int32_t reserved;           /* must be 0 */
+    const int32_t * cu_seq;     /* device, [n_groups + 1]: sequences cu_seq[g] .. cu_seq[g + 1] - 1 are group g's; ascending */
+    const int32_t * prefix_len; /* device, [n_groups]: the keys that the sequences of a group have in common, from key 0 on; any
+                                   number of them, whole pages or not */
+} mx_paged_prefix;
+
+/*
+ * mx_paged_decode of sequences that share prefixes: the results of mx_paged_decode within its rounding, while each shared key is read
+ * once for all rows of its group instead of once a sequence. Two launches: the prefixes, for all query rows of a group on the matrix
+ * cores together, then each sequence's own keys, with which the prefix's partials are joined.
+ *
+ * The keys of a prefix are found through the page table of its group's first sequence; the other sequences' entries for whole
+ * pages of it are not read, and rows of it in a page that holds keys of a sequence's own (where the prefix ends within a page) are
+ * never used. kv_len counts the prefix's keys too. Every row has to see the whole prefix: a sequence with fewer keys than the
+ * prefix (causal: than the prefix and all but one of its new rows), but not 0, or with a prefix_len outside
+ * [0, max_pages * page_size], gets NaN; one of 0 keys gets zeros, and takes nothing from its group. cu_seq entries are clamped to
+ * [0, n_seq]; what ranges that run backwards or overlap compute is undefined.
+ *
+ *   scales      of pages in 8 bits, or NULL: pages of dtype
+ *   workspace   as mx_paged_decode's, at least mx_paged_decode_shared_workspace_bytes(desc, n_groups) bytes, never NULL where there
+ *               is work to do. Nothing is kept in it between calls.
+ *
+ * desc->max_kv_len counts the keys of a sequence behind its prefix here (0: unknown). n_rows * n_head at most 2^26.
+ */
+MX_ATTN_API int32_t mx_paged_decode_shared(const mx_paged_desc * desc, const mx_paged_scales * scales, const mx_paged_prefix * prefix,
+                                           const void * q, const void * k, const void * v, const int32_t * table,
+                                           const int32_t * kv_len, void * out, float * lse, void * workspace, size_t ws_bytes,
+                                           mx_attn_stream stream);
+
+/* Workspace bytes mx_paged_decode_shared needs for desc and so many groups, or fewer; 0 and the last error set for an invalid
+ * descriptor. */
+MX_ATTN_API size_t mx_paged_decode_shared_workspace_bytes(const mx_paged_desc * desc, int32_t n_groups);
 
 /*
  * Attention of packed prompts: rows cu_q[b] .. cu_q[b + 1] - 1 are the last rows of sequence b, whose pages hold its keys

@@ -128,10 +128,11 @@ def test_front_end_refusals(monkeypatch):
 
 def test_other_extensions_are_refused(monkeypatch):
     from dooms_amd import _native as ext
-    version, size = _lib.lib().mx_attn_abi_version(), ctypes.sizeof(_lib.MxPagedScales)
-    for v, s in ((version + 1, size), (version, size + 8)):
+    version = _lib.lib().mx_attn_abi_version()
+    sizes = ctypes.sizeof(_lib.MxPagedScales), ctypes.sizeof(_lib.MxPagedPrefix)
+    for v, s in ((version + 1, sizes), (version, (sizes[0] + 8, sizes[1])), (version, (sizes[0], sizes[1] + 8))):
         with pytest.raises(ImportError, match="dooms_amd.build"):
-            ext.bind_paged_e4m3(v, s, 0, 0, 0)
+            ext.bind_paged_more(v, s, 0, 0, 0, 0)
     old = types.SimpleNamespace(bind=lambda *a: None, bind_paged=lambda *a: None)
     monkeypatch.setattr(A, "_bound", None)
     monkeypatch.setattr(A, "_ext", None)

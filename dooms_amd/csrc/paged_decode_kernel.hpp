@@ -192,7 +192,7 @@ __device__ __forceinline__ u32x4 load_kv(const char * a) {
 // already (PagedPrefix): positions count from the multiple of 16 at or below the first other key, and the prefix's partials are joined
 // in behind the sequence's own.
 template <int HD, int RT, class T, int NW, bool RANGES, bool Q8, bool SHARED>
-__global__ __launch_bounds__(NW * kWave) __attribute__((amdgpu_waves_per_eu(HD == 256 || RANGES ? 1 : 2)))
+__global__ __launch_bounds__(NW * kWave) __attribute__((amdgpu_waves_per_eu(HD == 256 || (RANGES && !(Q8 && RT <= 16)) ? 1 : 2)))
 void paged_decode_kernel(PagedAttnParams p) {
     constexpr int QT = RT > 16 ? 2 : 1;  // 16-row product tiles
     constexpr int KS = HD / 32;          // product steps along head_dim

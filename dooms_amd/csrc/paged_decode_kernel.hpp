@@ -192,7 +192,7 @@ __device__ __forceinline__ u32x4 load_kv(const char * a) {
 // already (PagedPrefix): positions count from the multiple of 16 at or below the first other key, and the prefix's partials are joined
 // in behind the sequence's own.
 template <int HD, int RT, class T, int NW, bool RANGES, bool Q8, bool SHARED>
-__global__ __launch_bounds__(NW * kWave) __attribute__((amdgpu_waves_per_eu(HD == 256 || (RANGES && !(Q8 && RT <= 16)) ? 1 : 2)))
+__global__ __launch_bounds__(NW * kWave) __attribute__((amdgpu_waves_per_eu(HD == 256 || (RANGES && !((Q8 || SHARED) && RT <= 16)) ? 1 : 2)))
 void paged_decode_kernel(PagedAttnParams p) {
     constexpr int QT = RT > 16 ? 2 : 1;  // 16-row product tiles
     constexpr int KS = HD / 32;          // product steps along head_dim
@@ -216,6 +216,7 @@ void paged_decode_kernel(PagedAttnParams p) {
                          : RANGES || HD == 256 || (HD == 128 && RT == 32) ? 1 : HD == 64 && RT <= 16 ? 3 : 2;
     constexpr int SS = RT * PR;
     constexpr int NQ = RT * HD / 4;      // output quads of the tile
+    constexpr int CQ = (NQ + kThreads - 1) / kThreads;  // of those a thread has
     constexpr int kLds = kBlock * VP * 2 > RT * HD * 4 ? kBlock * VP * 2 : RT * HD * 4;  // bytes of a wave: block, then outputs
     static_assert(16 % KPL == 0, "a load's rows lie in one page");
     __shared__ __attribute__((aligned(16))) char s_buf[NW][kLds];
@@ -432,6 +433,57 @@ void paged_decode_kernel(PagedAttnParams p) {
         }
     }
 
+    // SHARED: the prefix's part of the thread's quads, which the sequence's first part has beside its own keys: a few partials in flight,
+    // each at its maximum, fetched while the first of those are in flight.
+    [[maybe_unused]] int4 pre{};  // the prefix's partials of the sequence
+    [[maybe_unused]] float pre_m[CQ], pre_l[CQ];
+    [[maybe_unused]] float4_t pre_o[CQ];
+    auto fold_prefix = [&](int parts) __attribute__((always_inline)) {
+        if constexpr (SHARED) {
+            constexpr int AT_ONCE = CQ == 1 ? 8 : CQ == 2 ? 4 : 2;
+#pragma unroll
+            for (int c = 0; c < CQ; c++) {
+                pre_m[c] = kNegInf;
+                pre_l[c] = 0.f;
+                pre_o[c] = float4_t{0.f, 0.f, 0.f, 0.f};
+            }
+            const int64_t rows = pre.y, first = (int64_t)g * *p.x.rows + pre.x;
+            for (int k0 = 0; k0 < parts; k0 += AT_ONCE) {
+                float4_t w[CQ][AT_ONCE];
+                float2 ml[CQ][AT_ONCE];
+#pragma unroll
+                for (int c = 0; c < CQ; c++) {
+                    const int i = min((int)threadIdx.x + c * kThreads, NQ - 1), d4 = i % (HD / 4);
+                    const int64_t row = pre.w + min(rt * RT + i / (HD / 4), p.rows - 1);
+#pragma unroll
+                    for (int e = 0; e < AT_ONCE; e++) {
+                        const float * x = p.x.part + (first + min(k0 + e, parts - 1) * rows) * (HD + 4);
+                        w[c][e] = *reinterpret_cast<const float4_t *>(x + (d4 * rows + row) * 4);
+                        ml[c][e] = *reinterpret_cast<const float2 *>(x + HD * rows + 2 * row);
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < CQ; c++) {
+                    float top = pre_m[c];
+#pragma unroll
+                    for (int e = 0; e < AT_ONCE; e++) top = fmaxf(top, ml[c][e].x);
+                    const float use = top == kNegInf ? 0.f : top, corr = exp2_fast(pre_m[c] - use);
+                    pre_o[c] *= corr;
+                    pre_l[c] *= corr;
+                    pre_m[c] = top;
+#pragma unroll
+                    for (int e = 0; e < AT_ONCE; e++) {
+                        if (k0 + e >= parts) break;
+                        const float y = exp2_fast(ml[c][e].x - use);
+                        pre_o[c] += w[c][e] * y;
+                        pre_l[c] += ml[c][e].y * y;
+                    }
+                }
+            }
+        }
+    };
+    if constexpr (SHARED) pre = p.x.info[seg.b];
+
     uint16_t * vw = reinterpret_cast<uint16_t *>(s_buf[wave]);
     const int v_rd = (4 * sgrp + (lane % 16) / 4) * VP + 4 * (lane % 4);
     auto wave_sync = [&]() {
@@ -443,8 +495,8 @@ void paged_decode_kernel(PagedAttnParams p) {
     for (;;) {
         const int L = max(seg.L, 0);
         const int skip = SHARED ? seg.start & 15 : 0;  // keys of the first 16 that the prefix has
-        [[maybe_unused]] int4 pre{};                   // the prefix's partials of the sequence
-        if constexpr (SHARED) pre = p.x.info[seg.b];
+        const int pre_parts = SHARED ? pre.z : 0;
+        if constexpr (SHARED) fold_prefix((RANGES ? seg.at >= x.lo : ch.i == 0) ? pre.z : 0);
         int lim[QT];  // last key that the lane's row sees
 #pragma unroll
         for (int t = 0; t < QT; t++)
@@ -651,6 +703,7 @@ void paged_decode_kernel(PagedAttnParams p) {
         const Seg done = seg;
         next_segment(seg);
         if (seg.b >= 0) load_q(seg.b);  // in flight over what follows
+        if (SHARED && seg.b >= 0) pre = p.x.info[seg.b];
 
         // ---- join the waves; write the output, or publish this part ----
 #pragma unroll
@@ -674,37 +727,7 @@ void paged_decode_kernel(PagedAttnParams p) {
             const int rr = rt * RT + i;
             if (rr >= p.rows) return;
             const int t = rr / G, h = g * G + rr % G;
-            if constexpr (SHARED) {
-                // the prefix's parts, a few in flight, each at its maximum
-                constexpr int AT_ONCE = 8;
-                const int64_t row = pre.w + rr, rows = pre.y;
-                for (int k0 = 0; k0 < pre.z; k0 += AT_ONCE) {
-                    float4_t w[AT_ONCE];
-                    float2 ml[AT_ONCE];
-                    float top = M;
-#pragma unroll
-                    for (int e = 0; e < AT_ONCE; e++) {
-                        const int64_t first = (int64_t)g * *p.x.rows + pre.x + (int64_t)min(k0 + e, pre.z - 1) * rows;
-                        const float * x = p.x.part + first * (HD + 4);
-                        w[e] = *reinterpret_cast<const float4_t *>(x + (d / 4 * rows + row) * 4);
-                        ml[e] = *reinterpret_cast<const float2 *>(x + HD * rows + 2 * row);
-                    }
-#pragma unroll
-                    for (int e = 0; e < AT_ONCE; e++) top = fmaxf(top, ml[e].x);
-                    const float use = top == kNegInf ? 0.f : top, corr = exp2_fast(M - use);
-                    a *= corr;
-                    tot *= corr;
-#pragma unroll
-                    for (int e = 0; e < AT_ONCE; e++) {
-                        if (k0 + e >= pre.z) break;
-                        const float y = exp2_fast(ml[e].x - use);
-                        a += w[e] * y;
-                        tot += ml[e].y * y;
-                    }
-                    M = top;
-                }
-            }
-            const bool empty = !(SHARED && pre.z > 0) && (p.causal ? L - n_q + t < 0 : L == 0);  // no key: zeros (a length that is none: NaN)
+            const bool empty = !(SHARED && pre_parts > 0) && (p.causal ? L - n_q + t < 0 : L == 0);  // no key: zeros (a length that is none: NaN)
             const float inv = 1.f / tot;
             float4_t w = empty ? float4_t{0.f, 0.f, 0.f, 0.f} : a * inv;
             if (bad_len) w = float4_t{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
@@ -739,16 +762,24 @@ void paged_decode_kernel(PagedAttnParams p) {
         const __amdgpu_buffer_rsrc_t rsrc = dev_rsrc(part);
         auto slot = [&](int k) { return (k == 0 ? slot0 : slot1 + (k - 1) * slot_step) * stride; };
         const int at_own = slot(own);
-        for (int i = threadIdx.x; i < NQ; i += kThreads) {
+#pragma unroll
+        for (int c = 0; c < CQ; c++) {
+            const int i = threadIdx.x + c * kThreads;
+            if (i >= NQ) break;
             const int row = i / (HD / 4), d = 4 * (i % (HD / 4));
             if (rt * RT + row >= p.rows) continue;
-            float mw[NW], M = kNegInf, tot = 0.f;
+            float mw[NW], M = SHARED ? pre_m[c] : kNegInf, tot = 0.f;
 #pragma unroll
             for (int w = 0; w < NW; w++) mw[w] = s_m[w][row];
 #pragma unroll
             for (int w = 0; w < NW; w++) M = fmaxf(M, mw[w]);
             const float Mu = M == kNegInf ? 0.f : M;
             float4_t acc = {0.f, 0.f, 0.f, 0.f};
+            if constexpr (SHARED) {
+                const float wt = exp2_fast(pre_m[c] - Mu);
+                tot = pre_l[c] * wt;
+                acc = pre_o[c] * wt;
+            }
 #pragma unroll
             for (int w = 0; w < NW; w++) {
                 const float wt = exp2_fast(mw[w] - Mu);

@@ -12,7 +12,7 @@ LIB = os.path.join(PKG, "libmx_attn.so")
 SOURCES = ["api.hip", "decode.hip", "prefill.hip", "rope.hip", "small.hip", "linear.hip",
            "paged_api.hip", "paged_store.hip", "paged_decode.hip", "paged_prefill.hip",
            "paged_store_e4m3.hip", "paged_decode_e4m3.hip", "paged_prefill_e4m3.hip",
-           "paged_prefix.hip", "paged_decode_shared.hip", "paged_decode_shared_e4m3.hip"]
+           "paged_shared.hip", "paged_shared_e4m3.hip", "paged_join.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 # -packed-fp32-ops off: the compiler must not emit packed f32 arithmetic (its host pass warns that it does not know

@@ -145,23 +145,27 @@ struct PagedStoreParams {
     PagedScales s;  // pages of codes
 };
 
-// Sequences that share their first keys: groups of them, and what the prefixes' kernel leaves for the decode behind it.
+// Sequences that share their first keys: groups of them, and where their partials go: head_dim + 4 floats a row, o, m and l.
 struct PagedPrefix {
     const int32_t * cu_seq;      // [n_groups + 1]: sequences cu_seq[g] .. cu_seq[g + 1] - 1 are group g's
     const int32_t * prefix_len;  // [n_groups]
     int32_t n_groups;
+    int32_t resident;            // workgroups that run at once
+    uint32_t blocks, own_blocks; // workgroups of the prefixes and of the sequences' own keys, multiples of 8
+    int32_t own_chunk;           // own keys of a workgroup; PagedAttnParams::fixed of them a sequence (the last takes what is left)
     int64_t max_rows;            // rows that `part` has room for
-    float * part;                // partials: head_dim + 4 floats a row
-    int32_t * rows;              // rows of the partials of a kv head
-    int32_t * start;             // [n_seq]: keys that are shared
-    int32_t * own_len;           // [n_seq]: keys from the multiple of 16 at or below them on; -1: a length that is none
-    int4 * info;                 // [n_seq]: the group's first row among the partials, its rows, parts, the sequence's row among them
+    float * part;                // of the prefixes: [kv head][group][part][row]
+    float * own_part;            // [sequence][chunk][kv head][row]
+    // what the prefixes' workgroups leave for the join:
+    int32_t * rows;              // rows of a kv head among the prefixes' partials
+    int32_t * own_len;           // [n_seq]: OwnKeys::len
+    int4 * info;                 // [n_seq]: the group's first row among a kv head's, its rows, its parts, the sequence's row among them
 };
 struct PagedPrefixPart {  // of a workgroup
     int64_t first;  // first row
     int32_t rows;
 };
-constexpr int kPagedPrefixWaves = 4;
+constexpr int kPagedPrefixWaves = 4;  // of both kinds of workgroups
 
 struct PagedAttnParams {
     PagedCache c;
@@ -189,6 +193,44 @@ struct PagedAttnParams {
     PagedPrefix x;         // shared prefixes
 };
 
+// The keys of a sequence behind the `start` that it shares: `len` of them, counted from the multiple of 16 at or below start; len -1: a
+// length, or prefix, that is none.
+struct OwnKeys {
+    int32_t start, len;
+};
+// Of a sequence of `len` keys in a group of sequences s0 .. s1 - 1 that share `keys` (in: or in none). Every row has to see all of them; a
+// sequence alone in its group shares nothing, nor does one without keys.
+__device__ __forceinline__ OwnKeys own_of(const PagedAttnParams & p, bool in, int s0, int s1, int keys, int len) {
+    const bool wrong = in && (keys < 0 || keys > p.c.capacity);
+    if (len == 0 || !length_ok(p.c, len) || wrong) return OwnKeys{0, len == 0 ? 0 : -1};
+    if (!in || s1 - s0 < 2 || keys == 0) return OwnKeys{0, len};
+    return len >= keys + (p.causal ? p.n_q - 1 : 0) ? OwnKeys{keys, len - (keys & ~15)} : OwnKeys{0, -1};
+}
+// Of sequence b, the same in every lane: 64 probes a step narrow the groups, whose bounds ascend, to 64.
+__device__ __forceinline__ OwnKeys own_keys(const PagedAttnParams & p, int b) {
+    const PagedPrefix & x = p.x;
+    const int lane = (int)__lane_id(), len = p.c.kv_len[b];
+    int first = 0, left = x.n_groups;
+    while (left > kWave) {
+        const int step = (left + kWave - 1) / kWave;
+        const uint64_t below = __builtin_amdgcn_ballot_w64(lane * step < left && x.cu_seq[min(first + lane * step, x.n_groups)] <= b);
+        const int skip = max(__builtin_popcountll(below) - 1, 0) * step;
+        first += skip;
+        left = min(step, left - skip);
+    }
+    const int i = min(first + lane, x.n_groups - 1), lo = x.cu_seq[i], hi = x.cu_seq[i + 1], keys = x.prefix_len[i];
+    const uint64_t from = __builtin_amdgcn_ballot_w64(lane < left && lo <= b);
+    const int l = from ? 63 - __builtin_clzll(from) : 0;
+    auto clamp = [&](int s) { return min(max(s, 0), p.c.n_seq); };
+    const int s0 = clamp(__builtin_amdgcn_readlane(lo, l)), s1 = clamp(__builtin_amdgcn_readlane(hi, l));
+    const OwnKeys r = own_of(p, from != 0 && b < s1, s0, s1, __builtin_amdgcn_readlane(keys, l), len);
+    return OwnKeys{__builtin_amdgcn_readfirstlane(r.start), __builtin_amdgcn_readfirstlane(r.len)};
+}
+// Chunks of them.
+__device__ __forceinline__ int own_chunks(const PagedAttnParams & p, int len) {
+    return len <= 0 ? 0 : min(p.fixed, (int)((uint32_t)(len + p.x.own_chunk - 1) / (uint32_t)p.x.own_chunk));
+}
+
 // Parts of a sequence in a decode at most: the join takes one lane each (131072 keys, Qwen2.5-7B heads, 54 us; with 33 67).
 constexpr int kPagedMaxParts = 64;
 
@@ -211,8 +253,8 @@ hipError_t launch_paged_decode_e4m3(const PagedAttnParams & p, int head_dim, int
 hipError_t launch_paged_prefill_e4m3(const PagedAttnParams & p, int head_dim, int dtype, const PagedPrefillPlan & plan, hipStream_t stream);
 hipError_t launch_paged_prefill(const PagedAttnParams & p, int head_dim, int dtype, const PagedPrefillPlan & plan, hipStream_t stream);
 
-hipError_t launch_paged_prefix(const PagedAttnParams & p, int head_dim, int dtype, bool e4m3, uint32_t grid, hipStream_t stream);
-hipError_t launch_paged_decode_shared(const PagedAttnParams & p, int head_dim, int dtype, int rt, hipStream_t stream);
-hipError_t launch_paged_decode_shared_e4m3(const PagedAttnParams & p, int head_dim, int dtype, int rt, hipStream_t stream);
+hipError_t launch_paged_shared(const PagedAttnParams & p, int head_dim, int dtype, int rt, hipStream_t stream);
+hipError_t launch_paged_shared_e4m3(const PagedAttnParams & p, int head_dim, int dtype, int rt, hipStream_t stream);
+hipError_t launch_paged_join(const PagedAttnParams & p, int head_dim, int dtype, hipStream_t stream);
 
 }  // namespace mx

@@ -195,16 +195,21 @@ int64_t kv_bound(const mx_paged_desc & d) {
     return d.max_kv_len > 0 && d.max_kv_len < table ? d.max_kv_len : table;
 }
 
-// four: the kernels have 4 waves only.
-int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan, bool four = false) {
+// A sequence's query rows that share a kv head, and their tiles.
+int32_t row_tiles(const mx_paged_desc & d, int32_t & rows, int32_t & rt, int32_t & n_rowtiles) {
     const int n_q = d.n_rows / d.n_seq;
     if ((int64_t)n_q * (d.n_head / d.n_head_kv) > 65536)
         return fail(MX_ATTN_UNSUPPORTED, "%d rows a sequence are a prompt (mx_paged_prefill)", n_q);
-    plan.rows = n_q * (d.n_head / d.n_head_kv);
+    rows = n_q * (d.n_head / d.n_head_kv);
     // A tile of 32 rows reads the keys once where two of 16 would twice (nine sequences of 201-5999 keys, 28 rows, 24 us against 31);
     // at head dim 256 its registers do not fit.
-    plan.rt = plan.rows > 16 && d.head_dim != 256 ? 32 : mx::decode_rows_per_tile(plan.rows);
-    plan.n_rowtiles = (plan.rows + plan.rt - 1) / plan.rt;
+    rt = rows > 16 && d.head_dim != 256 ? 32 : mx::decode_rows_per_tile(rows);
+    n_rowtiles = (rows + rt - 1) / rt;
+    return MX_ATTN_OK;
+}
+
+int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
+    if (int32_t rc = row_tiles(d, plan.rows, plan.rt, plan.n_rowtiles)) return rc;
     const int64_t per_seq = (int64_t)d.n_head_kv * plan.n_rowtiles, bound = kv_bound(d);
     auto quanta = [&](int waves) { return (bound + mx::kPagedDecodeBlock * waves - 1) / (mx::kPagedDecodeBlock * waves); };
     if (per_seq > mx::kCounterLines)
@@ -234,7 +239,7 @@ int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan, bool four = fals
         // against 10.6; 8192, Llama-3-8B heads, 11.3 against 14.8), and so have tiles of more rows. At head dim 256 the LDS holds 4
         // waves.
         plan.whole_keys = d.head_dim == 64 ? 640 : 512;
-        plan.waves = four || d.head_dim == 256 || bound <= 128 || (plan.rt <= 8 && bound > plan.whole_keys && bound <= 2048) ? 4 : 8;
+        plan.waves = d.head_dim == 256 || bound <= 128 || (plan.rt <= 8 && bound > plan.whole_keys && bound <= 2048) ? 4 : 8;
         if (plan.waves == 4) plan.whole_keys = 256;
         plan.ranges = (int32_t)std::max<int64_t>(d.n_seq, (plan.waves == 8 ? 1 : 2) * kCUs / per_seq);
         // Where one round of workgroups has room for every quantum of every sequence the chunks need no planning from the lengths:
@@ -309,36 +314,47 @@ size_t prefill_bytes(int head_dim) {
 
 // ---- shared prefixes ----
 
-// How the two launches run, and where in the workspace their data lies: the decode's part as it is, then what the first leaves.
+// How the launches run, and where in the workspace their data lies, behind the counters of other calls.
 struct SharedPlan {
-    DecodePlan own;
-    uint32_t grid;     // of the prefixes' launch
-    int32_t resident;  // its workgroups that run at once
-    int64_t max_rows;  // rows of its partials
-    size_t rows, start, own_len, info, part, bytes;  // offsets
+    int32_t rows, rt, n_rowtiles;  // of a sequence's own keys, as a decode's
+    int32_t resident, chunks, chunk;
+    int64_t blocks, own_blocks;
+    int64_t max_rows;              // rows of the prefixes' partials
+    size_t group_rows, own_len, info, own_part, part, bytes;  // offsets
 };
 
 int32_t shared_plan(const mx_paged_desc & d, int64_t n_groups, SharedPlan & plan) {
     if (n_groups < 0 || n_groups > d.n_seq) return fail(MX_ATTN_INVALID_ARGUMENT, "n_groups (%lld) must be in [0, n_seq]", (long long)n_groups);
     if ((int64_t)d.n_rows * d.n_head > (int64_t)1 << 26)
         return fail(MX_ATTN_UNSUPPORTED, "%d rows of %d heads are more than one launch holds", d.n_rows, d.n_head);
-    // a sequence's own keys are walked from a multiple of 16 on: up to 15 more than it has
-    mx_paged_desc own = d;
-    own.max_kv_len = d.max_kv_len ? (int32_t)std::min<int64_t>((int64_t)d.max_kv_len + 15, INT32_MAX) : 0;
-    if (int32_t rc = decode_plan(own, plan.own, true)) return rc;
-    // groups of one sequence have no part here: at most n_seq / 2 tiles are not full
     constexpr int kTile = 32 * mx::kPagedPrefixWaves;
+    if (int32_t rc = row_tiles(d, plan.rows, plan.rt, plan.n_rowtiles)) return rc;
+    const int64_t pairs = (int64_t)d.n_seq * d.n_head_kv * plan.n_rowtiles;
+    // Own keys in chunks of 128 or more, as many as there are workgroups for four rounds of the chip: FIG
+    // They are walked from a multiple of 16 on, up to 15 more than there are.
+    constexpr int kOwn = 8 * kCUs, kQuantum = 4 * mx::kPagedDecodeBlock;
+    const int64_t bound = std::min<int64_t>(kv_bound(d) + 15, (int64_t)1 << 30), most = (bound + kQuantum - 1) / kQuantum;
+    const int64_t n = std::min(most, (kOwn + pairs - 1) / pairs);
+    plan.chunk = (int32_t)((bound + n * kQuantum - 1) / (n * kQuantum) * kQuantum);
+    plan.chunks = (int32_t)((bound + plan.chunk - 1) / plan.chunk);
+    plan.own_blocks = (pairs * plan.chunks + 8 * plan.n_rowtiles - 1) / (8 * plan.n_rowtiles) * (8 * plan.n_rowtiles);
+    // groups of one sequence have no part here: at most n_seq / 2 tiles are not full
     const int64_t rows = (int64_t)d.n_rows * (d.n_head / d.n_head_kv), tiles = rows / kTile + std::min<int64_t>(n_groups, d.n_seq / 2) + 1;
     plan.resident = d.head_dim == 256 ? kCUs : 2 * kCUs;
-    plan.grid = (uint32_t)std::max<int64_t>(plan.resident, tiles * d.n_head_kv);
+    plan.blocks = (std::max<int64_t>(plan.resident, tiles * d.n_head_kv) + 7) / 8 * 8;
+    if (plan.blocks + plan.own_blocks > (int64_t)1 << 23)  // threads of a grid's dimension: below 2^32
+        return fail(MX_ATTN_UNSUPPORTED, "%d sequences of %d heads are more than one launch holds", d.n_seq, d.n_head);
     plan.max_rows = std::max<int64_t>((int64_t)plan.resident * kTile, (int64_t)d.n_rows * d.n_head);
+    // room for the chunks of fewer sequences too, which have more each
+    const int64_t own_rows = std::min<int64_t>((kOwn + pairs) * plan.rt, (int64_t)d.n_rows * d.n_head * most);
     auto round = [](size_t n) { return (n + 255) / 256 * 256; };
-    plan.rows = round(std::max<size_t>(plan.own.bytes, mx::kCounterBytes));
-    plan.start = plan.rows + 256;
-    plan.own_len = plan.start + round(4 * (size_t)d.n_seq);
+    const size_t row_bytes = (size_t)(d.head_dim + 4) * sizeof(float);
+    plan.group_rows = mx::kCounterBytes;
+    plan.own_len = plan.group_rows + 256;
     plan.info = plan.own_len + round(4 * (size_t)d.n_seq);
-    plan.part = plan.info + round(16 * (size_t)d.n_seq);
-    plan.bytes = plan.part + (size_t)plan.max_rows * (d.head_dim + 4) * sizeof(float);
+    plan.own_part = plan.info + round(16 * (size_t)d.n_seq);
+    plan.part = plan.own_part + round((size_t)own_rows * row_bytes);
+    plan.bytes = plan.part + (size_t)plan.max_rows * row_bytes;
     return MX_ATTN_OK;
 }
 
@@ -544,24 +560,30 @@ MX_ATTN_API int32_t mx_paged_decode_shared(const mx_paged_desc * desc, const mx_
     if (!prefix->cu_seq || !prefix->prefix_len || !aligned(prefix->cu_seq, 4) || !aligned(prefix->prefix_len, 4))
         return fail(MX_ATTN_INVALID_ARGUMENT, "prefix->cu_seq and prefix->prefix_len must be 4-byte aligned pointers");
     char * const ws = static_cast<char *>(workspace);
+    p.n_q = d.n_rows / d.n_seq;
+    p.rows = plan.rows;
+    p.n_rowtiles = plan.n_rowtiles;
+    p.fixed = plan.chunks;
+    p.ranges = d.n_seq * plan.chunks;
+    p.max_pages = d.max_pages;
     p.x.cu_seq = prefix->cu_seq;
     p.x.prefix_len = prefix->prefix_len;
     p.x.n_groups = prefix->n_groups;
+    p.x.resident = plan.resident;
+    p.x.blocks = (uint32_t)plan.blocks;
+    p.x.own_blocks = (uint32_t)plan.own_blocks;
+    p.x.own_chunk = plan.chunk;
     p.x.max_rows = plan.max_rows;
     p.x.part = reinterpret_cast<float *>(ws + plan.part);
-    p.x.rows = reinterpret_cast<int32_t *>(ws + plan.rows);
-    p.x.start = reinterpret_cast<int32_t *>(ws + plan.start);
+    p.x.own_part = reinterpret_cast<float *>(ws + plan.own_part);
+    p.x.rows = reinterpret_cast<int32_t *>(ws + plan.group_rows);
     p.x.own_len = reinterpret_cast<int32_t *>(ws + plan.own_len);
     p.x.info = reinterpret_cast<int4 *>(ws + plan.info);
-    p.n_q = d.n_rows / d.n_seq;
-    p.ranges = plan.resident;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    hipError_t e = mx::launch_paged_prefix(p, d.head_dim, d.dtype, scales != nullptr, plan.grid, s);
+    hipError_t e = (scales ? mx::launch_paged_shared_e4m3 : mx::launch_paged_shared)(p, d.head_dim, d.dtype, plan.rt, s);
     if (e != hipSuccess) return fail(MX_ATTN_INTERNAL, "shared prefix launch: %s", hipGetErrorString(e));
-    decode_params(d, plan.own, workspace, p);
-    p.c.kv_len = p.x.own_len;
-    e = (scales ? mx::launch_paged_decode_shared_e4m3 : mx::launch_paged_decode_shared)(p, d.head_dim, d.dtype, plan.own.rt, s);
-    if (e != hipSuccess) return fail(MX_ATTN_INTERNAL, "shared decode launch: %s", hipGetErrorString(e));
+    e = mx::launch_paged_join(p, d.head_dim, d.dtype, s);
+    if (e != hipSuccess) return fail(MX_ATTN_INTERNAL, "shared prefix join launch: %s", hipGetErrorString(e));
     return MX_ATTN_OK;
 }
 

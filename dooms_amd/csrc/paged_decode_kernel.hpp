@@ -186,14 +186,23 @@ __device__ __forceinline__ u32x4 load_kv(const char * a) {
     return __builtin_nontemporal_load((const __attribute__((address_space(1))) u32x4 *)(a));
 }
 
-// HD: head_dim. RT: query rows per tile (4, 8, 16 or 32; the matrix products have 16 or 32, the others are zero). T: type of
-// query rows and pages. NW: waves. RANGES: a workgroup walks a range of the launch's keys over the sequences in it, else one chunk.
-// Q8: the pages hold e4m3 codes with a scale a row, expanded to T on their way to LDS. SHARED: the sequences' first keys are done
-// already (PagedPrefix): positions count from the multiple of 16 at or below the first other key, and the prefix's partials are joined
-// in behind the sequence's own.
+// LDS of a workgroup: for each wave a block of values (or keys), then its outputs, and its rows' maxima and sums.
+template <int HD, int RT, int NW>
+struct DecodeSmem {
+    static constexpr int kBytes = kBlock * (HD + 16) * 2 > RT * HD * 4 ? kBlock * (HD + 16) * 2 : RT * HD * 4;  // of a wave
+    __attribute__((aligned(16))) char buf[NW][kBytes];
+    float m[NW][RT], l[NW][RT];
+    int last;
+};
+
+// Workgroup `id`. HD: head_dim. RT: query rows per tile (4, 8, 16 or 32; the matrix products have 16 or 32, the others are zero). T:
+// type of query rows and pages. NW: waves. RANGES: a workgroup walks a range of the launch's keys over the sequences in it, else one
+// chunk. Q8: the pages hold e4m3 codes with a scale a row, expanded to T on their way to LDS. SHARED: a chunk of the keys that a sequence
+// has behind a prefix it shares; positions count from the multiple of 16 at or below the first of them, and the chunk's partial is
+// left to the join of all.
 template <int HD, int RT, class T, int NW, bool RANGES, bool Q8, bool SHARED>
-__global__ __launch_bounds__(NW * kWave) __attribute__((amdgpu_waves_per_eu(HD == 256 || (RANGES && !((Q8 || SHARED) && RT <= 16)) ? 1 : 2)))
-void paged_decode_kernel(PagedAttnParams p) {
+__device__ __forceinline__ void decode_body(const PagedAttnParams & p, DecodeSmem<HD, RT, NW> & sm, const uint32_t id) {
+    static_assert(!(RANGES && SHARED), "own keys go in chunks");
     constexpr int QT = RT > 16 ? 2 : 1;  // 16-row product tiles
     constexpr int KS = HD / 32;          // product steps along head_dim
     constexpr int ES = Q8 ? 1 : 2;       // bytes of an element of the pages
@@ -216,18 +225,17 @@ void paged_decode_kernel(PagedAttnParams p) {
                          : RANGES || HD == 256 || (HD == 128 && RT == 32) ? 1 : HD == 64 && RT <= 16 ? 3 : 2;
     constexpr int SS = RT * PR;
     constexpr int NQ = RT * HD / 4;      // output quads of the tile
-    constexpr int CQ = (NQ + kThreads - 1) / kThreads;  // of those a thread has
-    constexpr int kLds = kBlock * VP * 2 > RT * HD * 4 ? kBlock * VP * 2 : RT * HD * 4;  // bytes of a wave: block, then outputs
     static_assert(16 % KPL == 0, "a load's rows lie in one page");
-    __shared__ __attribute__((aligned(16))) char s_buf[NW][kLds];
-    __shared__ float s_m[NW][RT], s_l[NW][RT];
-    __shared__ int s_last;
+    auto & s_buf = sm.buf;
+    auto & s_m = sm.m;
+    auto & s_l = sm.l;
+    int & s_last = sm.last;
     auto s_o = [&](int w) { return reinterpret_cast<float *>(s_buf[w]); };
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
     // kv heads fastest (workgroups are dealt to the 8 XCDs round-robin), the row tiles of one range on one XCD, 8 ids apart:
     // all but the first find its keys in that XCD's L2
-    const uint32_t id = blockIdx.x, tiles = p.n_rowtiles;
+    const uint32_t tiles = p.n_rowtiles;
     const uint32_t grp = id / (8 * tiles) * 8 + id % 8;
     const int rt = id / 8 % tiles, g = grp % p.n_head_kv, r = grp / p.n_head_kv;
     if (r >= p.ranges) return;  // the grid in whole rounds of XCDs
@@ -273,10 +281,6 @@ void paged_decode_kernel(PagedAttnParams p) {
     Range x{};
     Chunk ch{};
     int lens = 0, lens0 = 0;  // RANGES: the lengths of 64 sequences from lens0 on
-    int starts = 0;           // RANGES and SHARED: where they start
-    auto read_starts = [&]() __attribute__((always_inline)) {
-        if constexpr (SHARED) starts = p.x.start[min(lens0 + lane, n_seq - 1)];
-    };
     auto segment = [&](Seg & s, int len) __attribute__((always_inline)) {  // of s.b and s.at; returns its first key
         s.L = length_ok(p.c, len) ? len : -1;
         const int q1 = x.hi - s.at;
@@ -291,9 +295,7 @@ void paged_decode_kernel(PagedAttnParams p) {
                 if ((uint32_t)(s.b - lens0) >= (uint32_t)kWave) {
                     lens0 = s.b;
                     lens = p.c.kv_len[min(lens0 + lane, n_seq - 1)];
-                    read_starts();
                 }
-                s.start = SHARED ? __builtin_amdgcn_readlane(starts, s.b - lens0) : 0;
                 segment(s, __builtin_amdgcn_readlane(lens, s.b - lens0));
                 return;
             }
@@ -303,23 +305,31 @@ void paged_decode_kernel(PagedAttnParams p) {
     if constexpr (RANGES) {
         x = find_range<kStep>(p, r, lane, lens, lens0);
         if (x.b < 0) return;  // uniform over the workgroup
-        read_starts();
         seg.b = x.b;
         seg.at = x.at;
-        seg.start = SHARED ? __builtin_amdgcn_readlane(starts, x.b - lens0) : 0;
+        seg.start = 0;
         key0 = segment(seg, __builtin_amdgcn_readlane(lens, x.b - lens0));
     } else {
-        if (p.fixed) {
+        [[maybe_unused]] int own_start = 0;
+        if (SHARED || p.fixed) {
             // the host found room for p.fixed chunks of a quantum for every sequence: the chunk follows from the workgroup's
             // number, and its length and first page numbers are one round trip instead of two
             ch.i = (uint32_t)r / (uint32_t)n_seq;
             ch.b = r - ch.i * n_seq;
 #pragma unroll
             for (int i = 0; i < D && !SHARED; i++) ids[i] = read_ids(ch.b, (ch.i + i) * kStep + kBlock * wave, 0);
-            ch.len = __builtin_amdgcn_readfirstlane(p.c.kv_len[ch.b]);
-            ch.keys = kStep;
-            ch.n = min(p.fixed, quanta_of<kStep>(p, ch.len));
-            if (ch.len <= p.whole_keys) ch.n = 1;
+            if constexpr (SHARED) {
+                const OwnKeys own = own_keys(p, ch.b);
+                ch.len = own.len;
+                own_start = own.start;
+                ch.keys = p.x.own_chunk;
+                ch.n = own_chunks(p, own.len);
+            } else {
+                ch.len = __builtin_amdgcn_readfirstlane(p.c.kv_len[ch.b]);
+                ch.keys = kStep;
+                ch.n = min(p.fixed, quanta_of<kStep>(p, ch.len));
+                if (ch.len <= p.whole_keys) ch.n = 1;
+            }
             if (ch.i >= ch.n) return;
             ch.ordinal = ch.b;
             ch.slot = ch.b * p.fixed;
@@ -327,13 +337,13 @@ void paged_decode_kernel(PagedAttnParams p) {
             ch = find_chunk<kStep>(p, r, lane);
             if (ch.b < 0) return;  // uniform over the workgroup
 #pragma unroll
-            for (int i = 0; i < D && !SHARED; i++) ids[i] = read_ids(ch.b, ch.i * ch.keys + i * kStep + kBlock * wave, 0);
+            for (int i = 0; i < D; i++) ids[i] = read_ids(ch.b, ch.i * ch.keys + i * kStep + kBlock * wave, 0);
         }
         seg.b = ch.b;
         seg.at = 0;
         seg.start = 0;
         if constexpr (SHARED) {
-            seg.start = __builtin_amdgcn_readfirstlane(p.x.start[ch.b]);
+            seg.start = own_start;
 #pragma unroll
             for (int i = 0; i < D; i++) ids[i] = read_ids(ch.b, ch.i * ch.keys + i * kStep + kBlock * wave, seg.start);
         }
@@ -433,57 +443,6 @@ void paged_decode_kernel(PagedAttnParams p) {
         }
     }
 
-    // SHARED: the prefix's part of the thread's quads, which the sequence's first part has beside its own keys: a few partials in flight,
-    // each at its maximum, fetched while the first of those are in flight.
-    [[maybe_unused]] int4 pre{};  // the prefix's partials of the sequence
-    [[maybe_unused]] float pre_m[CQ], pre_l[CQ];
-    [[maybe_unused]] float4_t pre_o[CQ];
-    auto fold_prefix = [&](int parts) __attribute__((always_inline)) {
-        if constexpr (SHARED) {
-            constexpr int AT_ONCE = CQ == 1 ? 8 : CQ == 2 ? 4 : 2;
-#pragma unroll
-            for (int c = 0; c < CQ; c++) {
-                pre_m[c] = kNegInf;
-                pre_l[c] = 0.f;
-                pre_o[c] = float4_t{0.f, 0.f, 0.f, 0.f};
-            }
-            const int64_t rows = pre.y, first = (int64_t)g * *p.x.rows + pre.x;
-            for (int k0 = 0; k0 < parts; k0 += AT_ONCE) {
-                float4_t w[CQ][AT_ONCE];
-                float2 ml[CQ][AT_ONCE];
-#pragma unroll
-                for (int c = 0; c < CQ; c++) {
-                    const int i = min((int)threadIdx.x + c * kThreads, NQ - 1), d4 = i % (HD / 4);
-                    const int64_t row = pre.w + min(rt * RT + i / (HD / 4), p.rows - 1);
-#pragma unroll
-                    for (int e = 0; e < AT_ONCE; e++) {
-                        const float * x = p.x.part + (first + min(k0 + e, parts - 1) * rows) * (HD + 4);
-                        w[c][e] = *reinterpret_cast<const float4_t *>(x + (d4 * rows + row) * 4);
-                        ml[c][e] = *reinterpret_cast<const float2 *>(x + HD * rows + 2 * row);
-                    }
-                }
-#pragma unroll
-                for (int c = 0; c < CQ; c++) {
-                    float top = pre_m[c];
-#pragma unroll
-                    for (int e = 0; e < AT_ONCE; e++) top = fmaxf(top, ml[c][e].x);
-                    const float use = top == kNegInf ? 0.f : top, corr = exp2_fast(pre_m[c] - use);
-                    pre_o[c] *= corr;
-                    pre_l[c] *= corr;
-                    pre_m[c] = top;
-#pragma unroll
-                    for (int e = 0; e < AT_ONCE; e++) {
-                        if (k0 + e >= parts) break;
-                        const float y = exp2_fast(ml[c][e].x - use);
-                        pre_o[c] += w[c][e] * y;
-                        pre_l[c] += ml[c][e].y * y;
-                    }
-                }
-            }
-        }
-    };
-    if constexpr (SHARED) pre = p.x.info[seg.b];
-
     uint16_t * vw = reinterpret_cast<uint16_t *>(s_buf[wave]);
     const int v_rd = (4 * sgrp + (lane % 16) / 4) * VP + 4 * (lane % 4);
     auto wave_sync = [&]() {
@@ -495,8 +454,6 @@ void paged_decode_kernel(PagedAttnParams p) {
     for (;;) {
         const int L = max(seg.L, 0);
         const int skip = SHARED ? seg.start & 15 : 0;  // keys of the first 16 that the prefix has
-        const int pre_parts = SHARED ? pre.z : 0;
-        if constexpr (SHARED) fold_prefix((RANGES ? seg.at >= x.lo : ch.i == 0) ? pre.z : 0);
         int lim[QT];  // last key that the lane's row sees
 #pragma unroll
         for (int t = 0; t < QT; t++)
@@ -703,7 +660,6 @@ void paged_decode_kernel(PagedAttnParams p) {
         const Seg done = seg;
         next_segment(seg);
         if (seg.b >= 0) load_q(seg.b);  // in flight over what follows
-        if (SHARED && seg.b >= 0) pre = p.x.info[seg.b];
 
         // ---- join the waves; write the output, or publish this part ----
 #pragma unroll
@@ -727,7 +683,7 @@ void paged_decode_kernel(PagedAttnParams p) {
             const int rr = rt * RT + i;
             if (rr >= p.rows) return;
             const int t = rr / G, h = g * G + rr % G;
-            const bool empty = !(SHARED && pre_parts > 0) && (p.causal ? L - n_q + t < 0 : L == 0);  // no key: zeros (a length that is none: NaN)
+            const bool empty = p.causal ? L - n_q + t < 0 : L == 0;  // no key: zeros (a length that is none: NaN)
             const float inv = 1.f / tot;
             float4_t w = empty ? float4_t{0.f, 0.f, 0.f, 0.f} : a * inv;
             if (bad_len) w = float4_t{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
@@ -762,37 +718,34 @@ void paged_decode_kernel(PagedAttnParams p) {
         const __amdgpu_buffer_rsrc_t rsrc = dev_rsrc(part);
         auto slot = [&](int k) { return (k == 0 ? slot0 : slot1 + (k - 1) * slot_step) * stride; };
         const int at_own = slot(own);
-#pragma unroll
-        for (int c = 0; c < CQ; c++) {
-            const int i = threadIdx.x + c * kThreads;
-            if (i >= NQ) break;
+        for (int i = threadIdx.x; i < NQ; i += kThreads) {
             const int row = i / (HD / 4), d = 4 * (i % (HD / 4));
             if (rt * RT + row >= p.rows) continue;
-            float mw[NW], M = SHARED ? pre_m[c] : kNegInf, tot = 0.f;
+            float mw[NW], M = kNegInf, tot = 0.f;
 #pragma unroll
             for (int w = 0; w < NW; w++) mw[w] = s_m[w][row];
 #pragma unroll
             for (int w = 0; w < NW; w++) M = fmaxf(M, mw[w]);
             const float Mu = M == kNegInf ? 0.f : M;
             float4_t acc = {0.f, 0.f, 0.f, 0.f};
-            if constexpr (SHARED) {
-                const float wt = exp2_fast(pre_m[c] - Mu);
-                tot = pre_l[c] * wt;
-                acc = pre_o[c] * wt;
-            }
 #pragma unroll
             for (int w = 0; w < NW; w++) {
                 const float wt = exp2_fast(mw[w] - Mu);
                 tot += s_l[w][row] * wt;
                 acc += *reinterpret_cast<const float4_t *>(s_o(w) + row * HD + d) * wt;
             }
-            if (ns == 1) {
+            if constexpr (SHARED) {
+                float * to = p.x.own_part + ((((int64_t)done.b * p.fixed + ch.i) * p.n_head_kv + g) * p.rows + rt * RT + row) * (HD + 4);
+                *reinterpret_cast<float4_t *>(to + d) = acc;
+                if (d == 0) *reinterpret_cast<float2 *>(to + HD) = make_float2(M, tot);
+            } else if (ns == 1) {
                 emit(row, d, acc, M, tot);
             } else {
                 store16_dev(rsrc, 4 * (at_own + row * PR + d), acc);
                 if (d == 0) publish2(part + at_own + row * PR + HD, M, tot);
             }
         }
+        if constexpr (SHARED) return;
         if (ns > 1) {
             // the partial is complete at device scope before it is counted in
             __builtin_amdgcn_s_waitcnt(0);
@@ -889,34 +842,37 @@ void paged_decode_kernel(PagedAttnParams p) {
     }
 }
 
-template <int HD, class T, int NW, bool RANGES, bool Q8, bool SHARED>
+template <int HD, int RT, class T, int NW, bool RANGES, bool Q8>
+__global__ __launch_bounds__(NW * kWave) __attribute__((amdgpu_waves_per_eu(HD == 256 || (RANGES && !(Q8 && RT <= 16)) ? 1 : 2)))
+void paged_decode_kernel(PagedAttnParams p) {
+    __shared__ DecodeSmem<HD, RT, NW> sm;
+    decode_body<HD, RT, T, NW, RANGES, Q8, false>(p, sm, blockIdx.x);
+}
+
+template <int HD, class T, int NW, bool RANGES, bool Q8>
 void launch_rt(const PagedAttnParams & p, int rt, hipStream_t stream) {
     const int64_t groups = (int64_t)p.ranges * p.n_head_kv;
     const dim3 grid((uint32_t)(p.n_rowtiles == 1 ? groups : (groups + 7) / 8 * 8 * p.n_rowtiles)), block(NW * kWave);
-    if (rt == 4) hipLaunchKernelGGL((paged_decode_kernel<HD, 4, T, NW, RANGES, Q8, SHARED>), grid, block, 0, stream, p);
-    else if (rt == 8) hipLaunchKernelGGL((paged_decode_kernel<HD, 8, T, NW, RANGES, Q8, SHARED>), grid, block, 0, stream, p);
-    else if (rt == 16) hipLaunchKernelGGL((paged_decode_kernel<HD, 16, T, NW, RANGES, Q8, SHARED>), grid, block, 0, stream, p);
-    else if constexpr (HD != 256) hipLaunchKernelGGL((paged_decode_kernel<HD, 32, T, NW, RANGES, Q8, SHARED>), grid, block, 0, stream, p);
+    if (rt == 4) hipLaunchKernelGGL((paged_decode_kernel<HD, 4, T, NW, RANGES, Q8>), grid, block, 0, stream, p);
+    else if (rt == 8) hipLaunchKernelGGL((paged_decode_kernel<HD, 8, T, NW, RANGES, Q8>), grid, block, 0, stream, p);
+    else if (rt == 16) hipLaunchKernelGGL((paged_decode_kernel<HD, 16, T, NW, RANGES, Q8>), grid, block, 0, stream, p);
+    else if constexpr (HD != 256) hipLaunchKernelGGL((paged_decode_kernel<HD, 32, T, NW, RANGES, Q8>), grid, block, 0, stream, p);
 }
 
-// SHARED runs 4 waves: what sequences have of their own is seldom long.
-template <int HD, class T, bool Q8, bool SHARED>
-void launch_waves(const PagedAttnParams & p, int rt, int waves, hipStream_t stream) {
-    if constexpr (HD != 256 && !SHARED) {
-        if (!p.by_ranges && waves == 8) {
-            launch_rt<HD, T, 8, false, Q8, SHARED>(p, rt, stream);
-            return;
-        }
-    }
-    if (p.by_ranges) launch_rt<HD, T, 4, true, Q8, SHARED>(p, rt, stream);
-    else launch_rt<HD, T, 4, false, Q8, SHARED>(p, rt, stream);
-}
-
-template <class T, bool Q8, bool SHARED>
+template <class T, bool Q8>
 void launch_hd(const PagedAttnParams & p, int head_dim, int rt, int waves, hipStream_t stream) {
-    if (head_dim == 256) launch_waves<256, T, Q8, SHARED>(p, rt, waves, stream);
-    else if (head_dim == 64) launch_waves<64, T, Q8, SHARED>(p, rt, waves, stream);
-    else launch_waves<128, T, Q8, SHARED>(p, rt, waves, stream);
+    if (head_dim == 256) {
+        if (p.by_ranges) launch_rt<256, T, 4, true, Q8>(p, rt, stream);
+        else launch_rt<256, T, 4, false, Q8>(p, rt, stream);
+    } else if (head_dim == 64) {
+        if (p.by_ranges) launch_rt<64, T, 4, true, Q8>(p, rt, stream);
+        else if (waves == 8) launch_rt<64, T, 8, false, Q8>(p, rt, stream);
+        else launch_rt<64, T, 4, false, Q8>(p, rt, stream);
+    } else {
+        if (p.by_ranges) launch_rt<128, T, 4, true, Q8>(p, rt, stream);
+        else if (waves == 8) launch_rt<128, T, 8, false, Q8>(p, rt, stream);
+        else launch_rt<128, T, 4, false, Q8>(p, rt, stream);
+    }
 }
 
 }  // namespace

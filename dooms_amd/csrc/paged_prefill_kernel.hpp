@@ -183,7 +183,7 @@ __device__ __forceinline__ bool odd_values(const PagedAttnParams & p, const Tile
 // reading it back costs more than the shorter walk saves. The waves of the last workgroups also write what the kernel behind this
 // one needs to know of each sequence.
 template <int R, int W>
-__device__ __forceinline__ Tile plan_prefix(const PagedAttnParams & p, int wave, PagedPrefixPart & part) {
+__device__ __forceinline__ Tile plan_prefix(const PagedAttnParams & p, int wave, uint32_t block, uint32_t blocks, PagedPrefixPart & part) {
     const PagedPrefix & x = p.x;
     const int lane = threadIdx.x % kWave, n_seq = p.c.n_seq, per_seq = p.n_q * p.group;
     struct Group {
@@ -215,7 +215,7 @@ __device__ __forceinline__ Tile plan_prefix(const PagedAttnParams & p, int wave,
     }
     longest = wave_imax(longest);
     sum = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_sum(sum))));
-    const int room = max(1, p.ranges / p.n_head_kv);
+    const int room = max(1, p.x.resident / p.n_head_kv);
     auto count = [&](int c) {  // parts of a kv head, at most 2^30
         int r = 0;
         for (int base = 0; base < x.n_groups; base += kWave) {
@@ -235,11 +235,11 @@ __device__ __forceinline__ Tile plan_prefix(const PagedAttnParams & p, int wave,
     }
     // only ranges of cu_seq that overlap have more parts or rows than the launch
     const int64_t all = (int64_t)per_kv * p.n_head_kv;
-    const bool fits = all <= (int64_t)gridDim.x && rows * p.n_head_kv <= x.max_rows;
+    const bool fits = all <= (int64_t)blocks && rows * p.n_head_kv <= x.max_rows;
 
     // ---- the sequences: where their own keys start, how many they are, and where the partials lie ----
-    if (blockIdx.x == 0 && threadIdx.x == 0) *x.rows = fits ? (int32_t)rows : 0;
-    for (int64_t b0 = ((int64_t)(gridDim.x - 1 - blockIdx.x) * W + wave) * kWave; b0 < n_seq; b0 += (int64_t)gridDim.x * W * kWave) {
+    if (block == 0 && threadIdx.x == 0) *x.rows = fits ? (int32_t)rows : 0;
+    for (int64_t b0 = ((int64_t)(blocks - 1 - block) * W + wave) * kWave; b0 < n_seq; b0 += (int64_t)blocks * W * kWave) {
         const int b = min((int)b0 + lane, n_seq - 1);
         int g = 0, end = x.n_groups;  // the last group that does not start behind b
         while (__builtin_amdgcn_ballot_w64(end - g > 1)) {
@@ -251,9 +251,8 @@ __device__ __forceinline__ Tile plan_prefix(const PagedAttnParams & p, int wave,
         }
         const int s0 = clamp(x.cu_seq[g]), s1 = clamp(x.cu_seq[g + 1]), len = p.c.kv_len[b];
         const bool in = s0 <= b && b < s1;
-        const int keys = in ? x.prefix_len[g] : 0;
-        const bool shared = in && s1 - s0 > 1 && keys > 0 && keys <= p.c.capacity;
-        int start = 0, own = len, np = 0, group_rows = 0;
+        OwnKeys own = own_of(p, in, s0, s1, x.prefix_len[g], len);
+        int np = 0, group_rows = 0;
         int64_t first_row = 0;
         for (int base = 0; base < x.n_groups; base += kWave) {
             const Group r = at(base);
@@ -271,19 +270,10 @@ __device__ __forceinline__ Tile plan_prefix(const PagedAttnParams & p, int wave,
                 first_row += (uint32_t)last;
             }
         }
-        if (shared && len != 0) {
-            // a row has to see the keys of the prefix, every one
-            const bool ok = fits && length_ok(p.c, len) && len >= keys + (p.causal ? p.n_q - 1 : 0);
-            start = ok ? keys : 0;
-            own = ok ? len - (keys & ~15) : -1;
-            if (!ok) np = 0;
-        } else {
-            np = 0;
-            if (in && (keys < 0 || keys > p.c.capacity) && len != 0) own = -1;
-        }
+        if (own.start == 0) np = 0;
+        else if (!fits) own.len = -1;
         if ((int)b0 + lane < n_seq) {
-            x.own_len[b] = own;
-            x.start[b] = start;
+            x.own_len[b] = own.len;
             x.info[b] = make_int4((int)first_row, group_rows, np, (b - s0) * per_seq);
         }
     }
@@ -291,8 +281,8 @@ __device__ __forceinline__ Tile plan_prefix(const PagedAttnParams & p, int wave,
     // ---- the workgroup's part: by kv head, group, keys, then tiles, neighbours on one XCD ----
     Tile t{};
     t.b = -1;
-    if (!fits || blockIdx.x >= (uint32_t)all) return t;
-    int o = (int)xcd_remap(blockIdx.x, (uint32_t)all);
+    if (!fits || block >= (uint32_t)all) return t;
+    int o = (int)xcd_remap(block, (uint32_t)all);
     t.kvh = o / per_kv;
     o -= t.kvh * per_kv;
     int64_t before = 0;
@@ -327,8 +317,7 @@ __device__ __forceinline__ Tile plan_prefix(const PagedAttnParams & p, int wave,
 // each. Q8: the pages hold e4m3 codes with a scale a row, expanded to T in LDS. PREFIX: the keys that groups of sequences share, for all
 // rows of a group; a row is one of a query head then, and a workgroup computes one part of a tile and leaves it to the next kernel.
 template <int HD, class T, int W, int HPW, bool Q8, bool PREFIX>
-__global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(HD <= 128 ? 2 : 1, HD <= 128 ? 2 : 1)))
-void paged_prefill_kernel(PagedAttnParams p) {
+__device__ __forceinline__ void prefill_body(const PagedAttnParams & p, Smem<HD, W, Q8> & sm, int & s_last, const uint32_t block, const uint32_t blocks) {
     constexpr int RPW = W / HPW, R = 32 * RPW;  // row tiles of a head, and rows
     static_assert(R % kBK == 0, "tiles of whole steps");
     constexpr int KS = HD / 16;                 // product steps along head_dim for S^T
@@ -341,8 +330,6 @@ void paged_prefill_kernel(PagedAttnParams p) {
     constexpr int NBUF = Mem::NBUF, RING = Mem::RING, AHEAD = Mem::AHEAD;
     constexpr int LOADS = 2 * NI + (Q8 ? 1 : 0);  // of a step, a wave's
     static_assert(NB % W == 0 && W % RB == 0, "whole loads per wave, all of one row block");
-    __shared__ Mem sm;
-    __shared__ int s_last;
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x % kWave;
@@ -388,11 +375,11 @@ void paged_prefill_kernel(PagedAttnParams p) {
     int64_t hi_unit = 0, share = 1;
     int range = 0;
     if constexpr (PREFIX) {
-        t = plan_prefix<R, W>(p, wave, prefix_part);
+        t = plan_prefix<R, W>(p, wave, block, blocks, prefix_part);
         if (t.b < 0) return;
     } else if (direct) {
-        if (blockIdx.x >= (uint32_t)all) return;
-        int o = (int)xcd_remap(blockIdx.x, (uint32_t)all);
+        if (block >= (uint32_t)all) return;
+        int o = (int)xcd_remap(block, (uint32_t)all);
         t.kvh = o / (tiles * sets);
         o -= t.kvh * tiles * sets;
         t.set = o % sets;
@@ -415,7 +402,7 @@ void paged_prefill_kernel(PagedAttnParams p) {
     } else {
         if (total <= 0) return;
         // workgroups are dealt to the 8 XCDs round-robin: each XCD walks one eighth of the list, so few kv heads
-        range = (int)(blockIdx.x % 8) * (p.ranges / 8) + (int)(blockIdx.x / 8);
+        range = (int)(block % 8) * (p.ranges / 8) + (int)(block / 8);
         if (range >= p.ranges) return;
         share = max((total + p.ranges - 1) / p.ranges, (int64_t)kMinShare);
         const int64_t from = range * share;
@@ -870,17 +857,37 @@ void paged_prefill_kernel(PagedAttnParams p) {
         }
 
         if constexpr (PREFIX) {
-            // ---- the partial of this part: O in quads [HD / 4][rows], so that lanes of neighbouring rows store side by side, then (m, l) ----
+            // ---- the partial of this part: rows of O, m and l. Lanes hold rows; through LDS, 64 dims at a time, they store 256 bytes of a
+            // row side by side ----
             const float l = __builtin_amdgcn_ballot_w64(bad != 0) ? __builtin_nanf("") : xor32_add(l_run);
-            if (row < t.n) {
-                float * d = p.x.part + prefix_part.first * (HD + 4);
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();  // the keys and values are read
+            if (idle) return;
+            constexpr int PITCH = 64 + 4;
+            static_assert(sizeof(Mem) >= W * 32 * PITCH * 4, "a wave's rows");
+            float * mine = reinterpret_cast<float *>(&sm) + wave * 32 * PITCH;
+            float * d = p.x.part + (prefix_part.first + first_row) * (HD + 4);
+            if (row < t.n && hgrp == 0) *reinterpret_cast<float2 *>(d + (int64_t)l32 * (HD + 4) + HD) = make_float2(m_run, l);
 #pragma unroll
-                for (int dt = 0; dt < DT; dt++)
+            for (int part = 0; part < DT / 2; part++) {
+#pragma unroll
+                for (int x = 0; x < 2; x++)
 #pragma unroll
                     for (int gq = 0; gq < 4; gq++)
-                        *reinterpret_cast<float4_t *>(d + ((int64_t)(8 * dt + 2 * gq + hgrp) * prefix_part.rows + row) * 4) =
-                            float4_t{o[dt][4 * gq], o[dt][4 * gq + 1], o[dt][4 * gq + 2], o[dt][4 * gq + 3]};
-                if (hgrp == 0) *reinterpret_cast<float2 *>(d + (int64_t)HD * prefix_part.rows + 2 * row) = make_float2(m_run, l);
+                        *reinterpret_cast<float4_t *>(mine + l32 * PITCH + 32 * x + 8 * gq + 4 * hgrp) =
+                            float4_t{o[2 * part + x][4 * gq], o[2 * part + x][4 * gq + 1], o[2 * part + x][4 * gq + 2], o[2 * part + x][4 * gq + 3]};
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int r = 4 * i + lane / 16;
+                    const float4_t x = *reinterpret_cast<const float4_t *>(mine + r * PITCH + 4 * (lane % 16));
+                    if (first_row + r < t.n) *reinterpret_cast<float4_t *>(d + (int64_t)r * (HD + 4) + 64 * part + 4 * (lane % 16)) = x;
+                }
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
             }
             return;
         }
@@ -1039,8 +1046,16 @@ void paged_prefill_kernel(PagedAttnParams p) {
 }
 
 template <int HD, class T, int W, int HPW, bool Q8>
+__global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(HD <= 128 ? 2 : 1, HD <= 128 ? 2 : 1)))
+void paged_prefill_kernel(PagedAttnParams p) {
+    __shared__ Smem<HD, W, Q8> sm;
+    __shared__ int s_last;
+    prefill_body<HD, T, W, HPW, Q8, false>(p, sm, s_last, blockIdx.x, gridDim.x);
+}
+
+template <int HD, class T, int W, int HPW, bool Q8>
 void launch_shape(const PagedAttnParams & p, hipStream_t stream) {
-    hipLaunchKernelGGL((paged_prefill_kernel<HD, T, W, HPW, Q8, false>), dim3((uint32_t)p.ranges), dim3(W * kWave), 0, stream, p);
+    hipLaunchKernelGGL((paged_prefill_kernel<HD, T, W, HPW, Q8>), dim3((uint32_t)p.ranges), dim3(W * kWave), 0, stream, p);
 }
 
 // The shapes that the plans take: 8 waves at head dim 128 only, several heads with 8 waves only.
@@ -1062,14 +1077,6 @@ void launch_hd(const PagedAttnParams & p, int head_dim, const PagedPrefillPlan &
     if (head_dim == 64) launch_plan<64, T, Q8>(p, plan, stream);
     else if (head_dim == 128) launch_plan<128, T, Q8>(p, plan, stream);
     else launch_plan<256, T, Q8>(p, plan, stream);
-}
-
-template <class T, bool Q8>
-void launch_prefix(const PagedAttnParams & p, int head_dim, uint32_t grid, hipStream_t stream) {
-    const dim3 block(kPagedPrefixWaves * kWave);
-    if (head_dim == 64) hipLaunchKernelGGL((paged_prefill_kernel<64, T, kPagedPrefixWaves, 1, Q8, true>), dim3(grid), block, 0, stream, p);
-    else if (head_dim == 128) hipLaunchKernelGGL((paged_prefill_kernel<128, T, kPagedPrefixWaves, 1, Q8, true>), dim3(grid), block, 0, stream, p);
-    else hipLaunchKernelGGL((paged_prefill_kernel<256, T, kPagedPrefixWaves, 1, Q8, true>), dim3(grid), block, 0, stream, p);
 }
 
 }  // namespace

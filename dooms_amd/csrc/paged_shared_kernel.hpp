@@ -1,0 +1,54 @@
+// Decode attention of sequences that share prefixes: one launch that computes the partials of all keys, each shared one once for all rows
+// of its group, and one that joins them.
+//
+// For row r of a sequence with keys split into parts i (of the prefix, and of its own): m_i = max s, l_i = sum e^(s - m_i), o_i = sum
+// e^(s - m_i) v over the part's keys; M = max m_i, out = sum e^(m_i - M) o_i / sum e^(m_i - M) l_i.
+//
+// The first launch has two kinds of workgroups, dealt to the chip in turn: those of the prefixes are the packed prompts' kernel over all
+// query rows of a group (bound by the matrix cores and the exponentials), those of the sequences' own keys the decode kernel in chunks
+// (bound by the memory), so that a CU runs one of each side by side. FIGURES
+#pragma once
+
+#include "paged_decode_kernel.hpp"
+#include "paged_prefill_kernel.hpp"
+
+namespace mx {
+
+namespace {
+
+template <int HD, int RT, class T, bool Q8>
+__global__ __launch_bounds__(kPagedPrefixWaves * kWave) __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2)))
+void paged_shared_kernel(PagedAttnParams p) {
+    constexpr int W = kPagedPrefixWaves;
+    using Own = DecodeSmem<HD, RT, W>;
+    using Prefix = Smem<HD, W, Q8>;
+    __shared__ __attribute__((aligned(16))) char lds[sizeof(Own) > sizeof(Prefix) ? sizeof(Own) : sizeof(Prefix)];
+    __shared__ int last;
+    // eight of each kind (one an XCD) in turn, while there are both
+    const uint32_t id = blockIdx.x, a = p.x.blocks, b = p.x.own_blocks, both = min(a, b);
+    const bool own = id < 2 * both ? (id / 8) % 2 : b > a;
+    const uint32_t n = id < 2 * both ? id / 16 * 8 + id % 8 : id - both;
+    if (own) decode_body<HD, RT, T, W, false, Q8, true>(p, *reinterpret_cast<Own *>(lds), n);
+    else prefill_body<HD, T, W, 1, Q8, true>(p, *reinterpret_cast<Prefix *>(lds), last, n, a);
+}
+
+template <int HD, class T, bool Q8>
+void launch_shared_rt(const PagedAttnParams & p, int rt, hipStream_t stream) {
+    const dim3 grid(p.x.blocks + p.x.own_blocks), block(kPagedPrefixWaves * kWave);
+    if (rt == 4) hipLaunchKernelGGL((paged_shared_kernel<HD, 4, T, Q8>), grid, block, 0, stream, p);
+    else if (rt == 8) hipLaunchKernelGGL((paged_shared_kernel<HD, 8, T, Q8>), grid, block, 0, stream, p);
+    else if (rt == 16) hipLaunchKernelGGL((paged_shared_kernel<HD, 16, T, Q8>), grid, block, 0, stream, p);
+    else if constexpr (HD != 256) hipLaunchKernelGGL((paged_shared_kernel<HD, 32, T, Q8>), grid, block, 0, stream, p);
+}
+
+template <bool Q8>
+hipError_t launch_shared(const PagedAttnParams & p, int head_dim, int dtype, int rt, hipStream_t stream) {
+    if (head_dim == 64) dtype == 1 ? launch_shared_rt<64, F16, Q8>(p, rt, stream) : launch_shared_rt<64, BF16, Q8>(p, rt, stream);
+    else if (head_dim == 128) dtype == 1 ? launch_shared_rt<128, F16, Q8>(p, rt, stream) : launch_shared_rt<128, BF16, Q8>(p, rt, stream);
+    else dtype == 1 ? launch_shared_rt<256, F16, Q8>(p, rt, stream) : launch_shared_rt<256, BF16, Q8>(p, rt, stream);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+}  // namespace mx

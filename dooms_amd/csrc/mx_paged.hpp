@@ -150,8 +150,8 @@ struct PagedPrefix {
     const int32_t * cu_seq;      // [n_groups + 1]: sequences cu_seq[g] .. cu_seq[g + 1] - 1 are group g's
     const int32_t * prefix_len;  // [n_groups]
     int32_t n_groups;
-    int32_t resident;            // workgroups that run at once
-    uint32_t blocks, own_blocks; // workgroups of the prefixes and of the sequences' own keys, multiples of 8
+    int32_t room;                // workgroups that the prefixes are cut for
+    uint32_t blocks, own_blocks; // workgroups of the prefixes, and behind them those of the sequences' own keys; multiples of 8
     int32_t own_chunk;           // own keys of a workgroup; PagedAttnParams::fixed of them a sequence (the last takes what is left)
     int64_t max_rows;            // rows that `part` has room for
     float * part;                // of the prefixes: [kv head][group][part][row]

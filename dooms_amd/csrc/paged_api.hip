@@ -317,7 +317,7 @@ size_t prefill_bytes(int head_dim) {
 // How the launches run, and where in the workspace their data lies, behind the counters of other calls.
 struct SharedPlan {
     int32_t rows, rt, n_rowtiles;  // of a sequence's own keys, as a decode's
-    int32_t resident, chunks, chunk;
+    int32_t room, chunks, chunk;
     int64_t blocks, own_blocks;
     int64_t max_rows;              // rows of the prefixes' partials
     size_t group_rows, own_len, info, own_part, part, bytes;  // offsets
@@ -330,9 +330,10 @@ int32_t shared_plan(const mx_paged_desc & d, int64_t n_groups, SharedPlan & plan
     constexpr int kTile = 32 * mx::kPagedPrefixWaves;
     if (int32_t rc = row_tiles(d, plan.rows, plan.rt, plan.n_rowtiles)) return rc;
     const int64_t pairs = (int64_t)d.n_seq * d.n_head_kv * plan.n_rowtiles;
-    // Own keys in chunks of 128 or more, as many as there are workgroups for four rounds of the chip: FIG
+    // Own keys in chunks of 128 or more, up to two rounds of the chip's workgroups (64 sequences of 40-900 own keys behind 4096, Llama-3-8B
+    // heads, 43.4 us; one round 44.5, four 45.3; 192 of 100-1500 behind 16384, 179, 179 and 182).
     // They are walked from a multiple of 16 on, up to 15 more than there are.
-    constexpr int kOwn = 8 * kCUs, kQuantum = 4 * mx::kPagedDecodeBlock;
+    constexpr int kOwn = 4 * kCUs, kQuantum = 4 * mx::kPagedDecodeBlock;
     const int64_t bound = std::min<int64_t>(kv_bound(d) + 15, (int64_t)1 << 30), most = (bound + kQuantum - 1) / kQuantum;
     const int64_t n = std::min(most, (kOwn + pairs - 1) / pairs);
     plan.chunk = (int32_t)((bound + n * kQuantum - 1) / (n * kQuantum) * kQuantum);
@@ -340,11 +341,13 @@ int32_t shared_plan(const mx_paged_desc & d, int64_t n_groups, SharedPlan & plan
     plan.own_blocks = (pairs * plan.chunks + 8 * plan.n_rowtiles - 1) / (8 * plan.n_rowtiles) * (8 * plan.n_rowtiles);
     // groups of one sequence have no part here: at most n_seq / 2 tiles are not full
     const int64_t rows = (int64_t)d.n_rows * (d.n_head / d.n_head_kv), tiles = rows / kTile + std::min<int64_t>(n_groups, d.n_seq / 2) + 1;
-    plan.resident = d.head_dim == 256 ? kCUs : 2 * kCUs;
-    plan.blocks = (std::max<int64_t>(plan.resident, tiles * d.n_head_kv) + 7) / 8 * 8;
+    // The prefixes are cut for a workgroup on each CU: a second one there walks own keys, and more parts are more to write and join (40 x
+    // 2 rows in five groups, Qwen2.5-7B heads in 8 bits, 31.1 us, cut for two 35.4; 192 sequences behind 16384 keys 176 and 179).
+    plan.room = kCUs;
+    plan.blocks = (std::max<int64_t>(plan.room, tiles * d.n_head_kv) + 7) / 8 * 8;
     if (plan.blocks + plan.own_blocks > (int64_t)1 << 23)  // threads of a grid's dimension: below 2^32
         return fail(MX_ATTN_UNSUPPORTED, "%d sequences of %d heads are more than one launch holds", d.n_seq, d.n_head);
-    plan.max_rows = std::max<int64_t>((int64_t)plan.resident * kTile, (int64_t)d.n_rows * d.n_head);
+    plan.max_rows = std::max<int64_t>((int64_t)plan.room * kTile, (int64_t)d.n_rows * d.n_head);
     // room for the chunks of fewer sequences too, which have more each
     const int64_t own_rows = std::min<int64_t>((kOwn + pairs) * plan.rt, (int64_t)d.n_rows * d.n_head * most);
     auto round = [](size_t n) { return (n + 255) / 256 * 256; };
@@ -569,7 +572,7 @@ MX_ATTN_API int32_t mx_paged_decode_shared(const mx_paged_desc * desc, const mx_
     p.x.cu_seq = prefix->cu_seq;
     p.x.prefix_len = prefix->prefix_len;
     p.x.n_groups = prefix->n_groups;
-    p.x.resident = plan.resident;
+    p.x.room = plan.room;
     p.x.blocks = (uint32_t)plan.blocks;
     p.x.own_blocks = (uint32_t)plan.own_blocks;
     p.x.own_chunk = plan.chunk;

@@ -215,7 +215,7 @@ __device__ __forceinline__ Tile plan_prefix(const PagedAttnParams & p, int wave,
     }
     longest = wave_imax(longest);
     sum = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_sum(sum))));
-    const int room = max(1, p.x.resident / p.n_head_kv);
+    const int room = max(1, p.x.room / p.n_head_kv);
     auto count = [&](int c) {  // parts of a kv head, at most 2^30
         int r = 0;
         for (int base = 0; base < x.n_groups; base += kWave) {

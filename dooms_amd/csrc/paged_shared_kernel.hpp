@@ -24,10 +24,9 @@ void paged_shared_kernel(PagedAttnParams p) {
     using Prefix = Smem<HD, W, Q8>;
     __shared__ __attribute__((aligned(16))) char lds[sizeof(Own) > sizeof(Prefix) ? sizeof(Own) : sizeof(Prefix)];
     __shared__ int last;
-    // eight of each kind (one an XCD) in turn, while there are both
-    const uint32_t id = blockIdx.x, a = p.x.blocks, b = p.x.own_blocks, both = min(a, b);
-    const bool own = id < 2 * both ? (id / 8) % 2 : b > a;
-    const uint32_t n = id < 2 * both ? id / 16 * 8 + id % 8 : id - both;
+    const uint32_t id = blockIdx.x, a = p.x.blocks;
+    const bool own = id >= a;
+    const uint32_t n = own ? id - a : id;
     if (own) decode_body<HD, RT, T, W, false, Q8, true>(p, *reinterpret_cast<Own *>(lds), n);
     else prefill_body<HD, T, W, 1, Q8, true>(p, *reinterpret_cast<Prefix *>(lds), last, n, a);
 }

@@ -358,7 +358,11 @@ int32_t shared_plan(const mx_paged_desc & d, int64_t n_groups, SharedPlan & plan
     plan.own_part = plan.info + round(16 * (size_t)d.n_seq);
     plan.part = plan.own_part + round((size_t)own_rows * row_bytes);
     plan.bytes = plan.part + (size_t)plan.max_rows * row_bytes;
-    return MX_ATTN_OK;
+    // without groups the call is a decode
+    DecodePlan alone;
+    const int32_t rc = decode_plan(d, alone);
+    if (rc == MX_ATTN_OK) plan.bytes = std::max(plan.bytes, alone.bytes);
+    return n_groups == 0 ? rc : MX_ATTN_OK;
 }
 
 // ---- the calls, over pages of the queries' type (s null) or of codes ----

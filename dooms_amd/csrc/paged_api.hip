@@ -329,6 +329,7 @@ int32_t shared_plan(const mx_paged_desc & d, int64_t n_groups, SharedPlan & plan
         return fail(MX_ATTN_UNSUPPORTED, "%d rows of %d heads are more than one launch holds", d.n_rows, d.n_head);
     constexpr int kTile = 32 * mx::kPagedPrefixWaves;
     if (int32_t rc = row_tiles(d, plan.rows, plan.rt, plan.n_rowtiles)) return rc;
+    plan.rt = std::max(plan.rt, 16);  // the products have 16 rows, and a partial the live ones, with tiles of 4 and 8 too
     const int64_t pairs = (int64_t)d.n_seq * d.n_head_kv * plan.n_rowtiles;
     // Own keys in chunks of 128 or more, up to two rounds of the chip's workgroups (64 sequences of 40-900 own keys behind 4096, Llama-3-8B
     // heads, 43.4 us; one round 44.5, four 45.3; 192 of 100-1500 behind 16384, 179, 179 and 182).
@@ -349,7 +350,7 @@ int32_t shared_plan(const mx_paged_desc & d, int64_t n_groups, SharedPlan & plan
         return fail(MX_ATTN_UNSUPPORTED, "%d sequences of %d heads are more than one launch holds", d.n_seq, d.n_head);
     plan.max_rows = std::max<int64_t>((int64_t)plan.room * kTile, (int64_t)d.n_rows * d.n_head);
     // room for the chunks of fewer sequences too, which have more each
-    const int64_t own_rows = std::min<int64_t>((kOwn + pairs) * plan.rt, (int64_t)d.n_rows * d.n_head * most);
+    const int64_t own_rows = std::min<int64_t>((kOwn + pairs) * std::min(plan.rt, plan.rows), (int64_t)d.n_rows * d.n_head * most);
     auto round = [](size_t n) { return (n + 255) / 256 * 256; };
     const size_t row_bytes = (size_t)(d.head_dim + 4) * sizeof(float);
     plan.group_rows = mx::kCounterBytes;

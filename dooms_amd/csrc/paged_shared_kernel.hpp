@@ -34,9 +34,7 @@ void paged_shared_kernel(PagedAttnParams p) {
 template <int HD, class T, bool Q8>
 void launch_shared_rt(const PagedAttnParams & p, int rt, hipStream_t stream) {
     const dim3 grid(p.x.blocks + p.x.own_blocks), block(kPagedPrefixWaves * kWave);
-    if (rt == 4) hipLaunchKernelGGL((paged_shared_kernel<HD, 4, T, Q8>), grid, block, 0, stream, p);
-    else if (rt == 8) hipLaunchKernelGGL((paged_shared_kernel<HD, 8, T, Q8>), grid, block, 0, stream, p);
-    else if (rt == 16) hipLaunchKernelGGL((paged_shared_kernel<HD, 16, T, Q8>), grid, block, 0, stream, p);
+    if (rt == 16) hipLaunchKernelGGL((paged_shared_kernel<HD, 16, T, Q8>), grid, block, 0, stream, p);
     else if constexpr (HD != 256) hipLaunchKernelGGL((paged_shared_kernel<HD, 32, T, Q8>), grid, block, 0, stream, p);
 }
 

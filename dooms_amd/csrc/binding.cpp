@@ -540,7 +540,7 @@ PyObject * attend(PyObject * const * a) {
     [[maybe_unused]] mx_paged_prefix prefix{};
     if constexpr (KIND == kShared) {
         const at::Tensor & n = tensor(a[18]);
-        need(n.dim() == 1 && n.size(0) <= d.n_seq);
+        need(n.dim() == 1 && n.size(0) <= INT32_MAX);
         prefix.n_groups = (int32_t)n.size(0);
         prefix.prefix_len = data<int32_t>(ints(a[18], n.size(0), q));
         prefix.cu_seq = data<int32_t>(ints(a[17], n.size(0) + 1, q));

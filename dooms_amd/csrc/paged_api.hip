@@ -324,7 +324,7 @@ struct SharedPlan {
 };
 
 int32_t shared_plan(const mx_paged_desc & d, int64_t n_groups, SharedPlan & plan) {
-    if (n_groups < 0 || n_groups > d.n_seq) return fail(MX_ATTN_INVALID_ARGUMENT, "n_groups (%lld) must be in [0, n_seq]", (long long)n_groups);
+    if (n_groups < 0 || n_groups > 65535) return fail(MX_ATTN_INVALID_ARGUMENT, "n_groups (%lld) must be in [0, 65535]", (long long)n_groups);
     if ((int64_t)d.n_rows * d.n_head > (int64_t)1 << 26)
         return fail(MX_ATTN_UNSUPPORTED, "%d rows of %d heads are more than one launch holds", d.n_rows, d.n_head);
     constexpr int kTile = 32 * mx::kPagedPrefixWaves;

@@ -164,7 +164,7 @@ MX_ATTN_API size_t mx_paged_decode_workspace_bytes(const mx_paged_desc * desc);
  * that no group has share nothing.
  */
 typedef struct mx_paged_prefix {
-    int32_t n_groups;           /* 0 .. n_seq (0: nothing is shared) */
+    int32_t n_groups;           /* 0 .. 65535 (0: nothing is shared); groups may be empty */
     int32_t reserved;           /* must be 0 */
     const int32_t * cu_seq;     /* device, [n_groups + 1]: sequences cu_seq[g] .. cu_seq[g + 1] - 1 are group g's; ascending */
     const int32_t * prefix_len; /* device, [n_groups]: the keys that the sequences of a group have in common, from key 0 on; any
@@ -176,7 +176,7 @@ typedef struct mx_paged_prefix {
  * once for all rows of its group instead of once a sequence. Two launches: the prefixes, for all query rows of a group on the matrix
  * cores together, then each sequence's own keys, with which the prefix's partials are joined.
  *
- * The keys of a prefix are found through the page table of its group's first sequence; the other sequences' entries for whole
+ * The keys of a prefix are found through the page table of its group's first sequence, also where that one has 0 keys; the other sequences' entries for whole
  * pages of it are not read, and rows of it in a page that holds keys of a sequence's own (where the prefix ends within a page) are
  * never used. kv_len counts the prefix's keys too. Every row has to see the whole prefix: a sequence with fewer keys than the
  * prefix (causal: than the prefix and all but one of its new rows), but not 0, or with a prefix_len outside

@@ -437,3 +437,48 @@ def test_extension_and_general_path_agree(device, monkeypatch):
     monkeypatch.setattr(A, "_native", lambda: A._General())
     for a, b in zip(want, calls()):
         assert torch.equal(a, b)
+
+
+def test_pages_four_gigabytes_apart(device):
+    """Codes and scales whose offsets pass 32 bits, for the append, a decode and a prompt."""
+    g = gen(42)
+    c = Cache8(g, [40, 33], 2, 128, 16, F16)
+    total, apart = c.k.shape[0], (1 << 32) // 3 // 16 * 16 + 4096  # the pool spans more than 2^32 bytes from its fourth page on
+
+    def far(t, shape, strides):
+        wide = torch.empty(apart * total, dtype=torch.uint8, device=device).as_strided(shape, (apart, *strides))
+        wide.copy_(t)
+        return wide
+    k, v = (far(t, t.shape, (256, 128, 1)).view(E4M3) for t in (c.k, c.v))
+    scales = [far(t, t.shape, (16, 1)).view(E8M0) for t in (c.ks, c.vs)]
+    _, _, table, kv_len, _ = c.to(device)
+    q = torch.randn(2, 8 * 128, generator=g).to(F16)
+    ref, _, tol, _ = attend(c, q, [1, 1], 8, 128 ** -0.5, True, False, F16)
+    close(A.paged_decode(q.to(device), k, v, table, kv_len, n_head=8, scales=scales)[0], ref, tol, "decode")
+    ref, _, tol, _ = attend(c, q, [1, 1], 8, 128 ** -0.5, True, True, F16)
+    close(A.paged_prefill(q.to(device), k, v, table, kv_len, cu_of([1, 1], device), n_head=8, scales=scales)[0], ref, tol, "prompt")
+    x = torch.randn(2, 12 * 128, generator=g)
+    A.paged_store(x.to(device), k, v, table, kv_len, n_head=8, rope_mode=2, scales=scales)
+    for b, L in enumerate(c.lens):
+        page, row = int(c.table[b, (L - 1) // 16]), (L - 1) % 16
+        for pool, scale, at in ((k, scales[0], 1024), (v, scales[1], 1280)):
+            check_rows(pool.view(torch.uint8)[page, row][None].cpu(), scale.view(torch.uint8)[page, :, row][None].cpu(),
+                       x[b, at:at + 256].double().view(1, 2, 128), torch.zeros(1, 2, 128, dtype=torch.float64), f"row {b}")
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_results_do_not_depend_on_the_run(device, hd):
+    g = gen(43)
+    lens = [2100, 7, 900, 0, 333]
+    c = Cache8(g, lens, 4, hd, 16, BF16)
+    k, v, table, kv_len, scales = c.to(device)
+    q = torch.randn(5, 16 * hd, generator=g).to(BF16).to(device)
+    rows = [200, 7, 90, 0, 333]
+    p = torch.randn(sum(rows), 16 * hd, generator=g).to(BF16).to(device)
+    ws = A.new_workspace(128 << 20, device)
+    call = lambda: (A.paged_decode(q, k, v, table, kv_len, n_head=16, scales=scales, workspace=ws)[0],
+                    A.paged_prefill(p, k, v, table, kv_len, cu_of(rows, device), n_head=16, scales=scales, workspace=ws)[0])
+    want = call()
+    for _ in range(10):
+        for a, b in zip(call(), want):
+            assert torch.equal(a, b)

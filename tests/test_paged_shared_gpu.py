@@ -306,3 +306,71 @@ def test_extension_and_general_path_agree(device, monkeypatch):
                                      scales=scales)  # no groups: nothing is shared
         alone, _ = A.paged_decode(q[:1], *args[:2], args[2][:1].contiguous(), args[3][:1].contiguous(), n_head=8, scales=scales)
         assert torch.equal(o, alone)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_groups_of_one_and_one_sequence(device, eight):
+    """Nothing is shared then, and the results are those of a decode."""
+    for groups in ([(30, [5])], [(30 + 7 * i, [1 + 40 * i]) for i in range(9)]):
+        check(device, 65, 8, 2, 128, groups, 16, F16, eight=eight, what=f"{len(groups)}")
+
+
+@pytest.mark.parametrize("n_groups", [64, 65, 4200])
+def test_many_groups(device, n_groups):
+    """A sequence's group among many, with runs of empty ones."""
+    groups = [(16 + i % 40, [] if i % 7 == 3 or 20 <= i < 30 else [1 + i % 9] * (1 + i % 3 // 2)) for i in range(n_groups)]
+    check(device, 66, 1, 1, 64, groups, 16, F16, own_hint=9)
+
+
+def test_calls_on_two_streams(device):
+    """Each with a workspace of its own."""
+    g = gen(67)
+    s = Shared(g, [(2000, [1 + 37 * i % 300 for i in range(20)])], 4, 128, 16, BF16)
+    args, _ = s.to(device)
+    qs = [torch.randn(20, 16 * 128, generator=g).to(BF16).to(device) for _ in range(2)]
+    ws = [A.new_workspace(64 << 20, device) for _ in range(2)]
+    want = [A.paged_decode_shared(q, *args, n_head=16, workspace=w)[0] for q, w in zip(qs, ws)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(A.paged_decode_shared(qs[i], *args, n_head=16, workspace=ws[i])[0])
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o in got[i]:
+            assert torch.equal(o, want[i])
+
+
+def test_workspace_shared_with_other_calls(device):
+    """The counters of the calls that keep them lie in front of what this one writes."""
+    g = gen(68)
+    s = Shared(g, [(2496, [1 + 37 * i % 500 for i in range(12)])], 4, 128, 16, F16)
+    q = torch.randn(12, 16 * 128, generator=g).to(F16).to(device)
+    args, _ = s.to(device)
+    table = s.cache.table.clone()
+    table[1:, :156] = table[0, :156]  # whole pages of the prefix, which a plain decode reads too
+    plain = (args[0], args[1], table.to(device), args[3])
+    prompt = torch.randn(300, 16 * 128, generator=g).to(F16).to(device)
+    cu = torch.tensor([0] * 12 + [300], dtype=torch.int32, device=device)
+    calls = [lambda w: A.paged_decode_shared(q, *args, n_head=16, workspace=w)[0], lambda w: A.paged_decode(q, *plain, n_head=16, workspace=w)[0],
+             lambda w: A.paged_prefill(prompt, *plain, cu, n_head=16, workspace=w)[0]]
+    want = [f(A.new_workspace(128 << 20, device)) for f in calls]
+    ws = A.new_workspace(128 << 20, device)
+    for _ in range(3):
+        for f, w in zip(calls, want):
+            assert torch.equal(f(ws), w)
+            assert not ws[:A._PAGED_COUNTERS].any()
+
+
+def test_calls_without_groups_need_no_more(device):
+    """The workspace sized for a call serves it without groups as well."""
+    for n_head, n_kv, hd, n_seq in ((8, 2, 128, 1), (14, 2, 64, 3), (4, 1, 256, 40)):
+        g = gen(69)
+        c = Cache(g, [900 + 7 * i for i in range(n_seq)], n_kv, hd, 16, F16)
+        q = torch.randn(n_seq, n_head * hd, generator=g).to(F16).to(device)
+        none = torch.zeros(1, dtype=torch.int32, device=device)
+        nb = A.paged_shared_workspace_bytes(n_head=n_head, n_head_kv=n_kv, head_dim=hd, n_q=1, n_seq=n_seq, n_groups=0, max_own_len=2000)
+        ws = A.new_workspace(nb, device)
+        ref, _, tol, _ = attend(c, q.cpu(), [1] * n_seq, n_head, hd ** -0.5, True, False, F16)
+        close(A.paged_decode_shared(q, *c.to(device), none, none[:0], n_head=n_head, max_own_len=2000, workspace=ws)[0], ref, tol, "out")

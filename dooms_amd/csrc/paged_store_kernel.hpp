@@ -43,6 +43,43 @@ __device__ __forceinline__ float2 cos_sin(double x) {
     return q == 0 ? make_float2(c, s) : q == 1 ? make_float2(-s, c) : q == 2 ? make_float2(-c, -s) : make_float2(s, -c);
 }
 
+// cos and sin of an angle in 64 bits, reduced as above; the Taylor series on |r| <= pi / 4 to degree 17 (truncation below 2^-58).
+__device__ __forceinline__ double2 cos_sin64(double x) {
+    constexpr double kTwoOverPi = 0.63661977236758134308, kPio2Hi = 1.5707963267948966, kPio2Lo = 6.123233995736766e-17;
+    const double k = __builtin_rint(x * kTwoOverPi);
+    const double r = __builtin_fma(-k, kPio2Lo, __builtin_fma(-k, kPio2Hi, x)), r2 = r * r;
+    double s = 1. / 355687428096000.;
+    s = __builtin_fma(s, r2, -1. / 1307674368000.);
+    s = __builtin_fma(s, r2, 1. / 6227020800.);
+    s = __builtin_fma(s, r2, -1. / 39916800.);
+    s = __builtin_fma(s, r2, 1. / 362880.);
+    s = __builtin_fma(s, r2, -1. / 5040.);
+    s = __builtin_fma(s, r2, 1. / 120.);
+    s = __builtin_fma(s, r2, -1. / 6.);
+    s = __builtin_fma(s * r2, r, r);
+    double c = 1. / 20922789888000.;
+    c = __builtin_fma(c, r2, -1. / 87178291200.);
+    c = __builtin_fma(c, r2, 1. / 479001600.);
+    c = __builtin_fma(c, r2, -1. / 3628800.);
+    c = __builtin_fma(c, r2, 1. / 40320.);
+    c = __builtin_fma(c, r2, -1. / 720.);
+    c = __builtin_fma(c, r2, 1. / 24.);
+    c = __builtin_fma(c, r2, -0.5);
+    c = __builtin_fma(c, r2, 1.);
+    const int q = (int)((long long)k & 3);
+    return q == 0 ? make_double2(c, s) : q == 1 ? make_double2(-s, c) : q == 2 ? make_double2(-c, -s) : make_double2(s, -c);
+}
+
+// v in 32 bits, rounded to odd: towards zero, with the last bit set where that was not exact, so that rounding the result to fewer bits
+// gives what rounding v once does. An infinity or NaN, and what 32 bits do not hold, stay no finite number.
+__device__ __forceinline__ float round_odd(double v) {
+    const float f = (float)v;
+    const double back = (double)f;
+    if (back == v || !__builtin_isfinite(f)) return f;
+    const uint32_t b = __float_as_uint(f);
+    return __uint_as_float((__builtin_fabs(back) > __builtin_fabs(v) ? b - 1 : b) | 1u);
+}
+
 // The maximum over N lanes in a row (a power of two up to 32, aligned), in each; lanes outside may be off.
 template <int N>
 __device__ __forceinline__ float lanes_max(float v) {
@@ -77,6 +114,7 @@ __global__ __launch_bounds__(512) void paged_store_kernel(PagedStoreParams p) {
     constexpr int HALF = HD / 2;
     constexpr int AHEAD = 2;                  // units a thread loads at once
     __shared__ float2 s_cs[HALF];
+    __shared__ double2 s_cd[Q8 ? HALF : 1];  // Q8: for the keys, whose codes are those of the rotation in 64 bits
 
     const int64_t block = blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
     if (block >= p.n_rows) return;
@@ -146,7 +184,12 @@ __global__ __launch_bounds__(512) void paged_store_kernel(PagedStoreParams p) {
                 for (int a = 0; a + 1 < kPagedMaxAxes; a++) axis += a + 1 < p.n_axes && i >= p.axis_end[a];
                 at = p.positions[(int64_t)axis * p.n_rows + row];
             }
-            s_cs[i] = cos_sin((double)at * p.freq[i]);
+            if constexpr (Q8) {
+                s_cd[i] = cos_sin64((double)at * p.freq[i]);
+                s_cs[i] = make_float2((float)s_cd[i].x, (float)s_cd[i].y);
+            } else {
+                s_cs[i] = cos_sin((double)at * p.freq[i]);
+            }
         }
         __syncthreads();
     }
@@ -178,17 +221,25 @@ __global__ __launch_bounds__(512) void paged_store_kernel(PagedStoreParams p) {
                 d = c * z.y + d * z.x;
                 c = r;
             };
-            if (head < p.n_head + p.n_head_kv) {
+            auto turn64 = [&](float & c, float & d, int i) __attribute__((always_inline)) {
+                const double2 z = s_cd[Q8 ? i : 0];
+                const double a = c, b = d;
+                c = round_odd(a * z.x - b * z.y);
+                d = round_odd(a * z.y + b * z.x);
+            };
+            auto rotate = [&](auto && by) __attribute__((always_inline)) {
                 if (p.rope_mode == 1) {
 #pragma unroll
-                    for (int e = 0; e < E; e++) turn(x[0][e], x[1][e], e0 + e);
+                    for (int e = 0; e < E; e++) by(x[0][e], x[1][e], e0 + e);
                 } else if (p.rope_mode == 0) {
 #pragma unroll
                     for (int h = 0; h < 2; h++)
 #pragma unroll
-                        for (int e = 0; e < E; e += 2) turn(x[h][e], x[h][e + 1], (HALF * h + e0 + e) / 2);
+                        for (int e = 0; e < E; e += 2) by(x[h][e], x[h][e + 1], (HALF * h + e0 + e) / 2);
                 }
-            }
+            };
+            if (head < (Q8 ? p.n_head : p.n_head + p.n_head_kv)) rotate(turn);
+            else if (Q8 && head < p.n_head + p.n_head_kv) rotate(turn64);
             if constexpr (Q8) {
                 if (head >= p.n_head) {
                     // the UH lanes of the head's row find its scale together

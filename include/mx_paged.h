@@ -121,8 +121,8 @@ MX_ATTN_API int32_t mx_paged_store(const mx_paged_desc * desc, const mx_paged_ro
                                    const int32_t * kv_len, const int32_t * cu_q, void * q_out, mx_attn_stream stream);
 
 /*
- * mx_paged_store into pages in 8 bits. The scale of a row is 2^e with e the least (from -127 on) for which its largest finite
- * magnitude, rotated in f32, is at most 448 x 2^e; each element is divided by it, which is exact, and rounded to nearest even. A
+ * mx_paged_store into pages in 8 bits. Keys are rotated in 64 bits. The scale of a row is 2^e with e the least (from -127 on) for which
+ * its largest finite magnitude is at most 448 x 2^e; each element is divided by it, which is exact, and rounded to nearest even. A
  * row of zeros has scale byte 0. An infinity or NaN becomes a NaN code, and leaves the scale to the others. The queries are rounded
  * to desc->dtype.
  */

@@ -1,8 +1,10 @@
 """The paged cache in 8 bits: its kernels against their definitions in 64 bits (e4m3_helpers.py, paged_helpers.py).
 
-The append's codes and scales are held to the definition itself: a value x that the kernel rotates in f32 is off by at most d = 2^-21
-of its two products (none without rotation), and rounding is monotone, so the scale lies between those of the largest magnitude less
-and plus d, and the code between the roundings of x - d and x + d by that scale."""
+The append's codes and scales are held to the definition itself: a key x that the kernel rotates in 64 bits is off by at most d of its
+two products (none without rotation), and rounding is monotone, so the scale lies between those of the largest magnitude less and plus
+d, and the code between the roundings of x - d and x + d by that scale. d: a frequency is within 10 steps of 2^-53 of the power (the
+ladder's 7 products, the power itself, the angle), here and below alike, so the angle of position p within p 2^-48, and the cosine and
+the products within 2^-50."""
 import math
 
 import pytest
@@ -49,8 +51,9 @@ def store_case(device, seed, n_head, n_kv, hd, rows, lens, page, dtype, in_dtype
     pos = torch.cat([torch.arange(L - n, L) for n, L in zip(rows, lens)])[None] if positions is None else positions
     xr = x[:total].double().view(total, n_head + 2 * n_kv, hd)
     ref, mag = rotate(xr[:, :n_head + n_kv], pos, mode, base, axis_pairs or (hd // 2,), restart)
-    off = (0.0 if mode == 2 else 2.0 ** -21) * mag
-    tol = U[dtype] * ref.abs() + off + TINY[dtype]
+    far = pos.abs().double().amax(0)[:, None, None]
+    off = (0.0 if mode == 2 else 2.0 ** -48 * (2 + far)) * mag
+    tol = U[dtype] * ref.abs() + (0.0 if mode == 2 else 2.0 ** -21) * mag + TINY[dtype]
     close(got[:total], ref[:, :n_head].flatten(1), tol[:, :n_head].flatten(1), f"{what} q")
     if tail:
         assert (got[total:] == 7.0).all()

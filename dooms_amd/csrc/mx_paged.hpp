@@ -151,6 +151,7 @@ struct PagedPrefix {
     const int32_t * prefix_len;  // [n_groups]
     int32_t n_groups;
     int32_t room;                // workgroups that the prefixes are cut for
+    int32_t least;               // steps of 64 keys that each of them takes at least
     uint32_t blocks, own_blocks; // workgroups of the prefixes, and behind them those of the sequences' own keys; multiples of 8
     int32_t own_chunk;           // own keys of a workgroup; PagedAttnParams::fixed of them a sequence (the last takes what is left)
     int64_t max_rows;            // rows that `part` has room for

@@ -317,13 +317,13 @@ size_t prefill_bytes(int head_dim) {
 // How the launches run, and where in the workspace their data lies, behind the counters of other calls.
 struct SharedPlan {
     int32_t rows, rt, n_rowtiles;  // of a sequence's own keys, as a decode's
-    int32_t room, chunks, chunk;
+    int32_t room, least, chunks, chunk;
     int64_t blocks, own_blocks;
     int64_t max_rows;              // rows of the prefixes' partials
     size_t group_rows, own_len, info, own_part, part, bytes;  // offsets
 };
 
-int32_t shared_plan(const mx_paged_desc & d, int64_t n_groups, SharedPlan & plan) {
+int32_t shared_plan(const mx_paged_desc & d, bool eight, int64_t n_groups, SharedPlan & plan) {
     if (n_groups < 0 || n_groups > 65535) return fail(MX_ATTN_INVALID_ARGUMENT, "n_groups (%lld) must be in [0, 65535]", (long long)n_groups);
     if ((int64_t)d.n_rows * d.n_head > (int64_t)1 << 26)
         return fail(MX_ATTN_UNSUPPORTED, "%d rows of %d heads are more than one launch holds", d.n_rows, d.n_head);
@@ -345,6 +345,11 @@ int32_t shared_plan(const mx_paged_desc & d, int64_t n_groups, SharedPlan & plan
     // The prefixes are cut for a workgroup on each CU: a second one there walks own keys, and more parts are more to write and join (40 x
     // 2 rows in five groups, Qwen2.5-7B heads in 8 bits, 31.1 us, cut for two 35.4; 192 sequences behind 16384 keys 176 and 179).
     plan.room = kCUs;
+    // Beside many own keys, which take their bytes / 5 TB/s, a part of a prefix may last about 0.6 of that at 1.5 us a step: fewer
+    // workgroups then leave more of the chip to the own keys (64 sequences of 40-900 own keys behind 4096, Llama-3-8B heads, 42.7 us for
+    // 48.6). Half the hint is taken for the mean; at most 16 steps, as it may be far off.
+    const double own_bytes = 0.5 * d.n_seq * std::max(d.max_kv_len, 0) * 2. * d.n_head_kv * d.head_dim * (eight ? 1 : 2);
+    plan.least = (int32_t)std::min(16., std::max(1., own_bytes * 8e-8));
     plan.blocks = (std::max<int64_t>(plan.room, tiles * d.n_head_kv) + 7) / 8 * 8;
     if (plan.blocks + plan.own_blocks > (int64_t)1 << 23)  // threads of a grid's dimension: below 2^32
         return fail(MX_ATTN_UNSUPPORTED, "%d sequences of %d heads are more than one launch holds", d.n_seq, d.n_head);
@@ -543,7 +548,7 @@ MX_ATTN_API int32_t mx_paged_prefill_e4m3(const mx_paged_desc * desc, const mx_p
 MX_ATTN_API size_t mx_paged_decode_shared_workspace_bytes(const mx_paged_desc * desc, int32_t n_groups) {
     if (check_shape(desc) || check_uniform(*desc) || desc->n_seq == 0 || desc->n_rows == 0) return 0;
     SharedPlan plan;
-    return shared_plan(*desc, n_groups, plan) ? 0 : plan.bytes;
+    return shared_plan(*desc, false, n_groups, plan) ? 0 : plan.bytes;
 }
 
 MX_ATTN_API int32_t mx_paged_decode_shared(const mx_paged_desc * desc, const mx_paged_scales * scales, const mx_paged_prefix * prefix,
@@ -559,7 +564,7 @@ MX_ATTN_API int32_t mx_paged_decode_shared(const mx_paged_desc * desc, const mx_
     if (int32_t rc = attn_params(d, scales, q, k, v, table, kv_len, nullptr, out, lse, p)) return rc;
     if (d.n_seq == 0 || d.n_rows == 0) return MX_ATTN_OK;
     SharedPlan plan;
-    if (int32_t rc = shared_plan(d, prefix->n_groups, plan)) return rc;
+    if (int32_t rc = shared_plan(d, scales != nullptr, prefix->n_groups, plan)) return rc;
     if (!workspace || !aligned(workspace, 256))
         return fail(MX_ATTN_INVALID_ARGUMENT, "a 256-byte aligned workspace of %zu bytes is needed", plan.bytes);
     if (ws_bytes < plan.bytes)
@@ -578,6 +583,7 @@ MX_ATTN_API int32_t mx_paged_decode_shared(const mx_paged_desc * desc, const mx_
     p.x.prefix_len = prefix->prefix_len;
     p.x.n_groups = prefix->n_groups;
     p.x.room = plan.room;
+    p.x.least = plan.least;
     p.x.blocks = (uint32_t)plan.blocks;
     p.x.own_blocks = (uint32_t)plan.own_blocks;
     p.x.own_chunk = plan.chunk;

@@ -1,7 +1,8 @@
 // The join of a decode's partials where sequences share prefixes: out = sum e^(m_i - M) o_i / sum e^(m_i - M) l_i over the parts of the
 // prefix and of the sequence's own keys, in order.
 //
-// Bound by the memory and, in small calls, by two round trips: head_dim + 4 floats a row and part. FIGURES
+// Bound by the memory, head_dim + 4 floats a row and part, and in small calls by two round trips: 6144 rows of 12 parts (Llama-3-8B heads,
+// 39 MB) 9.5 us, 2048 of 18 (19 MB) 6.5, 112 of 6 (Qwen2.5-0.5B heads) 3.5 to 4, of which an empty launch is 2.
 //
 //   * A quad of dims to a thread, and kStripes threads to a quad, each with every kStripes-th part: many parts are in flight at once.
 #include "mx_paged.hpp"

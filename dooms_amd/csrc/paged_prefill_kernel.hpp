@@ -20,6 +20,8 @@
 //     step and the probabilities are already the operand of O^T += V^T P^T, whose V^T comes through the transposing LDS read.
 //   * The reference maximum of a row moves only when a block's probabilities would pass 2^8, so the common block computes no
 //     maximum; the mask only where a block crosses the diagonal or the end.
+//   * Pages of e4m3 codes: the loads put codes and scales into LDS, each lane expands the 16 codes that it loaded itself into the tile
+//     that the products read, and the rest is as in 16 bits (the two chunks 767 to 800 us, the 12 prompts 162 to 175, 2 to 5 % more).
 //   * The tiles of all sequences, with their key steps, are one list of units, which the lengths in device memory give; each of the
 //     workgroups that run at once takes an equal range of it, and walks it without a break: the first steps of a tile are loaded
 //     under the last ones of the tile before. A range that ends within a tile leaves a partial (m, l, O) in the workspace, and the
@@ -179,8 +181,9 @@ __device__ __forceinline__ bool odd_values(const PagedAttnParams & p, const Tile
 
 // Rows of R a tile: the tile, and the part of its keys, that workgroup o of the launch computes (b -1: none), with the group's row of
 // the page table in t.b and its first query row in t.row0. Every part takes the same count of steps, the least for which the chip
-// holds all parts of the launch at once, and no fewer than a tile has waves with rows: with fewer, writing the partial and
-// reading it back costs more than the shorter walk saves. The waves of the last workgroups also write what the kernel behind this
+// gives each CU one, and up to 4 no fewer than make 8 parts, as more are more to write, read back and join than the shorter walks save
+// (64 rows, Llama-3-8B heads, 2048 shared keys, 20.4 us, in 16 parts 21.5; 32 x 2 rows, Qwen2.5-7B heads, 1024, 17.2 and 18.2; at least 4
+// always: 512 keys and 16 rows 12.8 for 12.2), nor than x.least. The waves of the last workgroups also write what the kernel behind this
 // one needs to know of each sequence.
 template <int R, int W>
 __device__ __forceinline__ Tile plan_prefix(const PagedAttnParams & p, int wave, uint32_t block, uint32_t blocks, PagedPrefixPart & part) {
@@ -200,7 +203,7 @@ __device__ __forceinline__ Tile plan_prefix(const PagedAttnParams & p, int wave,
         r.rows = shared ? r.n * per_seq : 0;
         r.steps = shared ? (r.keys + kBK - 1) / kBK : 0;
         r.tiles = (r.rows + R - 1) / R;
-        r.least = min(W, (r.rows + 31) / 32);
+        r.least = max(min(4, (r.steps + 7) / 8), x.least);
         return r;
     };
     const Group first = group_at(0);

@@ -179,12 +179,12 @@ __device__ __forceinline__ bool odd_values(const PagedAttnParams & p, const Tile
 
 // ---- shared prefixes: the rows of a group's sequences are one tile list over the keys they share ----
 
-// Rows of R a tile: the tile, and the part of its keys, that workgroup o of the launch computes (b -1: none), with the group's row of
-// the page table in t.b and its first query row in t.row0. Every part takes the same count of steps, the least for which the chip
-// gives each CU one, and up to 4 no fewer than make 8 parts, as more are more to write, read back and join than the shorter walks save
-// (64 rows, Llama-3-8B heads, 2048 shared keys, 20.4 us, in 16 parts 21.5; 32 x 2 rows, Qwen2.5-7B heads, 1024, 17.2 and 18.2; at least 4
-// always: 512 keys and 16 rows 12.8 for 12.2), nor than x.least. The waves of the last workgroups also write what the kernel behind this
-// one needs to know of each sequence.
+// Rows of R a tile: the tile, and the part of its keys, that workgroup `block` of the launch computes (b -1: none), with the group's row
+// of the page table in t.b and its first query row in t.row0. Every part takes the same count of steps, the least for which the
+// prefixes have no more parts than workgroups (x.room); 2 to 4 steps at least where 8 parts suffice, as more are more to write, read back
+// and join than the shorter walks save (64 rows, Llama-3-8B heads, 2048 shared keys, 20.4 us, in 16 parts 21.5; 32 x 2 rows, Qwen2.5-7B
+// heads, 1024, 17.2 and 18.2; but 16 rows behind 512 keys 12.2 in 8 parts, 12.8 in 4); and x.least. The waves of the last workgroups also
+// write what the join needs to know of each sequence.
 template <int R, int W>
 __device__ __forceinline__ Tile plan_prefix(const PagedAttnParams & p, int wave, uint32_t block, uint32_t blocks, PagedPrefixPart & part) {
     const PagedPrefix & x = p.x;

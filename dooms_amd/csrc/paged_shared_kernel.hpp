@@ -8,7 +8,7 @@
 // query rows of a group (bound by the matrix cores and the exponentials), those of the sequences' own keys the decode kernel in chunks
 // (bound by the memory). Those of the prefixes come first, one for a CU; beside it, and behind it, the CU walks own keys (192 sequences
 // of 100-1500 own keys behind 16384, Llama-3-8B heads, f16: 62 GFLOP and 0.70 GB in 160 to 171 us from card to card; the prefixes alone
-// 75, the own keys alone 118, each key of each sequence on its own 1323. 64 sequences of 40-900 behind 4096: 47, 112 unshared. Two
+// 75, the own keys alone 118, each key of each sequence on its own 1323. 64 sequences of 40-900 behind 4096: 40 to 42, 112 unshared. Two
 // launches one behind the other took 214 and 51, the two kinds in turn 207 and 52).
 // Small calls are a chain of round trips: the groups' bounds, the pages' numbers, the keys, then the join (eight answers to 700 shared
 // keys, Qwen2.5-0.5B heads, 11.2 us, of which the join 3.5; a decode that shares nothing takes 7.0 there, as all of it is in the caches).

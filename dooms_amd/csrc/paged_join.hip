@@ -23,7 +23,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnParam
     const int token = (int)(row / p.n_head), h = (int)(row - (int64_t)token * p.n_head);
     const int b = token / p.n_q, t = token - b * p.n_q, g = h / p.group, rr = t * p.group + h - g * p.group;
     const int4 info = p.x.info[b];
-    const int own = p.x.own_len[b], np = info.z, parts = np + (own > 0 ? own_chunks(p, own) : 0);
+    const int own = p.x.own_len[b], np = info.z, parts = own < 0 ? 0 : np + own_chunks(p, own);
     const float * pre = p.x.part + ((int64_t)g * *p.x.rows + info.x + info.w + rr) * (HD + 4);
     const float * mine = p.x.own_part + (((int64_t)b * p.fixed * p.n_head_kv + g) * p.rows + rr) * (HD + 4);
     const int64_t pre_step = (int64_t)info.y * (HD + 4), own_step = (int64_t)p.n_head_kv * p.rows * (HD + 4);

@@ -273,8 +273,11 @@ __device__ __forceinline__ Tile plan_prefix(const PagedAttnParams & p, int wave,
                 first_row += (uint32_t)last;
             }
         }
-        if (own.start == 0) np = 0;
-        else if (!fits) own.len = -1;
+        if (own.start != 0 && !fits) own.len = -1;
+        if (own.start == 0 || !fits) {  // nothing for the join to read: without room the sums above are of no rows that there are
+            np = group_rows = 0;
+            first_row = 0;
+        }
         if ((int)b0 + lane < n_seq) {
             x.own_len[b] = own.len;
             x.info[b] = make_int4((int)first_row, group_rows, np, (b - s0) * per_seq);

@@ -1,0 +1,46 @@
+"""Decode behind shared prefixes where its own plan can go wrong: what the first launch leaves for the join, and sizes at the ends of what
+the call takes."""
+import math
+
+import pytest
+import torch
+
+from dooms_amd import attention as A
+from paged_helpers import attend, close
+from test_paged_gpu import BF16, F16, F32, gen
+from test_paged_shared_gpu import Shared, check
+
+pytestmark = pytest.mark.gpu
+
+
+def left_for_the_join(ws, n_seq):
+    """(rows of a kv head's partials, own keys of each sequence, [first row, rows of a part, parts, own row] of each) in a workspace: they lie
+    behind the counters, each block in whole 256 bytes."""
+    w = ws.view(torch.int32)[A._PAGED_COUNTERS // 4:].cpu()
+    own = 64 + (n_seq + 63) // 64 * 64
+    return int(w[0]), w[64:64 + n_seq], w[own:own + 4 * n_seq].view(n_seq, 4)
+
+
+@pytest.mark.parametrize("n_groups", [200, 20000])
+def test_overlapping_groups_that_have_no_room(device, n_groups):
+    """Groups of all sequences over and over: more parts than the launch has workgroups for, and rows than the workspace. The join is
+    given none of them, and nothing around the workspace is written."""
+    n_seq, n_head, n_kv, hd, keys = 192, 32, 8, 128, 256
+    g = gen(80)
+    s = Shared(g, [(keys, [5 + i % 9 for i in range(n_seq)])], n_kv, hd, 16, F16)
+    q = torch.randn(n_seq, n_head * hd, generator=g).to(F16).to(device)
+    (k, v, table, kv_len, cu, plen), _ = s.to(device)
+    nb = A.paged_shared_workspace_bytes(n_head=n_head, n_head_kv=n_kv, head_dim=hd, n_q=1, n_seq=n_seq, n_groups=n_groups, max_own_len=16)
+    room = torch.zeros(nb + (64 << 20), dtype=torch.uint8, device=device)
+    ws = room[32 << 20:(32 << 20) + nb]
+    many = torch.tensor([0, n_seq] * (n_groups // 2) + [0], dtype=torch.int32, device=device)
+    call = lambda cu, plen: A.paged_decode_shared(q, k, v, table, kv_len, cu, plen, n_head=n_head, max_own_len=16, workspace=ws)[0]
+    call(many, torch.full((n_groups,), keys, dtype=torch.int32, device=device))  # undefined, in bounds
+    rows, _, info = left_for_the_join(ws, n_seq)
+    assert rows == 0  # there was no room
+    assert (info[:, :3] == 0).all()
+    assert not room[:32 << 20].any() and not room[(32 << 20) + nb:].any()
+    ref, _, tol, _ = attend(s, q.cpu(), [1] * n_seq, n_head, hd ** -0.5, True, True, F16)
+    close(call(cu, plen), ref, tol, "the next call")
+    rows, _, info = left_for_the_join(ws, n_seq)
+    assert rows > 0 and (info[:, 2] > 0).all()

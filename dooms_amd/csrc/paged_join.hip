@@ -7,6 +7,8 @@
 //   * A quad of dims to a thread, and kStripes threads to a quad, each with every kStripes-th part: many parts are in flight at once.
 #include "mx_paged.hpp"
 
+#include <algorithm>
+
 namespace mx {
 
 namespace {
@@ -19,7 +21,9 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnParam
     __shared__ float4_t s_o[kStripes][ROWS * QR];
     __shared__ float2 s_ml[kStripes][ROWS * QR];
     const int quad = threadIdx.x % QR, stripe = threadIdx.x / QR % kStripes, r = threadIdx.x / (QR * kStripes);
-    const int64_t total = (int64_t)p.n_rows * p.n_head, row = min((int64_t)blockIdx.x * ROWS + r, total - 1);
+    const int64_t block = blockIdx.x + (int64_t)blockIdx.y * gridDim.x, total = (int64_t)p.n_rows * p.n_head;
+    if (block * ROWS >= total) return;
+    const int64_t row = min(block * ROWS + r, total - 1);
     const int token = (int)(row / p.n_head), h = (int)(row - (int64_t)token * p.n_head);
     const int b = token / p.n_q, t = token - b * p.n_q, g = h / p.group, rr = t * p.group + h - g * p.group;
     const int4 info = p.x.info[b];
@@ -57,7 +61,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnParam
     s_o[stripe][r * QR + quad] = o;
     s_ml[stripe][r * QR + quad] = make_float2(M, l);
     __syncthreads();
-    if (stripe != 0 || (int64_t)blockIdx.x * ROWS + r >= total) return;
+    if (stripe != 0 || block * ROWS + r >= total) return;
     float2 ml[kStripes];
     float top = kNegInf;
 #pragma unroll
@@ -86,8 +90,10 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnParam
 
 template <class T>
 void launch(const PagedAttnParams & p, int head_dim, hipStream_t stream) {
+    constexpr int64_t kMost = 1 << 23;  // workgroups along x: a dimension holds fewer than 2^32 threads
     const int rows = kJoinThreads / (head_dim / 4 * kStripes);
-    const dim3 grid((uint32_t)(((int64_t)p.n_rows * p.n_head + rows - 1) / rows)), block(kJoinThreads);
+    const int64_t blocks = ((int64_t)p.n_rows * p.n_head + rows - 1) / rows;
+    const dim3 grid((uint32_t)std::min(blocks, kMost), (uint32_t)((blocks + kMost - 1) / kMost)), block(kJoinThreads);
     if (head_dim == 64) hipLaunchKernelGGL((paged_join_kernel<64, T>), grid, block, 0, stream, p);
     else if (head_dim == 128) hipLaunchKernelGGL((paged_join_kernel<128, T>), grid, block, 0, stream, p);
     else hipLaunchKernelGGL((paged_join_kernel<256, T>), grid, block, 0, stream, p);

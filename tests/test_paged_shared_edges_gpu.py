@@ -44,3 +44,37 @@ def test_overlapping_groups_that_have_no_room(device, n_groups):
     close(call(cu, plen), ref, tol, "the next call")
     rows, _, info = left_for_the_join(ws, n_seq)
     assert rows > 0 and (info[:, 2] > 0).all()
+
+
+class Sample:
+    """Some sequences of a cache whose sequences all have the same first keys, for `attend`."""
+
+    def __init__(self, k, v, lens):
+        self.k, self.v, self.lens, self.dtype = k.double(), v.double(), lens, k.dtype
+        self.n_head_kv, self.hd = k.shape[1:]
+
+    def keys(self, b):
+        return self.k[:self.lens[b]], self.v[:self.lens[b]]
+
+
+def test_more_rows_than_a_grid_holds_in_a_line(device):
+    """2^24 rows of heads of 256: a row a workgroup of the join, and 2^32 threads."""
+    n_seq = n_head = 4096
+    n_kv, hd, page = 64, 256, 16
+    g = gen(81)
+    kp, vp = (torch.randn(2, page, n_kv, hd, generator=g).to(F16) for _ in range(2))
+    lens = [page + 1 + b % 3 for b in range(n_seq)]
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=device)
+    dg = torch.Generator(device=device).manual_seed(81)
+    q = torch.randn(n_seq, n_head * hd, generator=dg, dtype=F16, device=device)
+    out = torch.full_like(q, math.nan)
+    o, lse = A.paged_decode_shared(q, kp.to(device), vp.to(device), ints([[0, 1]] * n_seq), ints(lens), ints([0, n_seq]), ints([page]), n_head=n_head,
+                                   out=out, want_lse=True, max_own_len=3)
+    assert torch.isfinite(lse).all()
+    for rows in o.split(256):
+        assert torch.isfinite(rows).all()
+    some = [0, 2047, 2048, 4095]
+    c = Sample(kp.flatten(0, 1), vp.flatten(0, 1), [lens[b] for b in some])
+    ref, rlse, tol, ltol = attend(c, q[some].cpu(), [1] * len(some), n_head, hd ** -0.5, True, True, F16)
+    close(o[some], ref, tol, "out")
+    close(lse[some], rlse, ltol, "lse")

@@ -78,3 +78,19 @@ def test_more_rows_than_a_grid_holds_in_a_line(device):
     ref, rlse, tol, ltol = attend(c, q[some].cpu(), [1] * len(some), n_head, hd ** -0.5, True, True, F16)
     close(o[some], ref, tol, "out")
     close(lse[some], rlse, ltol, "lse")
+
+
+@pytest.mark.parametrize("n_q", [1, 3])
+@pytest.mark.parametrize("eight", [False, True])
+def test_a_prefix_longer_than_a_sequence_alone(device, eight, n_q):
+    """A row has to see the whole prefix, of a group of one sequence too."""
+    g = gen(82)
+    s = Shared(g, [(100, [9]), (40, [4, 5]), (300, [n_q - 1 or 1])], 2, 64, 16, F16, eight)
+    q = torch.randn(4 * n_q, 4 * 64, generator=g).to(F16)
+    ref, rlse, tol, ltol = attend(s, q, [n_q] * 4, 4, 0.125, True, True, F16)
+    (k, v, table, kv_len, cu, plen), scales = s.to(device)
+    kv_len[0] = 100 + n_q - 2  # one row sees all but a key
+    o, lse = A.paged_decode_shared(q.to(device), k, v, table, kv_len, cu, plen, n_head=4, n_q=n_q, want_lse=True, scales=scales)
+    assert torch.isnan(o[:n_q]).all() and torch.isnan(lse[:n_q]).all()
+    close(o[n_q:], ref[n_q:], tol[n_q:], "others")
+    close(lse[n_q:], rlse[n_q:], ltol[n_q:], "others' lse")

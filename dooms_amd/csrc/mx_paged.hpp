@@ -206,7 +206,7 @@ __device__ __forceinline__ OwnKeys own_of(const PagedAttnParams & p, bool in, in
     if (len == 0 || !length_ok(p.c, len) || wrong) return OwnKeys{0, len == 0 ? 0 : -1};
     if (!in || keys == 0) return OwnKeys{0, len};
     if (len < keys + (p.causal ? p.n_q - 1 : 0)) return OwnKeys{0, -1};
-    return s1 - s0 > 1 ? OwnKeys{keys, len - (keys & ~15)} : OwnKeys{0, len};
+    return s1 - s0 > 1 ? OwnKeys{keys, len > keys ? len - (keys & ~15) : 0} : OwnKeys{0, len};
 }
 // Of sequence b, the same in every lane: 64 probes a step narrow the groups, whose bounds ascend, to 64.
 __device__ __forceinline__ OwnKeys own_keys(const PagedAttnParams & p, int b) {

@@ -94,3 +94,24 @@ def test_a_prefix_longer_than_a_sequence_alone(device, eight, n_q):
     assert torch.isnan(o[:n_q]).all() and torch.isnan(lse[:n_q]).all()
     close(o[n_q:], ref[n_q:], tol[n_q:], "others")
     close(lse[n_q:], rlse[n_q:], ltol[n_q:], "others' lse")
+
+
+@pytest.mark.parametrize("n_q,causal", [(1, True), (3, False)])
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_no_keys_behind_the_prefix(device, hd, eight, n_q, causal):
+    """Sequences that end with their prefix, at a page's end, a multiple of 16 and neither: what their tables say from there on places none
+    of their keys, and may be no page."""
+    groups = [(64, [0, 9, 0]), (48, [0, 0]), (100, [30, 0, 0, 5]), (7, [0, 3])]
+    check(device, 83, 8, 2, hd, groups, 32, F16, n_q=n_q, causal=causal, eight=eight)
+    g = gen(84)
+    s = Shared(g, groups, 2, hd, 32, F16, eight)
+    q = torch.randn(len(s.lens) * n_q, 8 * hd, generator=g).to(F16)
+    ref, rlse, tol, ltol = attend(s, q, [n_q] * len(s.lens), 8, hd ** -0.5, causal, True, F16)
+    for b in range(len(s.lens)):
+        if s.first[b] != b and s.lens[b] == s.prefix[b]:
+            s.cache.table[b] = -5
+    args, scales = s.to(device)
+    o, lse = A.paged_decode_shared(q.to(device), *args, n_head=8, n_q=n_q, causal=causal, want_lse=True, scales=scales)
+    close(o, ref, tol, "out")
+    close(lse, rlse, ltol, "lse")

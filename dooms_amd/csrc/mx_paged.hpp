@@ -199,14 +199,20 @@ struct PagedAttnParams {
 struct OwnKeys {
     int32_t start, len;
 };
-// Of a sequence of `len` keys in a group of sequences s0 .. s1 - 1 that share `keys` (in: or in none). Every row has to see all of them; a
-// sequence alone in its group shares nothing, nor does one without keys.
+// Whether the prefixes' workgroups compute the `keys` that the n sequences of a group share: of several always, of one alone where they are
+// more than a chunk of own keys. As its own keys, which the hint does not count, its last chunk would walk them (Llama-3-8B heads, a hint
+// of 120: one sequence alone behind 16384 keys 201 us, 23 so; beside 63 that share 4096 keys 227 and 36). Tiles of few rows cost more where
+// nothing is shared at all (32 sequences alone behind 4096 keys each 122 us, 92 as own keys, which is a plain decode's time).
+__device__ __forceinline__ bool prefix_apart(const PagedAttnParams & p, int n, int keys) {
+    return keys > 0 && (n > 1 || (n == 1 && keys > p.x.own_chunk));
+}
+// Of a sequence of `len` keys in a group of sequences s0 .. s1 - 1 that share `keys` (in: or in none). Every row has to see all of them.
 __device__ __forceinline__ OwnKeys own_of(const PagedAttnParams & p, bool in, int s0, int s1, int keys, int len) {
     const bool wrong = in && (keys < 0 || keys > p.c.capacity);
     if (len == 0 || !length_ok(p.c, len) || wrong) return OwnKeys{0, len == 0 ? 0 : -1};
     if (!in || keys == 0) return OwnKeys{0, len};
     if (len < keys + (p.causal ? p.n_q - 1 : 0)) return OwnKeys{0, -1};
-    return s1 - s0 > 1 ? OwnKeys{keys, len > keys ? len - (keys & ~15) : 0} : OwnKeys{0, len};
+    return prefix_apart(p, s1 - s0, keys) ? OwnKeys{keys, len > keys ? len - (keys & ~15) : 0} : OwnKeys{0, len};
 }
 // Of sequence b, the same in every lane: 64 probes a step narrow the groups, whose bounds ascend, to 64.
 __device__ __forceinline__ OwnKeys own_keys(const PagedAttnParams & p, int b) {

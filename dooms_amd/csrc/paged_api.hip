@@ -340,8 +340,8 @@ int32_t shared_plan(const mx_paged_desc & d, bool eight, int64_t n_groups, Share
     plan.chunk = (int32_t)((bound + n * kQuantum - 1) / (n * kQuantum) * kQuantum);
     plan.chunks = (int32_t)((bound + plan.chunk - 1) / plan.chunk);
     plan.own_blocks = (pairs * plan.chunks + 8 * plan.n_rowtiles - 1) / (8 * plan.n_rowtiles) * (8 * plan.n_rowtiles);
-    // groups of one sequence have no part here: at most n_seq / 2 tiles are not full
-    const int64_t rows = (int64_t)d.n_rows * (d.n_head / d.n_head_kv), tiles = rows / kTile + std::min<int64_t>(n_groups, d.n_seq / 2) + 1;
+    // at most one tile of a group is not full
+    const int64_t rows = (int64_t)d.n_rows * (d.n_head / d.n_head_kv), tiles = rows / kTile + std::min<int64_t>(n_groups, d.n_seq) + 1;
     // The prefixes are cut for a workgroup on each CU: a second one there walks own keys, and more parts are more to write and join (40 x
     // 2 rows in five groups, Qwen2.5-7B heads in 8 bits, 31.1 us, cut for two 35.4; 192 sequences behind 16384 keys 176 and 179).
     plan.room = kCUs;

@@ -199,7 +199,7 @@ __device__ __forceinline__ Tile plan_prefix(const PagedAttnParams & p, int wave,
         r.s0 = clamp(x.cu_seq[i]);
         r.n = base + lane < x.n_groups ? max(clamp(x.cu_seq[i + 1]) - r.s0, 0) : 0;
         r.keys = x.prefix_len[i];
-        const bool shared = r.n > 1 && r.keys > 0 && r.keys <= p.c.capacity;
+        const bool shared = prefix_apart(p, r.n, r.keys) && r.keys <= p.c.capacity;
         r.rows = shared ? r.n * per_seq : 0;
         r.steps = shared ? (r.keys + kBK - 1) / kBK : 0;
         r.tiles = (r.rows + R - 1) / R;

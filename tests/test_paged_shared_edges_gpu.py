@@ -115,3 +115,21 @@ def test_no_keys_behind_the_prefix(device, hd, eight, n_q, causal):
     o, lse = A.paged_decode_shared(q.to(device), *args, n_head=8, n_q=n_q, causal=causal, want_lse=True, scales=scales)
     close(o, ref, tol, "out")
     close(lse, rlse, ltol, "lse")
+
+
+@pytest.mark.parametrize("n_q", [1, 3])
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("hd,n_head,n_kv", [(64, 14, 2), (128, 8, 2), (256, 4, 1)])
+def test_long_prefixes_of_one_sequence(device, hd, n_head, n_kv, eight, n_q):
+    """The hint counts the keys behind the prefix, of a sequence alone in its group too: prefixes longer than a chunk of those are computed in
+    parts, as shared ones are."""
+    n = [max(i, n_q) for i in range(12)]
+    groups = [(4000, [9 + n_q]), (300, [n[4], n[9], n[1]]), (1003, [n[1]]), (20, [n[7]]), (0, [n[5]]), (2048, [n[2]])]
+    check(device, 85, n_head, n_kv, hd, groups, 16, BF16, n_q=n_q, eight=eight, own_hint=16)
+    check(device, 86, n_head, n_kv, hd, [(5000, [n[3]])], 64, F16, n_q=n_q, eight=eight, own_hint=16)
+    ws = A.new_workspace(64 << 20, device)
+    check(device, 85, n_head, n_kv, hd, groups, 16, BF16, n_q=n_q, eight=eight, own_hint=16, ws=ws)
+    _, own, info = left_for_the_join(ws, 8)
+    alone = [0, 4, 7]
+    assert (info[alone, 2] >= 8).all() and (own[alone] < 64).all()
+    assert info[5, 2] == 0 and int(own[5]) == 20 + n[7] and info[6, 2] == 0

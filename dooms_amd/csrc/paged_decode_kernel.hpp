@@ -316,26 +316,29 @@ __device__ __forceinline__ void decode_body(const PagedAttnParams & p, DecodeSme
         seg.start = 0;
         key0 = segment(seg, __builtin_amdgcn_readlane(lens, x.b - lens0));
     } else {
-        [[maybe_unused]] int own_start = 0;
-        if (SHARED || p.fixed) {
+        if constexpr (SHARED) {
+            // as many chunks of every sequence's own keys as the hint of those asks for; a sequence has as many of them as it has keys for
+            ch.i = (uint32_t)r / (uint32_t)n_seq;
+            ch.b = r - ch.i * n_seq;
+            const OwnKeys own = own_keys(p, ch.b);
+            ch.len = own.len;
+            ch.keys = p.x.own_chunk;
+            ch.n = own_chunks(p, own.len);
+            if (ch.i >= ch.n) return;
+            seg.start = own.start;
+#pragma unroll
+            for (int i = 0; i < D; i++) ids[i] = read_ids(ch.b, ch.i * ch.keys + i * kStep + kBlock * wave, own.start);
+        } else if (p.fixed) {
             // the host found room for p.fixed chunks of a quantum for every sequence: the chunk follows from the workgroup's
             // number, and its length and first page numbers are one round trip instead of two
             ch.i = (uint32_t)r / (uint32_t)n_seq;
             ch.b = r - ch.i * n_seq;
 #pragma unroll
-            for (int i = 0; i < D && !SHARED; i++) ids[i] = read_ids(ch.b, (ch.i + i) * kStep + kBlock * wave, 0);
-            if constexpr (SHARED) {
-                const OwnKeys own = own_keys(p, ch.b);
-                ch.len = own.len;
-                own_start = own.start;
-                ch.keys = p.x.own_chunk;
-                ch.n = own_chunks(p, own.len);
-            } else {
-                ch.len = __builtin_amdgcn_readfirstlane(p.c.kv_len[ch.b]);
-                ch.keys = kStep;
-                ch.n = min(p.fixed, quanta_of<kStep>(p, ch.len));
-                if (ch.len <= p.whole_keys) ch.n = 1;
-            }
+            for (int i = 0; i < D; i++) ids[i] = read_ids(ch.b, (ch.i + i) * kStep + kBlock * wave, 0);
+            ch.len = __builtin_amdgcn_readfirstlane(p.c.kv_len[ch.b]);
+            ch.keys = kStep;
+            ch.n = min(p.fixed, quanta_of<kStep>(p, ch.len));
+            if (ch.len <= p.whole_keys) ch.n = 1;
             if (ch.i >= ch.n) return;
             ch.ordinal = ch.b;
             ch.slot = ch.b * p.fixed;
@@ -347,12 +350,7 @@ __device__ __forceinline__ void decode_body(const PagedAttnParams & p, DecodeSme
         }
         seg.b = ch.b;
         seg.at = 0;
-        seg.start = 0;
-        if constexpr (SHARED) {
-            seg.start = own_start;
-#pragma unroll
-            for (int i = 0; i < D; i++) ids[i] = read_ids(ch.b, ch.i * ch.keys + i * kStep + kBlock * wave, seg.start);
-        }
+        if constexpr (!SHARED) seg.start = 0;
         seg.L = length_ok(p.c, ch.len) ? ch.len : -1;
         key0 = ch.i * ch.keys;
         seg.k1 = ch.i == ch.n - 1 ? max(seg.L, 0) : key0 + ch.keys;

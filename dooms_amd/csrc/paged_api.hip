@@ -208,16 +208,18 @@ int32_t row_tiles(const mx_paged_desc & d, int32_t & rows, int32_t & rt, int32_t
     return MX_ATTN_OK;
 }
 
-int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
+// say: what is refused becomes the last error.
+int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan, bool say = true) {
+    auto refuse = [&](const char * fmt, auto... args) { return say ? fail(MX_ATTN_UNSUPPORTED, fmt, args...) : MX_ATTN_UNSUPPORTED; };
     if (int32_t rc = row_tiles(d, plan.rows, plan.rt, plan.n_rowtiles)) return rc;
     const int64_t per_seq = (int64_t)d.n_head_kv * plan.n_rowtiles, bound = kv_bound(d);
     auto quanta = [&](int waves) { return (bound + mx::kPagedDecodeBlock * waves - 1) / (mx::kPagedDecodeBlock * waves); };
     if (per_seq > mx::kCounterLines)
-        return fail(MX_ATTN_UNSUPPORTED, "%lld (kv head, row tile) pairs of a sequence are more than one launch holds", (long long)per_seq);
+        return refuse("%lld (kv head, row tile) pairs of a sequence are more than one launch holds", (long long)per_seq);
     const int64_t pairs = d.n_seq * per_seq;
     // the kernel counts the quanta of all sequences in 32 bits
     if (d.n_seq * ((std::max<int64_t>(bound, (int64_t)d.max_pages * d.page_size) + 127) / 128) > (int64_t)1 << 30)
-        return fail(MX_ATTN_UNSUPPORTED, "%d sequences of up to %lld keys are more than one launch holds", d.n_seq,
+        return refuse("%d sequences of up to %lld keys are more than one launch holds", d.n_seq,
                     (long long)std::max<int64_t>(bound, (int64_t)d.max_pages * d.page_size));
     plan.whole = bound <= 128;
     // Ranges where the launch may hold many quanta of 128 keys for every workgroup (64 sequences of 111-8191 keys, Llama-3-8B heads,
@@ -252,7 +254,7 @@ int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan) {
         }
     }
     if (plan.ranges * per_seq * plan.waves > (int64_t)1 << 25)  // threads of a grid's dimension: below 2^32
-        return fail(MX_ATTN_UNSUPPORTED, "%d sequences of %lld (kv head, row tile) pairs are more than one launch holds", d.n_seq, (long long)per_seq);
+        return refuse("%d sequences of %lld (kv head, row tile) pairs are more than one launch holds", d.n_seq, (long long)per_seq);
     // Two partials a range and tile, or two chunks beyond one a sequence; sized for the most of any batch and length, so that one
     // workspace serves all calls of a head shape and row count.
     plan.bytes = plan.whole ? 0 : mx::kCounterBytes + (size_t)(2 * std::max<int64_t>(1, 2 * kCUs / per_seq) * per_seq * plan.rt * (d.head_dim + 4)) * sizeof(float);
@@ -364,9 +366,9 @@ int32_t shared_plan(const mx_paged_desc & d, bool eight, int64_t n_groups, Share
     plan.own_part = plan.info + round(16 * (size_t)d.n_seq);
     plan.part = plan.own_part + round((size_t)own_rows * row_bytes);
     plan.bytes = plan.part + (size_t)plan.max_rows * row_bytes;
-    // without groups the call is a decode
+    // without groups the call is a decode, and refused where that is
     DecodePlan alone;
-    const int32_t rc = decode_plan(d, alone);
+    const int32_t rc = decode_plan(d, alone, n_groups == 0);
     if (rc == MX_ATTN_OK) plan.bytes = std::max(plan.bytes, alone.bytes);
     return n_groups == 0 ? rc : MX_ATTN_OK;
 }

@@ -353,7 +353,7 @@ int32_t shared_plan(const mx_paged_desc & d, bool eight, int64_t n_groups, Share
     const double own_bytes = 0.5 * d.n_seq * std::max(d.max_kv_len, 0) * 2. * d.n_head_kv * d.head_dim * (eight ? 1 : 2);
     plan.least = (int32_t)std::min(16., std::max(1., own_bytes * 8e-8));
     plan.blocks = (std::max<int64_t>(plan.room, tiles * d.n_head_kv) + 7) / 8 * 8;
-    if (plan.blocks + plan.own_blocks > (int64_t)1 << 23)  // threads of a grid's dimension: below 2^32
+    if (plan.blocks + plan.own_blocks >= (int64_t)1 << 24)  // threads of a grid's dimension: below 2^32
         return fail(MX_ATTN_UNSUPPORTED, "%d sequences of %d heads are more than one launch holds", d.n_seq, d.n_head);
     plan.max_rows = std::max<int64_t>((int64_t)plan.room * kTile, (int64_t)d.n_rows * d.n_head);
     // room for the chunks of fewer sequences too, which have more each

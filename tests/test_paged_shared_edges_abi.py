@@ -11,3 +11,12 @@ def test_a_size_that_succeeds_leaves_the_last_error():
     assert "head_dim" in before
     assert size(1) > 0 and _lib.last_error() == before
     assert size(0) == 0 and "more than one launch" in _lib.last_error()
+
+
+def test_as_many_groups_as_sequences():
+    """At the most of both, as with half the groups."""
+    size = lambda n_groups, n_kv: A.paged_shared_workspace_bytes(n_head=n_kv, n_head_kv=n_kv, head_dim=64, n_q=1, n_seq=65535, n_groups=n_groups,
+                                                                 max_own_len=100)
+    for n_kv in (1, 64, 120):
+        assert size(65535, n_kv) >= size(32767, n_kv) > 0
+    assert size(65535, 256) == 0 and "more than one launch" in _lib.last_error()

@@ -209,32 +209,38 @@ __device__ __forceinline__ Tile plan_prefix(const PagedAttnParams & p, int wave,
     const Group first = group_at(0);
     auto at = [&](int base) { return base == 0 ? first : group_at(base); };
     auto parts = [&](const Group & r, int c) { return r.rows ? (r.steps + max(c, r.least) - 1) / max(c, r.least) : 0; };
+    const int room = max(1, p.x.room / p.n_head_kv);
     float sum = 0.f;
-    int longest = 1;
+    int longest = 1, tiles = 0;  // of a kv head, at most 2^29
+    int64_t rows = 0;            // of the partials of a kv head
     for (int base = 0; base < x.n_groups; base += kWave) {
         const Group r = at(base);
         sum += (float)r.tiles * (float)r.steps;
         longest = max(longest, r.steps);
+        tiles = min(tiles + wave_isum(min(r.tiles, 1 << 23)), 1 << 29);
+        rows += read_lane64(wave_scan64(r.rows), 63);
     }
     longest = wave_imax(longest);
-    sum = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_sum(sum))));
-    const int room = max(1, p.x.room / p.n_head_kv);
-    auto count = [&](int c) {  // parts of a kv head, at most 2^30
-        int r = 0;
+    int c = longest, per_kv = tiles;
+    if (tiles > 0 && tiles <= room) {  // else each prefix is one part, and the sums are done: with many groups they are what the plan costs
+        auto count = [&](int c) {  // parts of a kv head, at most 2^30
+            int r = 0;
+            for (int base = 0; base < x.n_groups; base += kWave) {
+                const Group y = at(base);
+                r = min(r + wave_isum((int)min((int64_t)y.tiles * parts(y, c), (int64_t)1 << 23)), 1 << 29);
+            }
+            return r;
+        };
+        sum = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_sum(sum))));
+        c = __builtin_amdgcn_readfirstlane((int)fminf(ceilf(sum / (float)room), (float)longest));
+        c = max(c, (longest + kPagedMaxParts - 1) / kPagedMaxParts);
+        for (int i = 0; c < longest && count(c) > room; i++) c = i < 16 ? min(c + max(1, c / 8), longest) : longest;
+        per_kv = count(c);
+        rows = 0;
         for (int base = 0; base < x.n_groups; base += kWave) {
-            const Group y = at(base);
-            r = min(r + wave_isum((int)min((int64_t)y.tiles * parts(y, c), (int64_t)1 << 23)), 1 << 29);
+            const Group r = at(base);
+            rows += read_lane64(wave_scan64((int64_t)r.rows * parts(r, c)), 63);
         }
-        return r;
-    };
-    int c = __builtin_amdgcn_readfirstlane((int)fminf(ceilf(sum / (float)room), (float)longest));
-    c = max(c, (longest + kPagedMaxParts - 1) / kPagedMaxParts);
-    for (int i = 0; c < longest && count(c) > room; i++) c = i < 16 ? min(c + max(1, c / 8), longest) : longest;
-    const int per_kv = count(c);
-    int64_t rows = 0;  // of the partials of a kv head
-    for (int base = 0; base < x.n_groups; base += kWave) {
-        const Group r = at(base);
-        rows += read_lane64(wave_scan64((int64_t)r.rows * parts(r, c)), 63);
     }
     // only ranges of cu_seq that overlap have more parts or rows than the launch
     const int64_t all = (int64_t)per_kv * p.n_head_kv;

@@ -133,3 +133,12 @@ def test_long_prefixes_of_one_sequence(device, hd, n_head, n_kv, eight, n_q):
     alone = [0, 4, 7]
     assert (info[alone, 2] >= 8).all() and (own[alone] < 64).all()
     assert info[5, 2] == 0 and int(own[5]) == 20 + n[7] and info[6, 2] == 0
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_more_groups_than_workgroups(device, eight):
+    """Prefixes of which none is cut into parts, as there are more of them than a kv head has workgroups: of two sequences and of one, and
+    under more kv heads than the chip has CUs."""
+    many = [(60 + 13 * i % 300, [1 + (i + j) % 20 for j in range(1 + i % 2)]) for i in range(300)]
+    check(device, 87, 4, 2, 64, many, 16, F16, eight=eight, own_hint=20)
+    check(device, 88, 600, 300, 64, [(200, [3, 5]), (70, [2, 4, 1]), (500, [9])], 16, F16, eight=eight, own_hint=9)

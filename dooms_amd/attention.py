@@ -521,7 +521,7 @@ def paged_decode_shared(q, k_pages, v_pages, page_table, kv_len, cu_seq, prefix_
     """mx_paged_decode_shared: paged_decode of sequences that come in groups which share their first keys. cu_seq int32 [groups + 1]
     and prefix_len int32 [groups] on the device: sequences cu_seq[g] .. cu_seq[g + 1] - 1 have the first prefix_len[g] keys in common,
     in the pages that the group's first sequence has for them; kv_len counts them too, and every new row has to see them all. The
-    shared keys are read once for a group. max_own_len: the most keys of a sequence behind its prefix, for the plan. workspace:
+    shared keys are read once for a group. max_own_len: the most keys of a sequence behind its prefix (all, of one in no group), for the plan. workspace:
     paged_shared_workspace_bytes from new_workspace. Everything else as paged_decode. Returns (out, lse or None)."""
     if q.dim() == 2 and page_table.dim() == 2 and q.shape[0] != page_table.shape[0] * n_q:
         raise ValueError(f"q has {q.shape[0]} rows, not {n_q} for each of {page_table.shape[0]} sequences")

@@ -225,7 +225,8 @@ int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan, bool say = true)
     // Ranges where the launch may hold many quanta of 128 keys for every workgroup (64 sequences of 111-8191 keys, Llama-3-8B heads,
     // 182 us against 227 of chunks), chunks below, where finding the range and joining over it cost more than its balance saves
     // (64 of 100-2000, Qwen2.5-0.5B heads, 13.8 of chunks against 17.1; equal at 32 of 111-2000, Llama-3-8B heads, 33.7). Tiles of
-    // more rows join slower, so their bound is higher (32 rows, 32 sequences of 201-5999, 52 against 67).
+    // more rows join slower, so their bound is higher (32 rows, 32 sequences of 201-5999, 52 against 67). All bounds here were measured
+    // over pages of 16 bits, and serve those of codes too.
     plan.by_ranges = d.n_seq > 1 && pairs * quanta(4) > (plan.rt <= 8 ? 16 : plan.rt == 16 ? 32 : 64) * kCUs;
     plan.fixed = 0;
     plan.whole_keys = 0;

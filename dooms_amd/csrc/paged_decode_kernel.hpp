@@ -20,8 +20,8 @@
 //   * Pages of e4m3 codes: the same, with half the bytes in flight and each row's codes expanded by its scale on their way to LDS
 //     (v_cvt_scalef32_pk, two codes an instruction), so that the products are those of 16 bits. 64 sequences of 0.1k-8k keys: 549 MB
 //     in 103 to 113 us from card to card, 4.9 to 5.3 TB/s (181 in 16 bits), 82 of one page that stays in the caches; where the heads of a
-//     page lie outermost, rows of 128 bytes are 2 KB in a row and it takes 103 for 114. 32768 keys 21.5 to 23.4 (28.6 in 16 bits), 513
-//     keys of Qwen2.5-0.5B heads 6.5 to 6.95 (6.4).
+//     page lie outermost, rows of 128 bytes are 2 KB in a row and it takes 103 for 114. 32768 keys 22.0 to 23.4 (27.9 in 16 bits), 513
+//     keys of Qwen2.5-0.5B heads 6.5 to 6.95 (6.3).
 //   * Parts of a sequence publish their partials with device-scope stores and count themselves in; the last one of a tile joins them
 //     in order (the result does not depend on which was last) and resets the counter.
 #pragma once

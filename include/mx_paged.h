@@ -17,7 +17,9 @@
  * Arithmetic of the attention calls. Scores, running maxima and sums, accumulators and joins are f32. The probabilities are
  * rounded to the pages' type for their product with the values, as the matrix cores take both operands in one type: half a step
  * of that type on each key's weight, with row_dtype MX_ATTN_F32 too, whose rows are only stored wider. The output is rounded once.
- * A probability that rounds to 0 (in f16 below 2^-25 of the largest) makes NaN of an infinite value at its key.
+ * A probability that rounds to 0 (in f16 below 2^-25 of the largest) makes NaN of an infinite value at its key. Prompts, and the
+ * prefixes of mx_paged_decode_shared, take scores below 2^27 in magnitude: from about 2^30 on (f16; 2^31 in bf16) a row is NaN. The
+ * decodes, and a sequence's own keys, take what f32 holds.
  *
  * Device metadata cannot be checked by the host, and no entry of it makes a call read or write outside the pool:
  *   - kv_len outside [0, max_pages * page_size] makes that sequence's outputs NaN, a page outside [0, n_pages) the rows that
@@ -173,21 +175,23 @@ typedef struct mx_paged_prefix {
 
 /*
  * mx_paged_decode of sequences that share prefixes: the results of mx_paged_decode within its rounding, while each shared key is read
- * once for all rows of its group instead of once a sequence. Two launches: the prefixes, for all query rows of a group on the matrix
- * cores together, then each sequence's own keys, with which the prefix's partials are joined.
+ * once for all rows of its group instead of once a sequence. Two launches: one for the partials of the prefixes, of all query rows of a
+ * group on the matrix cores together, and of each sequence's own keys; one that joins them.
  *
  * The keys of a prefix are found through the page table of its group's first sequence, also where that one has 0 keys; the other sequences' entries for whole
  * pages of it are not read, and rows of it in a page that holds keys of a sequence's own (where the prefix ends within a page) are
- * never used. kv_len counts the prefix's keys too. Every row has to see the whole prefix: a sequence with fewer keys than the
- * prefix (causal: than the prefix and all but one of its new rows), but not 0, or with a prefix_len outside
- * [0, max_pages * page_size], gets NaN; one of 0 keys gets zeros, and takes nothing from its group. cu_seq entries are clamped to
- * [0, n_seq]; what ranges that run backwards or overlap compute is undefined.
+ * never used. kv_len counts the prefix's keys too. Every row has to see the whole prefix, also where a sequence is alone in its group: one
+ * with fewer keys than the prefix (causal: than the prefix and all but one of its new rows), but not 0, or with a prefix_len outside
+ * [0, max_pages * page_size], gets NaN; one of 0 keys gets zeros, and takes nothing from its group; one that ends with its prefix has no
+ * keys of its own. cu_seq entries are clamped to [0, n_seq]; what ranges that run backwards or overlap compute is undefined, within the
+ * buffers.
  *
  *   scales      of pages in 8 bits, or NULL: pages of dtype
  *   workspace   as mx_paged_decode's, at least mx_paged_decode_shared_workspace_bytes(desc, n_groups) bytes, never NULL where there
  *               is work to do. Nothing is kept in it between calls.
  *
- * desc->max_kv_len counts the keys of a sequence behind its prefix here (0: unknown). n_rows * n_head at most 2^26.
+ * desc->max_kv_len counts the keys of a sequence behind its prefix here (0: unknown); a sequence of no group has no prefix, and all its
+ * keys count. n_rows * n_head at most 2^26. Every workgroup reads all groups: up to a hundred cost little, thousands milliseconds.
  */
 MX_ATTN_API int32_t mx_paged_decode_shared(const mx_paged_desc * desc, const mx_paged_scales * scales, const mx_paged_prefix * prefix,
                                            const void * q, const void * k, const void * v, const int32_t * table,

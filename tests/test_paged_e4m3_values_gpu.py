@@ -75,3 +75,30 @@ def test_keys(device, kind, dtype):
     bad = ~(err <= tol) & fine[:, None]
     assert not bad.any(), [(int(b), int(c), float(got[b, c]), float(want[b, c])) for b, c in torch.nonzero(bad)[:8]]
     assert torch.isnan(got[255]).all()
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("dtype,power_of_two", [(F16, 30), (BF16, 100)])
+def test_decode_of_large_scores(device, dtype, power_of_two, eight):
+    """Scores apart by more than any weight: the output is the value of the largest one, in the first block of keys, a later one and the
+    last. The dims of a row of keys are one number, those
+    of the query 2 to half the power."""
+    top = 2.0 ** (power_of_two - power_of_two // 2)
+    g = torch.Generator().manual_seed(90)
+    for at in (3, 41, 69):
+        k = torch.zeros(5, PAGE, 1, 64, dtype=torch.float64)
+        k.view(80, 64)[:] = (-top * (1 + torch.arange(80) % 7) / 64)[:, None]
+        k.view(80, 64)[at] = top * 7 / 8
+        v = torch.randint(1, 9, (5, PAGE, 1, 64), generator=g).double()
+        table = torch.arange(5, dtype=torch.int32, device=device)[None]
+        kv_len = torch.tensor([70], dtype=torch.int32, device=device)
+        q = torch.full((1, 64), 2.0 ** (power_of_two // 2) * 0.75, dtype=dtype, device=device)
+        scales = None
+        if eight:
+            e = int(math.log2(top)) + 1  # codes of a row below 1
+            scales = [torch.full((5, 1, PAGE), b, dtype=torch.uint8, device=device).view(E8M0) for b in (127 + e, 127)]
+            pages = [(k / 2.0 ** e).to(E4M3), v.to(E4M3)]
+        else:
+            pages = [k.to(dtype), v.to(dtype)]
+        o, _ = A.paged_decode(q, *(t.to(device) for t in pages), table, kv_len, n_head=1, scale=1.0, scales=scales)
+        assert torch.equal(o[0].double().cpu(), v.view(80, 64)[at]), at

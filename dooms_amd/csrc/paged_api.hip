@@ -220,7 +220,7 @@ int32_t decode_plan(const mx_paged_desc & d, DecodePlan & plan, bool say = true)
     // the kernel counts the quanta of all sequences in 32 bits
     if (d.n_seq * ((std::max<int64_t>(bound, (int64_t)d.max_pages * d.page_size) + 127) / 128) > (int64_t)1 << 30)
         return refuse("%d sequences of up to %lld keys are more than one launch holds", d.n_seq,
-                    (long long)std::max<int64_t>(bound, (int64_t)d.max_pages * d.page_size));
+                      (long long)std::max<int64_t>(bound, (int64_t)d.max_pages * d.page_size));
     plan.whole = bound <= 128;
     // Ranges where the launch may hold many quanta of 128 keys for every workgroup (64 sequences of 111-8191 keys, Llama-3-8B heads,
     // 182 us against 227 of chunks), chunks below, where finding the range and joining over it cost more than its balance saves
